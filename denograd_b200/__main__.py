@@ -1,6 +1,7 @@
 """Command line: python -m denograd_b200 <generate | info | trace> ...
 
   generate  continue a prompt of token ids:  --model DIR --tokens 1,2,3 --max-new 32 [--temperature T --top-k K --top-p P]
+            [--kv-dtype int8|fp8: the KV cache of a Llama model in 8 bits]
   info      what a model folder holds, without touching the GPU
   trace     replay a trace of token ids (same options as bin/trace_run)
 """
@@ -26,7 +27,8 @@ def generate(a) -> int:
         raise SystemExit("an empty prompt: give --tokens or --text")
     rand.manual_seed(a.seed)
     llm = registry.load(a.model, a.dtype, max_context=a.max_context or len(prompt) + a.max_new, temperature=a.temperature, top_k=a.top_k,
-                        top_p=a.top_p, alpha_f=a.alpha_f, alpha_p=a.alpha_p)
+                        top_p=a.top_p, alpha_f=a.alpha_f, alpha_p=a.alpha_p,
+                        **({} if a.kv_dtype == "float16" else {"kv_dtype": a.kv_dtype}))
     out = []
     if a.temperature < 1e-6:
         out = llm.generate(np.array(prompt, np.int32), a.max_new, batched=True)[0].tolist()
@@ -63,6 +65,7 @@ def main(argv=None) -> int:
     g.add_argument("--tokenizer", default="")
     g.add_argument("--max-new", type=int, default=32)
     g.add_argument("--max-context", type=int, default=0)
+    g.add_argument("--kv-dtype", default="float16", choices=["float16", "int8", "fp8"], help="element type of a Llama model's KV cache")
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--top-k", type=int, default=0)

@@ -1,0 +1,242 @@
+// The 8-bit KV cache: the object, storing new rows (RoPE, quantisation) and reading them back.  What attends to it: kvquant_attn.cu.
+#include <stdlib.h>
+#include <string.h>
+
+#include "kvquant.cuh"
+
+// ------------------------------------------------------------------------------------------------ the object
+JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t format, jg_kvq** out) {
+  JG_ENTER(dev);
+  JG_REQUIRE(desc != nullptr && out != nullptr, "kvq_create: null argument");
+  const jg_kvcache_desc& d = *desc;
+  JG_REQUIRE(format == JG_KVQ_INT8 || format == JG_KVQ_E4M3, "kvq_create: unknown format %d", format);
+  JG_REQUIRE(d.n_layers > 0 && d.n_kv_heads > 0 && d.n_pages > 0 && d.max_batch > 0 && d.max_pages_per_seq > 0 && d.n_heads > 0,
+             "kvq_create: non-positive dimension");
+  JG_REQUIRE(d.head_dim == 64 || d.head_dim == 128, "kvq_create: head_dim %d not supported (64 or 128)", d.head_dim);
+  JG_REQUIRE(d.page_size == 16 || d.page_size == 32 || d.page_size == 64, "kvq_create: page_size %d not in {16,32,64}", d.page_size);
+  JG_REQUIRE(d.n_heads % d.n_kv_heads == 0 && d.n_heads / d.n_kv_heads <= 8,
+             "kvq_create: %d query heads for %d kv heads: 1 to 8 to each are supported", d.n_heads, d.n_kv_heads);
+  JG_REQUIRE(d.n_heads <= 4096, "kvq_create: %d heads", d.n_heads);
+  JG_REQUIRE((long long)d.max_batch * d.max_pages_per_seq <= 0x7fffffffLL && (long long)d.max_pages_per_seq * d.page_size <= 0x7fffffffLL,
+             "kvq_create: block table too large");
+  JG_REQUIRE(!dev->capturing, "kvq_create: a graph capture is in progress");
+  jg_kvq* kv = new jg_kvq();
+  memset(kv, 0, sizeof(*kv));
+  kv->dev = dev;
+  kv->d = d;
+  kv->format = format;
+  kv->max_ctx = d.max_pages_per_seq * d.page_size;
+  kv->layer_rows = (size_t)d.n_pages * d.n_kv_heads * d.page_size;
+  const size_t rows = kv->layer_rows * d.n_layers, codes = rows * d.head_dim, table = (size_t)d.max_batch * d.max_pages_per_seq * sizeof(int32_t);
+  cudaError_t e = cudaMalloc(&kv->k_codes, codes);
+  if (e == cudaSuccess) e = cudaMalloc(&kv->v_codes, codes);
+  if (e == cudaSuccess) e = cudaMalloc(&kv->scales, rows * sizeof(__half2));
+  if (e == cudaSuccess) e = cudaMalloc(&kv->block_table, table);
+  int32_t* ids = (int32_t*)malloc(table);
+  if (e == cudaSuccess && ids == nullptr) e = cudaErrorMemoryAllocation;
+  if (e == cudaSuccess) {
+    // zeros, as a new fp16 cache has (positions nobody wrote are read behind masks); row b of the block table owns pages
+    // [b * max_pages_per_seq, ...) as far as the pool reaches
+    for (int b = 0; b < d.max_batch; b++)
+      for (int i = 0; i < d.max_pages_per_seq; i++) {
+        const long long pg = (long long)b * d.max_pages_per_seq + i;
+        ids[(size_t)b * d.max_pages_per_seq + i] = (int32_t)(pg < d.n_pages ? pg : d.n_pages - 1);
+      }
+    e = cudaMemsetAsync(kv->k_codes, 0, codes, dev->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->v_codes, 0, codes, dev->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->scales, 0, rows * sizeof(__half2), dev->stream);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(kv->block_table, ids, table, cudaMemcpyHostToDevice, dev->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
+  }
+  free(ids);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    jg_kvq_destroy(kv);
+    return jg_cuda_fail(e, "kvq_create", __FILE__, __LINE__);
+  }
+  kv->bytes = 2 * codes + rows * sizeof(__half2) + table;
+  *out = kv;
+  return JG_OK;
+}
+
+static void kvq_destroy_now(void* p) { jg_kvq_destroy((jg_kvq*)p); }
+
+JG_API int jg_kvq_destroy(jg_kvq* kv) {
+  if (!kv) return JG_OK;
+  if (g_jg_capturing > 0) { jg_defer(kvq_destroy_now, kv); return JG_OK; }
+  cudaSetDevice(kv->dev->ordinal);
+  cudaStreamSynchronize(kv->dev->stream);
+  cudaFree(kv->k_codes); cudaFree(kv->v_codes); cudaFree(kv->scales); cudaFree(kv->block_table);
+  delete kv;
+  return JG_OK;
+}
+
+JG_API int jg_kvq_set_block_table(jg_kvq* kv, const int32_t* table) {
+  JG_REQUIRE(kv != nullptr && table != nullptr, "kvq_set_block_table: null argument");
+  JG_ENTER(kv->dev);
+  JG_REQUIRE(!kv->dev->capturing, "kvq_set_block_table: a graph capture is in progress");
+  const size_t n = (size_t)kv->d.max_batch * kv->d.max_pages_per_seq;
+  for (size_t i = 0; i < n; i++)
+    JG_REQUIRE(table[i] >= 0 && table[i] < kv->d.n_pages, "kvq_set_block_table: entry %zu = %d outside the pool of %d pages", i, table[i], kv->d.n_pages);
+  JG_CUDA(cudaMemcpyAsync(kv->block_table, table, n * sizeof(int32_t), cudaMemcpyHostToDevice, kv->dev->stream));
+  JG_CUDA(cudaStreamSynchronize(kv->dev->stream));
+  return JG_OK;
+}
+
+JG_API int jg_kvq_bytes(jg_kvq* kv, uint64_t* out) {
+  JG_REQUIRE(kv != nullptr && out != nullptr, "kvq_bytes: null argument");
+  *out = kv->bytes;
+  return JG_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ storing
+struct KvqWriteArgs {
+  KvqLayer c;
+  __half* q_out;
+  const __half* qkv;
+  const __half* table;  // [table_rows][hd/2][2], or null
+  const int32_t* pos;
+  const int32_t* seq;
+  int ldq, ldx, table_rows, R, H;
+};
+
+constexpr int KW_THREADS = 256;
+
+// A thread for each eight values of a row's Q heads, and of its K heads together with V.
+template <int FMT, int HD>
+__global__ void __launch_bounds__(KW_THREADS) kvq_write_kernel(const KvqWriteArgs a) {
+  constexpr int LPR = HD / 8;
+  pdl_launch();
+  pdl_wait();
+  const unsigned per_row = (unsigned)(a.H + a.c.G) * LPR, at = blockIdx.x * (unsigned)KW_THREADS + threadIdx.x;
+  const unsigned row = at / per_row;
+  const int piece = (int)(at - row * per_row), head = piece / LPR, sub = piece % LPR;
+  int t = -1;
+  const int32_t* bt_row = nullptr;
+  if (row < (unsigned)a.R) {
+    const int sq = a.seq ? a.seq[row] : (int)row;
+    t = a.pos[row];
+    if ((unsigned)sq >= (unsigned)a.c.n_seq || (unsigned)t >= (unsigned)a.c.max_ctx || (a.table && t >= a.table_rows)) t = -1;
+    else bt_row = a.c.block_table + (size_t)sq * a.c.max_pages;
+  }
+  const __half* x = a.qkv + (size_t)row * a.ldx + (size_t)head * HD + sub * 8;
+  const bool live = t >= 0, is_q = head < a.H;
+  uint4 v = make_uint4(0, 0, 0, 0), w = v;
+  if (live && (!is_q || a.q_out)) {
+    v = ld_128(x);
+    if (!is_q) w = ld_128(x + (size_t)a.c.G * HD);
+    if (a.table) v = kvq_rotate(v, ld_128(a.table + (size_t)t * HD + sub * 8));
+    if (is_q) *reinterpret_cast<uint4*>(a.q_out + (size_t)row * a.ldq + (size_t)head * HD + sub * 8) = v;
+  }
+  if (__all_sync(0xffffffffu, is_q || !live)) return;
+  uint2 kc, vc;
+  __half2 scale;
+  kvq_quantise<FMT, LPR>(v, w, kc, vc, scale);
+  if (live && !is_q) {
+    const size_t to = kvq_row(a.c, bt_row, t, head - a.H);
+    *reinterpret_cast<uint2*>(a.c.k + to * HD + sub * 8) = kc;
+    *reinterpret_cast<uint2*>(a.c.v + to * HD + sub * 8) = vc;
+    if (sub == 0) a.c.scales[to] = scale;
+  }
+}
+
+JG_API int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, int32_t ldq, uint64_t qkv, int32_t ldx, uint64_t table,
+                        int32_t table_rows, uint64_t pos, uint64_t seq, int32_t R, int32_t H) {
+  JG_ENTER(dev);
+  JG_REQUIRE(kv != nullptr && kv->dev == dev, "kvq_write: cache belongs to another device");
+  JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_write: layer %d out of range", layer);
+  const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
+  JG_REQUIRE(H == kv->d.n_heads, "kvq_write: H=%d does not match the cache (n_heads %d)", H, kv->d.n_heads);
+  JG_REQUIRE(R > 0 && (seq != 0 || R <= kv->d.max_batch), "kvq_write: R=%d rows for %d slots", R, kv->d.max_batch);
+  JG_REQUIRE(ldx >= (H + 2 * G) * hd && ldx % 8 == 0, "kvq_write: rows of %d elements are no multiple of 8 or too short", ldx);
+  JG_REQUIRE(q_out == 0 || (ldq >= H * hd && ldq % 8 == 0), "kvq_write: rows of q_out of %d elements are no multiple of 8 or too short", ldq);
+  JG_REQUIRE(jg_aligned(qkv, 16) && q_out % 16 == 0 && table % 16 == 0 && jg_aligned(pos, 4) && seq % 4 == 0, "kvq_write: null or misaligned pointer");
+  JG_REQUIRE(table == 0 || table_rows > 0, "kvq_write: empty RoPE table");
+  const unsigned long long pieces = (unsigned long long)R * (H + G) * (hd / 8);
+  JG_REQUIRE(pieces <= 0xffffff00ull, "kvq_write: %d rows are too many for one call", R);
+  KvqWriteArgs a = {};
+  a.c = kvq_layer(kv, layer);
+  a.q_out = (__half*)q_out; a.qkv = (const __half*)qkv; a.table = (const __half*)table;
+  a.pos = (const int32_t*)pos; a.seq = (const int32_t*)seq;
+  a.ldq = ldq; a.ldx = ldx; a.table_rows = table_rows; a.R = R; a.H = H;
+  const dim3 grid((unsigned)((pieces + KW_THREADS - 1) / KW_THREADS)), block(KW_THREADS);
+  if (kv->format == JG_KVQ_INT8)
+    return hd == 64 ? jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_INT8, 64>, grid, block, 0, a)
+                    : jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_INT8, 128>, grid, block, 0, a);
+  return hd == 64 ? jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_E4M3, 64>, grid, block, 0, a)
+                  : jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_E4M3, 128>, grid, block, 0, a);
+}
+
+// ------------------------------------------------------------------------------------------------ reading back
+struct KvqReadArgs {
+  KvqLayer c;
+  __half* k;
+  __half* v;
+  const int32_t* pos;
+  const int32_t* count;
+  const int32_t* first;
+  const int32_t* seq;
+  int ld, R, max_count, step;
+};
+
+constexpr int KR_THREADS = 256;
+
+// A thread for each eight values of K and the eight of V beside them.
+template <int FMT, int HD>
+__global__ void __launch_bounds__(KR_THREADS) kvq_read_kernel(const KvqReadArgs a) {
+  constexpr int LPR = HD / 8;
+  pdl_launch();
+  pdl_wait();
+  const int b = blockIdx.y;
+  const unsigned per_row = (unsigned)a.c.G * LPR, at = blockIdx.x * (unsigned)KR_THREADS + threadIdx.x, i = at / per_row;
+  const int n = a.count ? min(a.count[b], a.max_count) : a.max_count;
+  if ((long long)i >= n) return;
+  const int piece = (int)(at - i * per_row), g = piece / LPR, sub = piece % LPR;
+  const long long row = (long long)(a.first ? a.first[b] : b) + (long long)i * a.step, t = (long long)a.pos[b] + i;
+  if (row < 0 || row >= a.R) return;
+  const int sq = a.seq ? a.seq[b] : b;
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  if ((unsigned)sq < (unsigned)a.c.n_seq && t >= 0 && t < a.c.max_ctx) {
+    const size_t from = kvq_row(a.c, a.c.block_table + (size_t)sq * a.c.max_pages, (int)t, g);
+    const uint2 kc = *reinterpret_cast<const uint2*>(a.c.k + from * HD + sub * 8), vc = *reinterpret_cast<const uint2*>(a.c.v + from * HD + sub * 8);
+    const __half2 scale = a.c.scales[from];
+    const __half2 sk = __low2half2(scale), sv = __hisnan(__low2half(scale)) ? sk : __high2half2(scale);
+    __half2 h[4], w[4];
+    kvq_widen<FMT>(kc.x, h[0], h[1]);
+    kvq_widen<FMT>(kc.y, h[2], h[3]);
+    kvq_widen<FMT>(vc.x, w[0], w[1]);
+    kvq_widen<FMT>(vc.y, w[2], w[3]);
+#pragma unroll
+    for (int j = 0; j < 4; j++) { h[j] = __hmul2_rn(h[j], sk); w[j] = __hmul2_rn(w[j], sv); }
+    k = *reinterpret_cast<const uint4*>(h);
+    v = *reinterpret_cast<const uint4*>(w);
+  }
+  const size_t to = (size_t)row * a.ld + (size_t)g * HD + sub * 8;
+  *reinterpret_cast<uint4*>(a.k + to) = k;
+  *reinterpret_cast<uint4*>(a.v + to) = v;
+}
+
+JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint64_t v, int32_t ld, int32_t R, uint64_t pos, uint64_t count,
+                       uint64_t first, uint64_t seq, int32_t B, int32_t max_count, int32_t step) {
+  JG_ENTER(dev);
+  JG_REQUIRE(kv != nullptr && kv->dev == dev, "kvq_read: cache belongs to another device");
+  JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_read: layer %d out of range", layer);
+  const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
+  JG_REQUIRE(R > 0 && max_count > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
+             max_count, R, kv->d.max_batch);
+  JG_REQUIRE(ld >= G * hd && ld % 8 == 0, "kvq_read: rows of %d elements are no multiple of 8 or too short", ld);
+  JG_REQUIRE(jg_aligned(k, 16) && jg_aligned(v, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_read: null or misaligned pointer");
+  const unsigned long long pieces = (unsigned long long)max_count * G * (hd / 8);
+  JG_REQUIRE(pieces <= 0xffffff00ull, "kvq_read: %d positions are too many for one call", max_count);
+  KvqReadArgs a = {};
+  a.c = kvq_layer(kv, layer);
+  a.k = (__half*)k; a.v = (__half*)v;
+  a.pos = (const int32_t*)pos; a.count = (const int32_t*)count; a.first = (const int32_t*)first; a.seq = (const int32_t*)seq;
+  a.ld = ld; a.R = R; a.max_count = max_count; a.step = step;
+  const dim3 grid((unsigned)((pieces + KR_THREADS - 1) / KR_THREADS), (unsigned)B), block(KR_THREADS);
+  if (kv->format == JG_KVQ_INT8)
+    return hd == 64 ? jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_INT8, 64>, grid, block, 0, a)
+                    : jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_INT8, 128>, grid, block, 0, a);
+  return hd == 64 ? jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_E4M3, 64>, grid, block, 0, a)
+                  : jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_E4M3, 128>, grid, block, 0, a);
+}

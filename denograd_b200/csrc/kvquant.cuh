@@ -1,0 +1,161 @@
+// The paged KV cache in 8 bits: the object, the two code formats, and what the kernels that write and read it share.
+//
+// K and V of a (position, kv head) are rows of hd codes with a scale each, value = code * scale:
+//   int8   scale = max|x| / 127 rounded up to 4 significant bits (to a multiple of 2^-24 below 2^-21), code = rint(x / scale)
+//   e4m3   scale = the least 2^e with max|x| / 2^e <= 448, e >= -15,                                  code = e4m3(x / scale)
+// A code has at most 7 significant bits (int8) or 4 (e4m3), so code * scale has at most 11 and is an fp16 number: what
+// attends to the cache multiplies fp16 values, exact, and needs no scale inside a sum.  Rounding int8's scale up costs up to an
+// eighth of a step (0.5 dB), which is the price of that.  The quotients are computed in 32 bits and never round across a border:
+// max|x| has 11 significant bits, so a quotient that is not on a border is at least 2^-12 of itself away from it.
+// A value beyond 65504 (rounded up from just below) becomes the next lower code.
+// A row with a NaN or an infinity in its K or V has no codes that could stand for it: its K scale is NaN and the V row zero.
+// Scores against it are NaN, so every query that sees the position becomes NaN, and no other: a masked NaN is replaced, but a
+// masked V would still be multiplied by a weight of 0.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+struct jg_kvq {
+  jg_dev* dev;
+  jg_kvcache_desc d;
+  int format;
+  uint8_t* k_codes;  // [L][n_pages][G][page][hd]
+  uint8_t* v_codes;
+  __half2* scales;   // [L][n_pages][G][page], (K, V)
+  int32_t* block_table;
+  int max_ctx;
+  size_t layer_rows;  // (position, kv head) rows of a layer
+  uint64_t bytes;
+};
+
+// What the kernels see of one layer.
+struct KvqLayer {
+  uint8_t* k;
+  uint8_t* v;
+  __half2* scales;
+  const int32_t* block_table;
+  int G, page_shift, max_pages, n_seq, max_ctx;
+};
+
+static inline KvqLayer kvq_layer(const jg_kvq* kv, int layer) {
+  KvqLayer l;
+  const size_t rows = kv->layer_rows * layer;
+  l.k = kv->k_codes + rows * kv->d.head_dim;
+  l.v = kv->v_codes + rows * kv->d.head_dim;
+  l.scales = kv->scales + rows;
+  l.block_table = kv->block_table;
+  l.G = kv->d.n_kv_heads;
+  l.page_shift = 0;
+  while ((1 << l.page_shift) < kv->d.page_size) l.page_shift++;
+  l.max_pages = kv->d.max_pages_per_seq;
+  l.n_seq = kv->d.max_batch;
+  l.max_ctx = kv->max_ctx;
+  return l;
+}
+
+#ifdef __CUDACC__
+constexpr int KVQ_INT8 = JG_KVQ_INT8, KVQ_E4M3 = JG_KVQ_E4M3;
+
+// Row of (position t, kv head g) in a layer's pools, for the sequence with this row of the block table (entries were checked when
+// the table was set).
+__device__ __forceinline__ size_t kvq_row(const KvqLayer& c, const int32_t* bt_row, int t, int g) {
+  return ((((size_t)bt_row[t >> c.page_shift] * c.G + g) << c.page_shift)) + (t & ((1 << c.page_shift) - 1));
+}
+
+// Four codes (a word) as two pairs of halves, without their scale.
+template <int FMT>
+__device__ __forceinline__ void kvq_widen(uint32_t w, __half2& lo, __half2& hi) {
+  if (FMT == KVQ_INT8) {
+    const uint32_t v = w ^ 0x80808080u;  // code + 128, behind the exponent of 1024
+    const uint32_t a = __byte_perm(v, 0x64646464u, 0x4140), b = __byte_perm(v, 0x64646464u, 0x4342);
+    const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+    lo = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
+    hi = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    lo = *reinterpret_cast<const __half2*>(&a);
+    hi = *reinterpret_cast<const __half2*>(&b);
+  }
+}
+
+// The scale of a row whose largest magnitude is a (finite).
+template <int FMT>
+__device__ __forceinline__ float kvq_scale(float a) {
+  if (a == 0.f) return 0.f;
+  if (FMT == KVQ_INT8) {
+    const float s = __fdiv_rn(a, 127.f);
+    if (s < 4.76837158203125e-07f) return ceilf(s * 16777216.f) * 5.9604644775390625e-08f;  // below 2^-21: multiples of 2^-24
+    return __uint_as_float((__float_as_uint(s) + 0xFFFFFu) & ~0xFFFFFu);                      // 3 bits behind the leading one
+  }
+  const uint32_t s = (__float_as_uint(__fdiv_rn(a, 448.f)) + 0x7FFFFFu) & ~0x7FFFFFu;  // the next power of two
+  return fmaxf(__uint_as_float(s), 3.0517578125e-05f);
+}
+// Four values as a word of codes.
+template <int FMT>
+__device__ __forceinline__ uint32_t kvq_codes(const float (&x)[4], float scale) {
+  if (!(scale > 0.f)) return 0;
+  if (FMT == KVQ_INT8) {
+    const float top = fminf(127.f, floorf(__fdiv_rn(65504.f, scale)));
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -top), top) & 0xFFu) << (8 * i);
+    return w;
+  }
+  const float up = __uint_as_float(0x7F000000u - __float_as_uint(scale)), top = scale < 256.f ? 448.f : 240.f;  // 1 / 2^e
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) y[i] = fminf(fmaxf(x[i] * up, -top), top);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+// Eight halves, four pairs, turned by (cos, sin): products of halves are exact in 32 bits, so each value is rounded there once and
+// then to half.
+__device__ __forceinline__ uint4 kvq_rotate(const uint4& x, const uint4& t) {
+  const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ts[4] = {t.x, t.y, t.z, t.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float2 v = h2_to_f2(xs[i]), c = h2_to_f2(ts[i]);
+    const __half2 h = __floats2half2_rn(fmaf(v.x, c.x, -(v.y * c.y)), fmaf(v.x, c.y, v.y * c.x));
+    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// A K and a V row spread over LPR neighbouring lanes, eight values each (K rotated already): their codes and scales.
+template <int FMT, int LPR>
+__device__ __forceinline__ void kvq_quantise(const uint4& k, const uint4& v, uint2& kc, uint2& vc, __half2& scale) {
+  float x[8], y[8];
+  unpack8(k, x);
+  unpack8(v, y);
+  float a = 0.f, b = 0.f;
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    a = fmaxf(a, fabsf(x[i]));
+    b = fmaxf(b, fabsf(y[i]));
+    fine = fine && fabsf(x[i]) <= 65504.f && fabsf(y[i]) <= 65504.f;
+  }
+  if (!fine) a = INFINITY;
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) {
+    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+  }
+  if (a == INFINITY) {
+    kc = vc = make_uint2(0, 0);
+    scale = __halves2half2(__ushort_as_half(0x7FFF), __ushort_as_half(0));
+    return;
+  }
+  const float sk = kvq_scale<FMT>(a), sv = kvq_scale<FMT>(b);
+  kc.x = kvq_codes<FMT>({x[0], x[1], x[2], x[3]}, sk);
+  kc.y = kvq_codes<FMT>({x[4], x[5], x[6], x[7]}, sk);
+  vc.x = kvq_codes<FMT>({y[0], y[1], y[2], y[3]}, sv);
+  vc.y = kvq_codes<FMT>({y[4], y[5], y[6], y[7]}, sv);
+  scale = __floats2half2_rn(sk, sv);
+}
+#endif

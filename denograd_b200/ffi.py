@@ -40,6 +40,7 @@ class StepDesc(C.Structure):
 
 
 JG_F32, JG_BF16 = 0, 1
+KVQ_INT8, KVQ_E4M3 = 0, 1
 DENSE_STORE, DENSE_GLU, DENSE_MINGRU, DENSE_LOGITS = 0, 1, 2, 3
 ACT_NONE, ACT_SILU, ACT_RELU2, ACT_GELU_SIDE = 0, 1, 2, 3
 
@@ -146,6 +147,14 @@ SIGNATURES: dict[str, list] = {
     "jg_attn_rows": [_vp, _vp, _i32, _u64, _u64, _u64, _u64, _i32, _i32],
     "jg_attn_chunk": [_vp, _vp, _i32, _u64, _u64, _u64, _u64, _i32, _i32, _i32],
     "jg_attn_decode_noalloc": [_vp, _u64, _u64, _u64, _u64, _u64, _u64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
+    "jg_kvq_create": [_vp, _P(KvDesc), _i32, _P(_vp)],
+    "jg_kvq_destroy": [_vp],
+    "jg_kvq_set_block_table": [_vp, _vp],
+    "jg_kvq_bytes": [_vp, _P(_u64)],
+    "jg_kvq_write": [_vp, _vp, _i32, _u64, _i32, _u64, _i32, _u64, _i32, _u64, _u64, _i32, _i32],
+    "jg_kvq_decode": [_vp, _vp, _i32, _u64, _i32, _u64, _i32, _u64, _i32, _u64, _u64, _i32, _i32],
+    "jg_kvq_attn": [_vp, _vp, _i32, _u64, _i32, _u64, _i32, _i32, _u64, _u64, _u64, _u64, _i32, _i32, _i32, _i32],
+    "jg_kvq_read": [_vp, _vp, _i32, _u64, _u64, _i32, _i32, _u64, _u64, _u64, _u64, _i32, _i32, _i32],
     "jg_step_create": [_vp, _vp, _P(StepDesc), _P(_vp)],
     "jg_step_destroy": [_vp],
     "jg_step_run": [_vp, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _u64, _i32, _i32, _i32],

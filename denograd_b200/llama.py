@@ -23,6 +23,7 @@ import numpy as np
 from . import ffi
 from .decoder import Decoder, TinyJit, sample  # noqa: F401
 from .device import CUDA, Tensor
+from .kvquant import QuantKVCache
 from .nn import Embedding, Linear, RMSNorm, _dev
 
 
@@ -109,6 +110,8 @@ class Attention:
             raise NotImplementedError("multi-token calls are fed one position at a time on this device")
         B = x.numel() // x.shape[-1]
         xqkv = self._wqkv.call(x, out=qkv)  # xq | xk | xv
+        if isinstance(self._kv, QuantKVCache):
+            return self.wo.call(self._kv.decode(self._layer, xqkv, pos, freqs_cis, out=attn), residual=residual, out=out)
         apply_rotary_emb_kvwrite(xqkv, freqs_cis, pos, self._kv, self._layer, self.n_heads)
         a = attn if attn is not None else Tensor.empty((B, self.n_heads * self.head_dim), "float16", x.dev)
         x.dev.call("jg_attn_decode", self._kv.handle, self._layer, a.ptr, xqkv.ptr, pos.ptr, B, self.n_heads)
@@ -171,7 +174,9 @@ class TransformerBlock:
         else:
             dev.call("jg_norm_linear", ws.qkv.ptr, ws.h.ptr, self.attention_norm.weight.ptr, self.attention_norm.eps,
                      wqkv.weight.ptr, wqkv.scale_ptr, B, wqkv.out_features, d)
-        if a._kv.fused_attention:
+        if isinstance(a._kv, QuantKVCache):  # RoPE + cache write + attention in one launch
+            a._kv.decode(a._layer, ws.qkv, pos, freqs_cis, out=ws.attn)
+        elif a._kv.fused_attention:
             try:  # RoPE + cache write + attention in one cluster launch
                 dev.call("jg_attn_decode_fused", a._kv.handle, a._layer, ws.attn.ptr, ws.qkv.ptr, freqs_cis.ptr,
                          freqs_cis.shape[0], pos.ptr, B, a.n_heads)
@@ -179,7 +184,7 @@ class TransformerBlock:
                 if e.status != ffi.JG_ENOTSUP:
                     raise
                 a._kv.fused_attention = False  # context slice too long for shared memory: use the split kernels
-        if not a._kv.fused_attention:
+        if not isinstance(a._kv, QuantKVCache) and not a._kv.fused_attention:
             apply_rotary_emb_kvwrite(ws.qkv, freqs_cis, pos, a._kv, a._layer, a.n_heads)
             dev.call("jg_attn_decode", a._kv.handle, a._layer, ws.attn.ptr, ws.qkv.ptr, pos.ptr, B, a.n_heads)
         self._row_parallel(a.wo, ws.attn, ws, tp, fp16(a.wo)[0] if nf4 and not a.wo.direct(B) else None, split=split)
@@ -346,8 +351,10 @@ class Transformer(Decoder):
     def __init__(self, dim: int, hidden_dim: int, n_heads: int, n_layers: int, norm_eps: float, vocab_size: int,
                  linear=Linear, embedding=Embedding, n_kv_heads: int | None = None, rope_theta: float = 10000,
                  max_context: int = 1024, jit: bool = True, feed_forward=FeedForward, device=None, max_batch: int = 1,
-                 page_size: int = 64, tied_output: bool = False, fused: bool = True, n_split: int = 0, tp=None):
+                 page_size: int = 64, tied_output: bool = False, fused: bool = True, n_split: int = 0, tp=None,
+                 kv_dtype: str = "float16"):
         dev = _dev(device)
+        self.kv_dtype = kv_dtype  # "float16", or "int8" / "fp8": the cache in 8 bits (kvquant.py)
         self.dev, self.dim, self.vocab_size = dev, dim, vocab_size
         self.head_dim = dim // n_heads
         n_kv_heads = n_kv_heads if n_kv_heads is not None else n_heads
@@ -388,7 +395,7 @@ class Transformer(Decoder):
             self.output = Linear(dim, vocab_size, False, device=dev) if embedding is Embedding else linear(dim, vocab_size, False, device=dev)
         self.freqs_cis = precompute_freqs_cis(self.head_dim, self.max_context * 2, rope_theta, device=dev)
         self._kv_args = (n_layers, n_heads, self.n_kv_heads, self.head_dim, max_context, max_batch, page_size, n_split)
-        self._kv = KVCache(dev, *self._kv_args)
+        self._kv = self._new_kv()
         for i, layer in enumerate(self.layers):
             layer.attention._kv, layer.attention._layer = self._kv, i
         self._ws: dict[int, _Workspace] = {}
@@ -398,6 +405,11 @@ class Transformer(Decoder):
         self._dq_scratch: Tensor | None = None  # fp16 copies of quantised matrices (_fp16_weights)
         self._step_plan = None  # None: not tried yet, False: this model keeps the launch-per-op step
 
+    def _new_kv(self) -> "KVCache | QuantKVCache":
+        if self.kv_dtype == "float16":
+            return KVCache(self.dev, *self._kv_args)
+        return QuantKVCache(self.dev, *self._kv_args[:7], dtype=self.kv_dtype)
+
     def new_cache(self) -> None:
         """An empty (all-zero) KV cache in place of the current one, as a newly built model has (the lazily created
         Attention.cache_kv of jsgrad/models/llama.ts:78-90).  Everything that holds the old cache's addresses goes
@@ -406,7 +418,7 @@ class Transformer(Decoder):
         self._loop_graph.clear()
         self._step_plan = None
         self.dev.synchronize()
-        old, self._kv = self._kv, KVCache(self.dev, *self._kv_args)
+        old, self._kv = self._kv, self._new_kv()
         for layer in self.layers:
             layer.attention._kv = self._kv
         old.close()
@@ -448,7 +460,7 @@ class Transformer(Decoder):
             # rank's 8 us of weights; JG_STEP_KERNEL_TP=1 / 0 forces it on / off
             want_tp = os.environ.get("JG_STEP_KERNEL_TP", "1" if (self._tp is None or self._tp.world <= 4) else "0") != "0"
             tp_ok = self._tp is None or (self._tp.peer_capacity > 0 and want_tp)
-            plain = (self.fused and tp_ok and os.environ.get("JG_STEP_KERNEL", "1") != "0"
+            plain = (self.fused and tp_ok and self.kv_dtype == "float16" and os.environ.get("JG_STEP_KERNEL", "1") != "0"
                      and type(a0.wo) is Linear and type(self.output) is Linear and type(self.tok_embeddings) is Embedding
                      and type(self.layers[0].feed_forward) is FeedForward)
             if plain:
@@ -590,12 +602,16 @@ class Transformer(Decoder):
             layer.attention_norm.call(ws.h, out=ws.xn)
             (wp, sp), = weights(a._wqkv)
             dev.call("jg_linear", ws.qkv.ptr, ws.xn.ptr, wp, sp, 0, R, a._wqkv.out_features, d)
-            dev.call("jg_rope_kvwrite_rows", a._kv.handle, a._layer, ws.qkv.ptr, self.freqs_cis.ptr, self.freqs_cis.shape[0],
-                     ws.pos.ptr, ws.seq.ptr, R, a.n_heads)
-            if Sc >= 8 and os.environ.get("JG_ATTN_CHUNK", "1") != "0":  # tensor-core attention over the regular chunk
-                dev.call("jg_attn_chunk", a._kv.handle, a._layer, ws.attn.ptr, ws.qkv.ptr, ws.pos.ptr, ws.seq.ptr, B, Sc, a.n_heads)
+            if isinstance(a._kv, QuantKVCache):
+                a._kv.write(a._layer, ws.qkv, ws.pos, seq=ws.seq, freqs_cis=self.freqs_cis, q_out=ws.qkv)
+                a._kv.attend(a._layer, ws.qkv, ws.pos.view_rows(0, B), seq=ws.seq, max_count=Sc, step=B, out=ws.attn)
             else:
-                dev.call("jg_attn_rows", a._kv.handle, a._layer, ws.attn.ptr, ws.qkv.ptr, ws.pos.ptr, ws.seq.ptr, R, a.n_heads)
+                dev.call("jg_rope_kvwrite_rows", a._kv.handle, a._layer, ws.qkv.ptr, self.freqs_cis.ptr, self.freqs_cis.shape[0],
+                         ws.pos.ptr, ws.seq.ptr, R, a.n_heads)
+                if Sc >= 8 and os.environ.get("JG_ATTN_CHUNK", "1") != "0":  # tensor-core attention over the regular chunk
+                    dev.call("jg_attn_chunk", a._kv.handle, a._layer, ws.attn.ptr, ws.qkv.ptr, ws.pos.ptr, ws.seq.ptr, B, Sc, a.n_heads)
+                else:
+                    dev.call("jg_attn_rows", a._kv.handle, a._layer, ws.attn.ptr, ws.qkv.ptr, ws.pos.ptr, ws.seq.ptr, R, a.n_heads)
             layer._row_parallel(a.wo, ws.attn, ws, tp, weights(a.wo)[0] if dq else None)
             layer.ffn_norm.call(ws.h, out=ws.xn)
             (w1p, s1p), (w3p, s3p) = weights(f.w1, f.w3)

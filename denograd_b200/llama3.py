@@ -12,6 +12,7 @@ import numpy as np
 from . import synth
 from .device import Device
 from .driver import Driver, Llama3Usage  # noqa: F401
+from .kvquant import FORMATS
 from .llama import Transformer
 from .nn import Embedding, Int8Embedding, Int8Linear, Linear, NF4Linear, load_state_dict
 
@@ -53,10 +54,13 @@ class Llama3(Driver):
     args: dict = field(default_factory=dict)
     last_seen_toks: list = field(default_factory=list)
     tokenizer: object | None = None  # denograd_b200.tokenizer.Tokenizer, needed by _system / chat only
+    kv_dtype: str = "float16"  # of the KV cache: 'float16' | 'int8' | 'fp8' (kvquant.py)
 
     def __post_init__(self):
         if self.quantize not in ("float16", "int8", "nf4", None):
             raise ValueError(f"quantize={self.quantize!r}: expected 'float16', 'int8' or 'nf4'")
+        if self.kv_dtype not in ("float16", *FORMATS):
+            raise ValueError(f"kv_dtype={self.kv_dtype!r}: expected 'float16', 'int8' or 'fp8'")
         if self.quantize == "nf4" and self.tp is not None:
             raise NotImplementedError("NF4 weights under tensor parallelism")
         p = dict(MODEL_PARAMS[self.size]["args"])
@@ -72,7 +76,7 @@ class Llama3(Driver):
         self.model = Transformer(p["dim"], p["hidden_dim"], p["n_heads"], p["n_layers"], p["norm_eps"], p["vocab_size"],
                                  self.linear, self.embedding, p["n_kv_heads"], p["rope_theta"], self.max_context, self.jit,
                                  device=Device[self.device], max_batch=self.max_batch, page_size=self.page_size,
-                                 tied_output=tied, fused=self.fused, tp=self.tp)
+                                 tied_output=tied, fused=self.fused, tp=self.tp, kv_dtype=self.kv_dtype)
         self.usage = Llama3Usage()
         self.start_pos = 0
 

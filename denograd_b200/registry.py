@@ -16,6 +16,8 @@ def _weights_path(folder: str) -> str:
 
 
 def _hybrid(config: dict, folder: str, dtype: str | None, max_context: int, max_batch: int, **kw):
+    if kw.pop("kv_dtype", "float16") != "float16":
+        raise UnsupportedDtype(f"{architecture(config)} keeps its state in its own types: kv_dtype is for Llama models")
     from . import build, ffi
     ffi.use_component(build.component_of(lc["type"] for lc in config["layers"]))
     from .matulorn import Matulorn

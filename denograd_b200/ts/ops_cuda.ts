@@ -75,6 +75,14 @@ export const SYMBOLS = {
   jg_rope_kvwrite_rows: fn([ptr, ptr, i32, u64, u64, i32, u64, u64, i32, i32]),
   jg_attn_rows: fn([ptr, ptr, i32, u64, u64, u64, u64, i32, i32]),
   jg_attn_chunk: fn([ptr, ptr, i32, u64, u64, u64, u64, i32, i32, i32]),
+  jg_kvq_create: fn([ptr, buf, i32, buf]),
+  jg_kvq_destroy: fn([ptr]),
+  jg_kvq_set_block_table: fn([ptr, buf]),
+  jg_kvq_bytes: fn([ptr, buf]),
+  jg_kvq_write: fn([ptr, ptr, i32, u64, i32, u64, i32, u64, i32, u64, u64, i32, i32]),
+  jg_kvq_decode: fn([ptr, ptr, i32, u64, i32, u64, i32, u64, i32, u64, u64, i32, i32]),
+  jg_kvq_attn: fn([ptr, ptr, i32, u64, i32, u64, i32, i32, u64, u64, u64, u64, i32, i32, i32, i32]),
+  jg_kvq_read: fn([ptr, ptr, i32, u64, u64, i32, i32, u64, u64, u64, u64, i32, i32, i32]),
   jg_attn_decode_noalloc: fn([ptr, u64, u64, u64, u64, u64, u64, i32, i32, i32, i32, i32, i32, i32, i32]),
   jg_pos_advance: fn([ptr, u64, i32]),
   jg_dequant_i8_f16: fn([ptr, u64, u64, u64, 'i64', 'i64']),

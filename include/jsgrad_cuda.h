@@ -293,6 +293,45 @@ int jg_attn_decode_noalloc(jg_dev* dev, uint64_t out, uint64_t qkv, uint64_t k_l
                            uint64_t block_table, uint64_t pos, int32_t B, int32_t H, int32_t G, int32_t head_dim,
                            int32_t page_size, int32_t max_pages_per_seq, int32_t n_split, int32_t n_pages);
 
+/* ---- The KV cache in 8 bits.  The reference keeps K and V in the model's 16-bit type (jsgrad/models/llama.ts:78-90); this is the same
+ *      paged pool with a code a value and a scale for each (position, kv head) of K and of V: 2 * head_dim + 4 bytes instead of
+ *      4 * head_dim.  JG_KVQ_INT8: scale = max|x| / 127 rounded up to 4 significant bits, code = rint(x / scale).  JG_KVQ_E4M3: e4m3 codes
+ *      with a power of two as the scale.  Either way code * scale is an fp16 number and attention multiplies those, exactly.
+ *      A position whose K or V holds a NaN or an infinity makes NaN of every query that sees it, and of no other.
+ *      The desc is jg_kvcache_create's (n_split is not used; 1 to 8 query heads per kv head).  Rows are fp16; ld* counts elements
+ *      between rows, a multiple of 8; a row's columns behind the named ones are left alone.  Positions and slots come from device memory and
+ *      are checked there: whatever lies outside the cache is not followed.  The rows of one call name different (slot, position)s. */
+#define JG_KVQ_INT8 0
+#define JG_KVQ_E4M3 1
+typedef struct jg_kvq jg_kvq; /* paged 8-bit K/V pool of one model on one device */
+int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t format, jg_kvq** out);
+int jg_kvq_destroy(jg_kvq* kv);
+int jg_kvq_set_block_table(jg_kvq* kv, const int32_t* table); /* as jg_kvcache_set_block_table */
+int jg_kvq_bytes(jg_kvq* kv, uint64_t* out);
+/* apply_rotary_emb on Q and K + cache assignment (jsgrad/models/llama.ts:23-32,87) for R independent rows: row r of qkv, wq|wk|wv outputs
+ * [(H + 2G) * hd], has position pos[r] of slot seq[r] (0: row r is slot r).  Q and K are rotated in 32 bits and rounded to fp16 once;
+ * rotated Q goes to q_out (0: nowhere; qkv itself: in place), K and V into the cache.  table = 0: nothing is rotated.
+ * A row whose slot or position lies outside the cache or the table is skipped. */
+int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, int32_t ldq, uint64_t qkv, int32_t ldx, uint64_t table,
+                 int32_t table_rows, uint64_t pos, uint64_t seq, int32_t R, int32_t H);
+/* One new token for each of B rows, of different slots: what jg_kvq_write does to K and V, and scaled_dot_product_attention over positions
+ * [0, pos[b]] (jsgrad/tensor.ts:3920-3934; jsgrad/models/llama.ts:34-39,89-96) in one launch.  qkv is left as it is.
+ * out: [B][H * hd]; a row whose slot or position lies outside the cache or the table gets zeros, and nothing is stored for it. */
+int jg_kvq_decode(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int32_t ldo, uint64_t qkv, int32_t ldx, uint64_t table,
+                  int32_t table_rows, uint64_t pos, uint64_t seq, int32_t B, int32_t H);
+/* Chunks: sequence b, in slot seq[b] (0: slot b), has count[b] new positions (0: max_count each; more than max_count are cut off), the
+ * first of them pos[b]; position pos[b] + i is row first[b] + i * step (first = 0: row b + i * step, so step = B is jg_attn_chunk's
+ * position-major order and first = running sums with step = 1 a ragged batch).  Their K and V are in the cache already (jg_kvq_write) and
+ * Q is rotated.  out[row] = attention of q[row] (the first H * hd columns) over positions [0, pos[b] + i].
+ * Rows outside [0, R) are not followed; rows that no sequence names are left as they were; a position or a slot outside the cache
+ * gives a row of zeros. */
+int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int32_t ldo, uint64_t q, int32_t ldq, int32_t R, uint64_t pos,
+                uint64_t count, uint64_t first, uint64_t seq, int32_t B, int32_t max_count, int32_t step, int32_t H);
+/* What the cache holds, as fp16 rows of G * hd: positions and rows are named as in jg_kvq_attn.  Positions and slots outside the cache read
+ * as zeros, a position that was stored with a NaN or an infinity as NaN. */
+int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint64_t v, int32_t ld, int32_t R, uint64_t pos, uint64_t count,
+                uint64_t first, uint64_t seq, int32_t B, int32_t max_count, int32_t step);
+
 /* pos[b] += 1 for b < B (the host-side `start_pos++` of the decode loop, jsgrad/models/llama3.ts:284-295,
  * kept on the device so a captured step can be replayed without host input). */
 int jg_pos_advance(jg_dev* dev, uint64_t pos, int32_t B);
