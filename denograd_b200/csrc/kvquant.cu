@@ -2,7 +2,7 @@
 #include <stdlib.h>
 #include <string.h>
 
-#include "kvquant.cuh"
+#include "kvquant_split.cuh"
 
 // ------------------------------------------------------------------------------------------------ the object
 JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t format, jg_kvq** out) {
@@ -32,6 +32,9 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
   if (e == cudaSuccess) e = cudaMalloc(&kv->v_codes, codes);
   if (e == cudaSuccess) e = cudaMalloc(&kv->scales, rows * sizeof(__half2));
   if (e == cudaSuccess) e = cudaMalloc(&kv->block_table, table);
+  const size_t part = (size_t)2 * ks_ctas(dev) * ks_part_floats(d.head_dim) * sizeof(float), tickets = (size_t)ks_ctas(dev) * sizeof(unsigned int);
+  if (e == cudaSuccess) e = cudaMalloc(&kv->part, part);
+  if (e == cudaSuccess) e = cudaMalloc(&kv->tickets, tickets);
   int32_t* ids = (int32_t*)malloc(table);
   if (e == cudaSuccess && ids == nullptr) e = cudaErrorMemoryAllocation;
   if (e == cudaSuccess) {
@@ -42,9 +45,11 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
         const long long pg = (long long)b * d.max_pages_per_seq + i;
         ids[(size_t)b * d.max_pages_per_seq + i] = (int32_t)(pg < d.n_pages ? pg : d.n_pages - 1);
       }
-    e = cudaMemsetAsync(kv->k_codes, 0, codes, dev->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(kv->v_codes, 0, codes, dev->stream);
+    const int zero = format == JG_KVQ_INT8 ? 128 : 0;
+    e = cudaMemsetAsync(kv->k_codes, zero, codes, dev->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->v_codes, zero, codes, dev->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(kv->scales, 0, rows * sizeof(__half2), dev->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->tickets, 0, tickets, dev->stream);
     if (e == cudaSuccess) e = cudaMemcpyAsync(kv->block_table, ids, table, cudaMemcpyHostToDevice, dev->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
   }
@@ -54,7 +59,7 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
     jg_kvq_destroy(kv);
     return jg_cuda_fail(e, "kvq_create", __FILE__, __LINE__);
   }
-  kv->bytes = 2 * codes + rows * sizeof(__half2) + table;
+  kv->bytes = 2 * codes + rows * sizeof(__half2) + table + part + tickets;
   *out = kv;
   return JG_OK;
 }
@@ -67,6 +72,7 @@ JG_API int jg_kvq_destroy(jg_kvq* kv) {
   cudaSetDevice(kv->dev->ordinal);
   cudaStreamSynchronize(kv->dev->stream);
   cudaFree(kv->k_codes); cudaFree(kv->v_codes); cudaFree(kv->scales); cudaFree(kv->block_table);
+  cudaFree(kv->part); cudaFree(kv->tickets);
   delete kv;
   return JG_OK;
 }

@@ -24,6 +24,8 @@ struct jg_kvq {
   uint8_t* v_codes;
   __half2* scales;   // [L][n_pages][G][page], (K, V)
   int32_t* block_table;
+  float* part;            // pieces of results that several CTAs share, and who has arrived (kvquant_split.cuh)
+  unsigned int* tickets;
   int max_ctx;
   size_t layer_rows;  // (position, kv head) rows of a layer
   uint64_t bytes;
@@ -57,6 +59,10 @@ static inline KvqLayer kvq_layer(const jg_kvq* kv, int layer) {
 #ifdef __CUDACC__
 constexpr int KVQ_INT8 = JG_KVQ_INT8, KVQ_E4M3 = JG_KVQ_E4M3;
 
+// Four codes of zeros.  An int8 code lies in the cache as code + 128, which saves what widens it an operation.
+template <int FMT>
+constexpr uint32_t KVQ_ZERO = FMT == KVQ_INT8 ? 0x80808080u : 0u;
+
 // Row of (position t, kv head g) in a layer's pools, for the sequence with this row of the block table (entries were checked when
 // the table was set).
 __device__ __forceinline__ size_t kvq_row(const KvqLayer& c, const int32_t* bt_row, int t, int g) {
@@ -67,8 +73,7 @@ __device__ __forceinline__ size_t kvq_row(const KvqLayer& c, const int32_t* bt_r
 template <int FMT>
 __device__ __forceinline__ void kvq_widen(uint32_t w, __half2& lo, __half2& hi) {
   if (FMT == KVQ_INT8) {
-    const uint32_t v = w ^ 0x80808080u;  // code + 128, behind the exponent of 1024
-    const uint32_t a = __byte_perm(v, 0x64646464u, 0x4140), b = __byte_perm(v, 0x64646464u, 0x4342);
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);  // behind the exponent of 1024
     const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
     lo = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
     hi = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
@@ -95,12 +100,12 @@ __device__ __forceinline__ float kvq_scale(float a) {
 // Four values as a word of codes.
 template <int FMT>
 __device__ __forceinline__ uint32_t kvq_codes(const float (&x)[4], float scale) {
-  if (!(scale > 0.f)) return 0;
+  if (!(scale > 0.f)) return KVQ_ZERO<FMT>;
   if (FMT == KVQ_INT8) {
     const float top = fminf(127.f, floorf(__fdiv_rn(65504.f, scale)));
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -top), top) & 0xFFu) << (8 * i);
+    for (int i = 0; i < 4; i++) w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -top), top) + 128u) << (8 * i);
     return w;
   }
   const float up = __uint_as_float(0x7F000000u - __float_as_uint(scale)), top = scale < 256.f ? 448.f : 240.f;  // 1 / 2^e
@@ -147,7 +152,7 @@ __device__ __forceinline__ void kvq_quantise(const uint4& k, const uint4& v, uin
     b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
   }
   if (a == INFINITY) {
-    kc = vc = make_uint2(0, 0);
+    kc = vc = make_uint2(KVQ_ZERO<FMT>, KVQ_ZERO<FMT>);
     scale = __halves2half2(__ushort_as_half(0x7FFF), __ushort_as_half(0));
     return;
   }

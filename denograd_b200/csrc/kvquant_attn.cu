@@ -3,7 +3,7 @@
 // o = sum_t w_t v_t / sum_t w_t with w_t = 2^((s_t - max) / ln 2), s_t = q.k_t / sqrt(hd), in one pass over the cache with a running maximum.
 #include <math.h>
 
-#include "kvquant.cuh"
+#include "kvquant_split.cuh"
 
 struct KvqAttnArgs {
   KvqLayer c;
@@ -89,16 +89,15 @@ JG_API int jg_kvq_decode(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, i
   JG_REQUIRE(ldo >= H * hd && ldo % 8 == 0, "kvq_decode: rows of out of %d elements are no multiple of 8 or too short", ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(qkv, 16) && table % 16 == 0 && jg_aligned(pos, 4) && seq % 4 == 0, "kvq_decode: null or misaligned pointer");
   JG_REQUIRE(table == 0 || table_rows > 0, "kvq_decode: empty RoPE table");
-  // rotated Q waits in `out`, whose row the kernel reads before it writes it
-  const int rc = jg_kvq_write(dev, kv, layer, out, ldo, qkv, ldx, table, table_rows, pos, seq, B, H);
-  if (rc) return rc;
-  KvqAttnArgs a = {};
+  KvqSplitArgs a = {};
   a.c = kvq_layer(kv, layer);
-  a.q = (const __half*)out; a.out = (__half*)out; a.pos = (const int32_t*)pos; a.seq = (const int32_t*)seq;
-  a.ldq = ldo; a.ldo = ldo; a.R = B; a.H = H; a.n_rep = H / G; a.max_count = 1; a.step = 1;
-  a.table_rows = table && table_rows < kv->max_ctx ? table_rows : kv->max_ctx;
+  a.x = (const __half*)qkv; a.table = (const __half*)table; a.out = (__half*)out; a.pos = (const int32_t*)pos; a.seq = (const int32_t*)seq;
+  a.ldx = ldx; a.ldo = ldo; a.R = B; a.B = B; a.H = H; a.n_rep = H / G; a.max_count = 1; a.step = 1;
+  a.limit = table && table_rows < kv->max_ctx ? table_rows : kv->max_ctx;
   a.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
-  return launch_attn(dev, kv, a, B, "kvq_decode");
+  a.part = kv->part; a.tickets = kv->tickets;
+  if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_split<KVQ_INT8, 64, 1, true>(dev, a) : launch_split<KVQ_INT8, 128, 1, true>(dev, a);
+  return hd == 64 ? launch_split<KVQ_E4M3, 64, 1, true>(dev, a) : launch_split<KVQ_E4M3, 128, 1, true>(dev, a);
 }
 
 JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int32_t ldo, uint64_t q, int32_t ldq, int32_t R, uint64_t pos,
@@ -112,6 +111,22 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
+  if ((long long)max_count * (H / G) <= 16) {
+    KvqSplitArgs s = {};
+    s.c = kvq_layer(kv, layer);
+    s.x = (const __half*)q; s.out = (__half*)out;
+    s.pos = (const int32_t*)pos; s.count = (const int32_t*)count; s.first = (const int32_t*)first; s.seq = (const int32_t*)seq;
+    s.ldx = ldq; s.ldo = ldo; s.R = R; s.B = B; s.H = H; s.n_rep = H / G; s.max_count = max_count; s.step = step;
+    s.limit = kv->max_ctx;
+    s.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
+    s.part = kv->part; s.tickets = kv->tickets;
+    const bool few = max_count * (H / G) <= 8;
+    if (kv->format == JG_KVQ_INT8)
+      return hd == 64 ? (few ? launch_split<KVQ_INT8, 64, 1, false>(dev, s) : launch_split<KVQ_INT8, 64, 2, false>(dev, s))
+                      : (few ? launch_split<KVQ_INT8, 128, 1, false>(dev, s) : launch_split<KVQ_INT8, 128, 2, false>(dev, s));
+    return hd == 64 ? (few ? launch_split<KVQ_E4M3, 64, 1, false>(dev, s) : launch_split<KVQ_E4M3, 64, 2, false>(dev, s))
+                    : (few ? launch_split<KVQ_E4M3, 128, 1, false>(dev, s) : launch_split<KVQ_E4M3, 128, 2, false>(dev, s));
+  }
   KvqAttnArgs a = {};
   a.c = kvq_layer(kv, layer);
   a.q = (const __half*)q; a.out = (__half*)out;

@@ -1,0 +1,470 @@
+// Attention of few queries over the 8-bit cache, bound by reading it: one new token a row, or short chunks.
+//
+// Queries of a (sequence, kv head) are columns, (position, query head) pairs, up to 8 * NT.  A warp takes 16 positions at a time:
+//   scores^T [16 positions x columns] = K [16 x hd] . q^T        weights in 16 bits, turned by movmatrix
+//   out^T [hd x columns] += V^T [hd x 16 positions] . w^T        mma.sync.m16n8k16, 32-bit sums
+// The inner index of a product and the order of its rows are free as long as both operands agree, so a lane's fragments are 16
+// neighbouring codes of a row: of K as they lie, of V two rows at a time with their bytes interleaved.  A lane copies the bytes that it
+// will itself read (cp.async into a ring of its own in shared memory), so nothing is shared between lanes and nobody waits for a
+// barrier in the loop.  V is multiplied by its scale as it is widened (exact), K's scale goes to the finished scores.
+//
+// The running maximum is a reference that scores may pass by 2^6 before sums and outputs are rescaled: a vote a tile instead of three
+// rounds of shuffles.
+//
+// The positions of all (sequence, kv head)s are one line of units of 16 * KS_WARPS, cut evenly over the CTAs: long and short
+// conversations of a batch cost what they hold.  A CTA's stretch holds pieces of several (sequence, kv head)s; those that others
+// share are left in a workspace (at most two a CTA: its first and its last), and the last to arrive puts them together in order.
+#pragma once
+#include "kvquant.cuh"
+
+struct KvqSplitArgs {
+  KvqLayer c;
+  const __half* x;      // rows of queries; with a new token rows of wq|wk|wv
+  const __half* table;  // RoPE of the new tokens, or null
+  __half* out;
+  const int32_t* pos;
+  const int32_t* count;
+  const int32_t* first;
+  const int32_t* seq;
+  int ldx, ldo, R, B, H, n_rep, max_count, step, limit;  // positions from `limit` on are outside
+  float scale2;                                          // log2 e / sqrt(hd)
+  float* part;                                           // [2 * CTAs][columns * (hd + 2)]
+  unsigned int* tickets;                                 // [CTAs], zero between launches
+};
+
+constexpr int KS_WARPS = 8, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_STAGES = 2;
+
+template <int HD, int NT>
+struct KsCfg {
+  static constexpr int COLS = 8 * NT, KJ = HD / 64;             // 16-byte pieces of a K row that a lane holds
+  static constexpr int VB = HD / 8;                             // bytes of a V row that a lane holds
+  static constexpr int K_BYTES = 2 * KJ * 512, V_BYTES = 4 * VB * 32, S_BYTES = 24 * 32, STAGE = K_BYTES + V_BYTES + S_BYTES;
+  static constexpr int RING = KS_WARPS * KS_STAGES * STAGE;
+  static constexpr int MERGE = KS_WARPS * COLS * HD * 4;        // the warps' outputs, over the ring
+  static constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
+  static constexpr int PART = COLS * (HD + 2);                  // floats of a piece: outputs, maxima, sums
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float ks_ex2(float x) {  // 2^x by the hardware's approximation (2^-22 relative), 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ks_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t ks_transpose(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <int BYTES>
+__device__ __forceinline__ void ks_copy(uint32_t dst, const void* src) {
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ uint32_t ks_half2(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+template <int FMT, int HD, int NT, bool NEW>
+__global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(const KvqSplitArgs a) {
+  using Cfg = KsCfg<HD, NT>;
+  constexpr int COLS = Cfg::COLS, KJ = Cfg::KJ, VB = Cfg::VB, MT = HD / 16;
+  extern __shared__ __align__(16) unsigned char ks_raw[];
+  __shared__ float s_m[KS_WARPS + 1][COLS], s_l[KS_WARPS + 1][COLS];
+  __shared__ __align__(16) __half s_new[2][HD];  // the new token's K and V as they are stored
+  __shared__ unsigned int s_ticket;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, c = lane & 3;
+  pdl_launch();
+  pdl_wait();
+
+  // positions of sequence b that queries look at in the cache (its new token, if any, comes on top), 0 where it has none
+  auto sequence = [&](int b, int& p0, int& n, const int32_t*& bt) -> int {
+    const int sq = a.seq ? a.seq[b] : b;
+    p0 = a.pos[b];
+    n = NEW ? 1 : max(0, a.count ? min(a.count[b], a.max_count) : a.max_count);
+    bt = nullptr;
+    if ((unsigned)sq >= (unsigned)a.c.n_seq) return 0;
+    if (NEW && (unsigned)p0 >= (unsigned)a.limit) return 0;
+    bt = a.c.block_table + (size_t)sq * a.c.max_pages;
+    if (NEW) return p0;
+    if (n == 0) return 0;
+    return (int)max(0ll, min((long long)p0 + n, (long long)a.limit));
+  };
+  auto units = [&](int b) -> int {
+    int p0, n;
+    const int32_t* bt;
+    return max(1, (sequence(b, p0, n, bt) + KS_UNIT - 1) / KS_UNIT);
+  };
+  // this CTA's stretch of the line of units, and the sequence that it begins in; every warp works it out for itself
+  long long total = 0;
+  for (int b = lane; b < a.B; b += 32) total += units(b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  total *= a.c.G;
+  const long long ctas = min((long long)gridDim.x, total);
+  if (blockIdx.x >= ctas) return;
+  const long long u_lo = blockIdx.x * total / ctas, u_hi = (blockIdx.x + 1) * total / ctas;
+  int b = 0;
+  long long at = 0;  // first unit of (b, head 0)
+  for (int base = 0;; base += 32) {
+    const int n = base + lane < a.B ? units(base + lane) : 0;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int below = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += below;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, at + (long long)sum * a.c.G > u_lo);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      b = base + l;
+      at += (long long)__shfl_sync(0xffffffffu, sum - n, l) * a.c.G;
+      break;
+    }
+    at += (long long)__shfl_sync(0xffffffffu, sum, 31) * a.c.G;
+  }
+
+  unsigned char* ring = ks_raw + warp * (KS_STAGES * Cfg::STAGE);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  for (long long u = u_lo; u < u_hi; b++) {
+    int p0, n_new;
+    const int32_t* bt;
+    const int T = sequence(b, p0, n_new, bt);
+    const int n_units = max(1, (T + KS_UNIT - 1) / KS_UNIT);
+    const bool stored = NEW && bt != nullptr;  // there is a new token, at p0
+    const long long row0 = NEW ? b : (a.first ? a.first[b] : b);
+    const int n_cols = n_new * a.n_rep;
+    for (int g = (int)((u - at) / n_units); g < a.c.G && u < u_hi; g++) {
+      const long long item = at + (long long)g * n_units;
+      const int j0 = (int)(u - item), j1 = (int)min((long long)n_units, u_hi - item);
+      u = item + j1;
+      const int t_lo = j0 * KS_UNIT, t_hi = min(T, j1 * KS_UNIT);
+      const int n_tiles = t_hi > t_lo + warp * 16 ? (t_hi - t_lo - warp * 16 + KS_UNIT - 1) / KS_UNIT : 0;  // of this warp
+
+      // ---- copies of a tile: the lane's own pieces of 16 positions
+      int pages = 0;  // lane l: page of the warp's tile 32 i + l
+      auto request = [&](int i) {
+        const int t0 = t_lo + i * KS_UNIT + warp * 16;
+        if ((i & 31) == 0) pages = i + lane < n_tiles ? bt[(t0 + lane * KS_UNIT) >> a.c.page_shift] : 0;
+        const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+        const size_t row = (((size_t)page * a.c.G + g) << a.c.page_shift) + (t0 & ((1 << a.c.page_shift) - 1));
+        uint32_t to = ring_at + (i % KS_STAGES) * Cfg::STAGE + lane * 16;
+        const uint8_t* k = a.c.k + (row + r) * HD + c * 16;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int j = 0; j < KJ; j++, to += 512) ks_copy<16>(to, k + h * 8 * HD + j * 64);
+        const uint8_t* v = a.c.v + (row + 2 * c) * HD + r * VB;
+        to += lane * (VB - 16);
+#pragma unroll
+        for (int h = 0; h < 4; h++, to += VB * 32) ks_copy<VB>(to, v + ((h >> 1) * 8 + (h & 1)) * HD);
+        to += lane * (8 - VB);
+        const __half2* s = a.c.scales + row;
+        ks_copy<8>(to, s + 2 * c);
+        ks_copy<8>(to + 256, s + 2 * c + 8);
+        to -= lane * 4;
+        ks_copy<4>(to + 512, s + r);
+        ks_copy<4>(to + 640, s + r + 8);
+      };
+#pragma unroll
+      for (int i = 0; i < KS_STAGES - 1; i++) {
+        if (i < n_tiles) request(i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+
+      // ---- fragments of q^T: the lane's column is nt * 8 + r
+      uint32_t qf[NT][KJ * 4][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        const int col = nt * 8 + r, i = col / a.n_rep;
+        const long long row = row0 + (long long)i * a.step;
+        const bool have = col < n_cols && row >= 0 && row < a.R;
+        const __half* q = a.x + (size_t)(have ? row : 0) * a.ldx + (size_t)(g * a.n_rep + col % a.n_rep) * HD + c * 16;
+#pragma unroll
+        for (int j = 0; j < KJ; j++) {
+          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+          if (have) {
+            lo = ld_128(q + j * 64);
+            hi = ld_128(q + j * 64 + 8);
+            if (NEW && a.table && stored) {
+              const __half* turn = a.table + (size_t)p0 * HD + c * 16 + j * 64;
+              lo = kvq_rotate(lo, ld_128(turn));
+              hi = kvq_rotate(hi, ld_128(turn + 8));
+            }
+          }
+          qf[nt][j * 4][0] = lo.x; qf[nt][j * 4][1] = lo.y; qf[nt][j * 4 + 1][0] = lo.z; qf[nt][j * 4 + 1][1] = lo.w;
+          qf[nt][j * 4 + 2][0] = hi.x; qf[nt][j * 4 + 2][1] = hi.y; qf[nt][j * 4 + 3][0] = hi.z; qf[nt][j * 4 + 3][1] = hi.w;
+        }
+      }
+      // ---- the new token, by the CTA with the end of its sequence: stored, and an entry of its own when the warps' sums meet
+      const bool entry = stored && j1 == n_units;
+      if (NEW && entry && warp == 0) {
+        constexpr int LPR = HD / 8;
+        const int sub = lane % LPR;
+        const __half* k = a.x + (size_t)b * a.ldx + (size_t)(a.H + g) * HD + sub * 8;
+        uint4 kx = ld_128(k), vx = ld_128(k + (size_t)a.c.G * HD);
+        if (a.table) kx = kvq_rotate(kx, ld_128(a.table + (size_t)p0 * HD + sub * 8));
+        uint2 kc, vc;
+        __half2 scale;
+        kvq_quantise<FMT, LPR>(kx, vx, kc, vc, scale);
+        if (lane < LPR) {
+          const size_t to = kvq_row(a.c, bt, p0, g);
+          *reinterpret_cast<uint2*>(a.c.k + to * HD + sub * 8) = kc;
+          *reinterpret_cast<uint2*>(a.c.v + to * HD + sub * 8) = vc;
+          if (sub == 0) a.c.scales[to] = scale;
+          __half2 h[4], w[4];
+          kvq_widen<FMT>(kc.x, h[0], h[1]);
+          kvq_widen<FMT>(kc.y, h[2], h[3]);
+          kvq_widen<FMT>(vc.x, w[0], w[1]);
+          kvq_widen<FMT>(vc.y, w[2], w[3]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) { h[j] = __hmul2_rn(h[j], __low2half2(scale)); w[j] = __hmul2_rn(w[j], __high2half2(scale)); }
+          *reinterpret_cast<uint4*>(&s_new[0][sub * 8]) = *reinterpret_cast<const uint4*>(h);
+          *reinterpret_cast<uint4*>(&s_new[1][sub * 8]) = *reinterpret_cast<const uint4*>(w);
+        }
+        __syncwarp();
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < KJ * 4; j++) {
+          const uint2 kw = *reinterpret_cast<const uint2*>(&s_new[0][(j >> 2) * 64 + c * 16 + (j & 3) * 4]);
+          const float2 k0 = h2_to_f2(kw.x), k1 = h2_to_f2(kw.y), q0 = h2_to_f2(qf[0][j][0]), q1 = h2_to_f2(qf[0][j][1]);
+          s = fmaf(k0.x, q0.x, fmaf(k0.y, q0.y, fmaf(k1.x, q1.x, fmaf(k1.y, q1.y, s))));
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if (c == 0) { s_m[KS_WARPS][r] = s * a.scale2; s_l[KS_WARPS][r] = 1.f; }
+      }
+
+      // ---- the loop over tiles
+      float o[NT][MT][4], m[NT][2], l[NT][2];
+      int lim[NT][2];  // last position that the lane's columns of a score tile see
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int k = 0; k < MT; k++) o[nt][k][0] = o[nt][k][1] = o[nt][k][2] = o[nt][k][3] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          m[nt][e] = -INFINITY;
+          l[nt][e] = 0.f;
+          lim[nt][e] = NEW ? T - 1 : (int)min((long long)T - 1, (long long)p0 + (nt * 8 + 2 * c + e) / a.n_rep);
+        }
+      }
+      for (int i = 0; i < n_tiles; i++) {
+        if (i + KS_STAGES - 1 < n_tiles) request(i + KS_STAGES - 1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(KS_STAGES - 1) : "memory");
+        const unsigned char* stage = ring + (i % KS_STAGES) * Cfg::STAGE;
+        const int t0 = t_lo + i * KS_UNIT + warp * 16;
+        // scores
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KJ; j++) {
+          const uint4 k0 = *reinterpret_cast<const uint4*>(stage + j * 512 + lane * 16), k1 = *reinterpret_cast<const uint4*>(stage + (KJ + j) * 512 + lane * 16);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            __half2 a0, a1, a2, a3;
+            kvq_widen<FMT>(w0[e], a0, a2);
+            kvq_widen<FMT>(w1[e], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+              ks_mma(s[nt], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), qf[nt][j * 4 + e][0], qf[nt][j * 4 + e][1]);
+          }
+        }
+        const unsigned char* sc = stage + Cfg::K_BYTES + Cfg::V_BYTES;
+        const float ks0 = __low2float(*reinterpret_cast<const __half2*>(sc + 512 + lane * 4)) * a.scale2;
+        const float ks1 = __low2float(*reinterpret_cast<const __half2*>(sc + 640 + lane * 4)) * a.scale2;
+        bool over = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          s[nt][0] = t0 + r <= lim[nt][0] ? s[nt][0] * ks0 : -INFINITY;
+          s[nt][1] = t0 + r <= lim[nt][1] ? s[nt][1] * ks0 : -INFINITY;
+          s[nt][2] = t0 + r + 8 <= lim[nt][0] ? s[nt][2] * ks1 : -INFINITY;
+          s[nt][3] = t0 + r + 8 <= lim[nt][1] ? s[nt][3] * ks1 : -INFINITY;
+          over = over || fmaxf(s[nt][0], s[nt][2]) > m[nt][0] + 6.f || fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + 6.f;
+        }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              float top = fmaxf(s[nt][e], s[nt][e + 2]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              top = fmaxf(top, m[nt][e]);
+              const float fade = top == m[nt][e] ? 1.f : ks_ex2(m[nt][e] - top);
+              m[nt][e] = top;
+              l[nt][e] *= fade;
+#pragma unroll
+              for (int k = 0; k < MT; k++) { o[nt][k][e] *= fade; o[nt][k][e + 2] *= fade; }
+            }
+        }
+        uint32_t w[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+          const float e0 = ks_ex2(s[nt][0] - b0), e1 = ks_ex2(s[nt][1] - b1), e2 = ks_ex2(s[nt][2] - b0), e3 = ks_ex2(s[nt][3] - b1);
+          l[nt][0] += e0 + e2;
+          l[nt][1] += e1 + e3;
+          w[nt][0] = ks_transpose(ks_half2(__floats2half2_rn(e0, e1)));
+          w[nt][1] = ks_transpose(ks_half2(__floats2half2_rn(e2, e3)));
+        }
+        // outputs
+        const unsigned char* vs = stage + Cfg::K_BYTES + lane * VB;
+        const uint2 sv0 = *reinterpret_cast<const uint2*>(sc + lane * 8), sv1 = *reinterpret_cast<const uint2*>(sc + 256 + lane * 8);
+        const uint32_t p0_ = __byte_perm(sv0.x, sv0.y, 0x7632), p1_ = __byte_perm(sv1.x, sv1.y, 0x7632);
+        const __half2 scale0 = *reinterpret_cast<const __half2*>(&p0_), scale1 = *reinterpret_cast<const __half2*>(&p1_);
+        uint32_t v[4][VB / 4];
+#pragma unroll
+        for (int h = 0; h < 4; h++) {
+          if (VB == 16) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vs + h * VB * 32);
+            v[h][0] = x.x; v[h][1] = x.y; v[h][VB / 4 - 2] = x.z; v[h][VB / 4 - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(vs + h * VB * 32);
+            v[h][0] = x.x; v[h][1] = x.y;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < VB / 4; e++)
+#pragma unroll
+          for (int half = 0; half < 2; half++) {
+            const uint32_t lo = __byte_perm(v[0][e], v[1][e], half ? 0x7362 : 0x5140), hi = __byte_perm(v[2][e], v[3][e], half ? 0x7362 : 0x5140);
+            __half2 a0, a1, a2, a3;
+            kvq_widen<FMT>(lo, a0, a1);
+            kvq_widen<FMT>(hi, a2, a3);
+            a0 = __hmul2_rn(a0, scale0); a1 = __hmul2_rn(a1, scale0);
+            a2 = __hmul2_rn(a2, scale1); a3 = __hmul2_rn(a3, scale1);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+              ks_mma(o[nt][2 * e + half], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), w[nt][0], w[nt][1]);
+          }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+      // ---- the warps' sums meet (their outputs lie over the ring)
+      float* so = reinterpret_cast<float*>(ks_raw);  // [warp][column][hd]
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float sum = l[nt][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          const int col = nt * 8 + 2 * c + e;
+          if (r == 0) { s_m[warp][col] = m[nt][e]; s_l[warp][col] = sum; }
+          float* to = so + ((size_t)warp * COLS + col) * HD + r * VB;
+#pragma unroll
+          for (int k = 0; k < MT; k++) *reinterpret_cast<float2*>(to + 2 * k) = make_float2(o[nt][k][e], o[nt][k][e + 2]);
+        }
+      __syncthreads();
+      const bool whole = j0 == 0 && j1 == n_units;
+      float* part = whole ? nullptr : a.part + (size_t)(2 * blockIdx.x + (j0 == 0 ? 1 : 0)) * Cfg::PART;
+      auto store = [&](int idx, const float (&x)[4]) {  // four finished values of a column
+        const int col = idx / HD, i = col / a.n_rep;
+        const long long row = row0 + (long long)i * a.step;
+        if (col >= n_cols || row < 0 || row >= a.R) return;
+        const bool outside = !NEW && (bt == nullptr || (long long)p0 + i >= a.limit || (long long)p0 + i < 0);
+        const __half2 h0 = __floats2half2_rn(outside ? 0.f : x[0], outside ? 0.f : x[1]), h1 = __floats2half2_rn(outside ? 0.f : x[2], outside ? 0.f : x[3]);
+        *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)(g * a.n_rep + col % a.n_rep) * HD + idx % HD) = make_uint2(ks_half2(h0), ks_half2(h1));
+      };
+      for (int idx = tid * 4; idx < COLS * HD; idx += KS_THREADS * 4) {
+        const int col = idx / HD;
+        float top = NEW && entry ? s_m[KS_WARPS][col] : -INFINITY;
+#pragma unroll
+        for (int w = 0; w < KS_WARPS; w++) top = fmaxf(top, s_m[w][col]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < KS_WARPS; w++) {
+          const float f = ks_ex2(s_m[w][col] - base);
+          const float4 y = *reinterpret_cast<const float4*>(so + (size_t)w * COLS * HD + idx);
+          sum = fmaf(s_l[w][col], f, sum);
+          x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
+        }
+        if (NEW && entry) {
+          const float f = ks_ex2(s_m[KS_WARPS][col] - base);
+          const uint2 y = *reinterpret_cast<const uint2*>(&s_new[1][idx % HD]);
+          const float2 y0 = h2_to_f2(y.x), y1 = h2_to_f2(y.y);
+          sum += f;
+          x[0] = fmaf(y0.x, f, x[0]); x[1] = fmaf(y0.y, f, x[1]); x[2] = fmaf(y1.x, f, x[2]); x[3] = fmaf(y1.y, f, x[3]);
+        }
+        if (whole) {
+          const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+          x[0] *= inv; x[1] *= inv; x[2] *= inv; x[3] *= inv;
+          store(idx, x);
+        } else {
+          __stcg(reinterpret_cast<float4*>(part + idx), make_float4(x[0], x[1], x[2], x[3]));
+          if (idx % HD == 0) { __stcg(part + COLS * HD + col, top); __stcg(part + COLS * HD + COLS + col, sum); }
+        }
+      }
+      if (whole) { __syncthreads(); continue; }
+      // ---- pieces of a (sequence, kv head) that CTAs c_lo .. c_hi share: the last to arrive adds them up in this order
+      const long long last = item + n_units - 1;
+      const int c_lo = (int)(((item + 1) * ctas - 1) / total), c_hi = (int)(((last + 1) * ctas - 1) / total), pieces = c_hi - c_lo + 1;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_ticket = atomicAdd(&a.tickets[c_lo], 1u);
+      __syncthreads();
+      if (s_ticket != (unsigned)(pieces - 1)) continue;
+      __threadfence();
+      if (tid == 0) a.tickets[c_lo] = 0;
+      auto piece = [&](int p) -> const float* { return a.part + (size_t)(2 * (c_lo + p) + (p == 0 ? 1 : 0)) * Cfg::PART; };
+      float* weight = so;  // [column][pieces], at most 2^13 of them: see the launch
+      for (int col = warp; col < COLS; col += KS_WARPS) {
+        float top = -INFINITY, sum = 0.f;
+        for (int p = lane; p < pieces; p += 32) top = fmaxf(top, __ldcg(piece(p) + COLS * HD + col));
+        top = warp_max(top);
+        const float base = top == -INFINITY ? 0.f : top;
+        for (int p = lane; p < pieces; p += 32) {
+          const float f = ks_ex2(__ldcg(piece(p) + COLS * HD + col) - base);
+          weight[col * pieces + p] = f;
+          sum = fmaf(__ldcg(piece(p) + COLS * HD + COLS + col), f, sum);
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) s_l[0][col] = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+      }
+      __syncthreads();
+      for (int idx = tid * 4; idx < COLS * HD; idx += KS_THREADS * 4) {
+        const int col = idx / HD;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int p = 0; p < pieces; p++) {
+          const float f = weight[col * pieces + p];
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(piece(p) + idx));
+          x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
+        }
+        const float inv = s_l[0][col];
+        x[0] *= inv; x[1] *= inv; x[2] *= inv; x[3] *= inv;
+        store(idx, x);
+      }
+      __syncthreads();
+    }
+    at += (long long)n_units * a.c.G;
+  }
+}
+
+// CTAs that a device runs at once, which is also how many pieces and tickets the workspace has.
+static inline int ks_ctas(const jg_dev* dev) { return 2 * dev->sm_count; }
+static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 2>::PART : KsCfg<128, 2>::PART; }
+
+template <int FMT, int HD, int NT, bool NEW>
+static int launch_split(jg_dev* dev, const KvqSplitArgs& a) {
+  auto kern = kvq_split_kernel<FMT, HD, NT, NEW>;
+  static bool attr_set[8] = {};
+  if (!attr_set[dev->ordinal & 7]) {
+    JG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KsCfg<HD, NT>::SMEM));
+    attr_set[dev->ordinal & 7] = true;
+  }
+  const long long most = (long long)a.B * a.c.G * ((a.c.max_ctx + KS_UNIT - 1) / KS_UNIT);
+  return jg_launch(dev, NEW ? "kvq_decode" : "kvq_attn", kern, dim3((unsigned)(most < ks_ctas(dev) ? most : ks_ctas(dev))), dim3(KS_THREADS), KsCfg<HD, NT>::SMEM, a);
+}
+#endif
