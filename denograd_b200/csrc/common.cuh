@@ -26,6 +26,7 @@ struct jg_dev {
                     // launch is the one that has to allocate it, and read without a copy
   float* pair_slots;    // gemm_pair.cuh: accumulators of tiles that several CTA pairs share, and their flags; allocated on first use
   uint32_t* pair_flags;
+  void (*on_error)(jg_dev*);  // clears what a launch that gave up left behind (kvquant.cu), or null
   bool tc_pending;  // such kernels were launched, or replayed from a graph, since the word was last checked
   bool tc_before_capture;  // tc_pending as it was when the capture in progress began
   bool peer_pending;  // peer-memory reductions (comm.cu) were launched since their error word was last checked

@@ -119,6 +119,7 @@ int jg_check_device_errors(jg_dev* dev) {
   if (code != 0) {
     *(volatile int*)dev->err_word = 0;
     jg_pair_reset(dev);
+    if (dev->on_error) dev->on_error(dev);
     jg_set_error("a device-side wait gave up (code %d: 1 = TMA producer, 2 = MMA issuer, 3 = epilogue of a tensor-core "
                  "projection, 4 = grid barrier of the single-kernel decode step); results since the last synchronisation "
                  "are invalid", code);

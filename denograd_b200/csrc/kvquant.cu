@@ -2,9 +2,23 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <mutex>
+
+#include "kvquant_chunk.cuh"
 #include "kvquant_split.cuh"
 
 // ------------------------------------------------------------------------------------------------ the object
+static inline int kvq_tickets(const jg_dev* dev) { return ks_ctas(dev) > kc_ctas(dev) ? ks_ctas(dev) : kc_ctas(dev); }
+
+// Every cache, so that tickets which a launch that gave up left behind are cleared with its error.
+static std::mutex g_lock;
+static jg_kvq* g_all = nullptr;
+static void kvq_on_error(jg_dev* dev) {
+  std::lock_guard<std::mutex> lock(g_lock);
+  for (jg_kvq* kv = g_all; kv != nullptr; kv = kv->next)
+    if (kv->dev == dev) cudaMemsetAsync(kv->tickets, 0, kvq_tickets(dev) * sizeof(unsigned int), dev->stream);
+}
+
 JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t format, jg_kvq** out) {
   JG_ENTER(dev);
   JG_REQUIRE(desc != nullptr && out != nullptr, "kvq_create: null argument");
@@ -32,7 +46,9 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
   if (e == cudaSuccess) e = cudaMalloc(&kv->v_codes, codes);
   if (e == cudaSuccess) e = cudaMalloc(&kv->scales, rows * sizeof(__half2));
   if (e == cudaSuccess) e = cudaMalloc(&kv->block_table, table);
-  const size_t part = (size_t)2 * ks_ctas(dev) * ks_part_floats(d.head_dim) * sizeof(float), tickets = (size_t)ks_ctas(dev) * sizeof(unsigned int);
+  // one workspace for both kernels: launches of a device follow one another, and each leaves the tickets at zero
+  const size_t few = (size_t)2 * ks_ctas(dev) * ks_part_floats(d.head_dim), many = (size_t)2 * kc_ctas(dev) * kc_part_floats(d.head_dim);
+  const size_t part = (few > many ? few : many) * sizeof(float), tickets = (size_t)kvq_tickets(dev) * sizeof(unsigned int);
   if (e == cudaSuccess) e = cudaMalloc(&kv->part, part);
   if (e == cudaSuccess) e = cudaMalloc(&kv->tickets, tickets);
   int32_t* ids = (int32_t*)malloc(table);
@@ -60,6 +76,12 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
     return jg_cuda_fail(e, "kvq_create", __FILE__, __LINE__);
   }
   kv->bytes = 2 * codes + rows * sizeof(__half2) + table + part + tickets;
+  {
+    std::lock_guard<std::mutex> lock(g_lock);
+    kv->next = g_all;
+    g_all = kv;
+    dev->on_error = kvq_on_error;
+  }
   *out = kv;
   return JG_OK;
 }
@@ -69,6 +91,11 @@ static void kvq_destroy_now(void* p) { jg_kvq_destroy((jg_kvq*)p); }
 JG_API int jg_kvq_destroy(jg_kvq* kv) {
   if (!kv) return JG_OK;
   if (g_jg_capturing > 0) { jg_defer(kvq_destroy_now, kv); return JG_OK; }
+  {
+    std::lock_guard<std::mutex> lock(g_lock);
+    for (jg_kvq** at = &g_all; *at != nullptr; at = &(*at)->next)
+      if (*at == kv) { *at = kv->next; break; }
+  }
   cudaSetDevice(kv->dev->ordinal);
   cudaStreamSynchronize(kv->dev->stream);
   cudaFree(kv->k_codes); cudaFree(kv->v_codes); cudaFree(kv->scales); cudaFree(kv->block_table);
@@ -228,7 +255,7 @@ JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint6
   JG_REQUIRE(kv != nullptr && kv->dev == dev, "kvq_read: cache belongs to another device");
   JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_read: layer %d out of range", layer);
   const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
-  JG_REQUIRE(R > 0 && max_count > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
+  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ld >= G * hd && ld % 8 == 0, "kvq_read: rows of %d elements are no multiple of 8 or too short", ld);
   JG_REQUIRE(jg_aligned(k, 16) && jg_aligned(v, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_read: null or misaligned pointer");

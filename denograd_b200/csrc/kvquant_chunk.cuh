@@ -1,0 +1,26 @@
+// The tensor-core form of attention over the 8-bit cache: its arguments and the size of its workspace (kvquant_chunk.cu).
+#pragma once
+#include "kvquant.cuh"
+
+struct KvqChunkArgs {
+  KvqLayer c;
+  const __half* q;
+  __half* out;
+  const int32_t* pos;
+  const int32_t* count;
+  const int32_t* first;
+  const int32_t* seq;
+  int ldq, ldo, R, B, n_rep, max_count, step;
+  int max_tiles;          // items that max_count positions make
+  int grain;              // key tiles that a CTA has at least, where there are so many
+  float scale2;           // log2 e / sqrt(hd)
+  float* part;            // [2 * CTAs][kc_part_floats]
+  unsigned int* tickets;  // [CTAs], zero between launches
+  int* err;
+};
+
+constexpr int KC_ROWS = 256, KC_KEYS = 128;  // query rows of an item, keys of a tile
+static inline int kc_ctas(const jg_dev* dev) { return dev->sm_count; }
+__host__ __device__ constexpr size_t kc_part_floats(int hd) { return (size_t)KC_ROWS * (hd + 2); }  // outputs, maxima, sums
+
+int kvq_chunk(jg_dev* dev, int format, int hd, const KvqChunkArgs& a);

@@ -27,6 +27,7 @@ __attribute__((visibility("default"))) int fake_launches = 0;
 cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t*, const void*, void**) { fake_launches++; return cudaSuccess; }
 cudaError_t cudaLaunchKernel(const void*, dim3, dim3, void**, size_t, cudaStream_t) { return cudaSuccess; }
 cudaError_t cudaFuncSetAttribute(const void*, cudaFuncAttribute, int) { return cudaSuccess; }
+cudaError_t cudaFuncGetAttributes(cudaFuncAttributes* a, const void*) { a->numRegs = 128; return cudaSuccess; }
 cudaError_t cudaGetLastError() { return cudaSuccess; }
 void __cudaRegisterFunction(void**, const char*, char*, const char*, int, uint3*, uint3*, dim3*, dim3*, int*) {}
 cudaError_t __cudaPopCallConfiguration(dim3*, dim3*, size_t*, void*) { return cudaSuccess; }
@@ -113,9 +114,9 @@ CALLS = {
     "decode": (dict(layer=1, out=P, ldo=512, qkv=P, ldx=768, table=P, table_rows=9, pos=P, seq=P, B=5, H=8),
                dict(layer=[-1, 2], out=[0, P + 2], ldo=[504, 513], qkv=[0, P + 8], ldx=[760, 772], table=[P + 4], table_rows=[0, -1], pos=[0, P + 1], seq=[P + 2], B=[0, -1, 65536], H=[4, 0])),
     "attn": (dict(layer=1, out=P, ldo=512, q=P, ldq=512, R=20, pos=P, count=P, first=P, seq=P, B=5, max_count=4, step=1, H=8),
-             dict(layer=[-1, 2], out=[0, P + 2], ldo=[504, 513], q=[0, P + 8], ldq=[504, 515], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4], H=[4, 0])),
+             dict(layer=[-1, 2], out=[0, P + 2], ldo=[504, 513], q=[0, P + 8], ldq=[504, 515], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 65], H=[4, 0])),
     "read": (dict(layer=1, k=P, v=P, ld=128, R=20, pos=P, count=P, first=P, seq=P, B=5, max_count=4, step=1),
-             dict(layer=[-1, 2], k=[0, P + 2], v=[0, P + 8], ld=[120, 129], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 2 ** 31 - 1])),
+             dict(layer=[-1, 2], k=[0, P + 2], v=[0, P + 8], ld=[120, 129], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 65, 2 ** 31 - 1])),
 }
 
 
