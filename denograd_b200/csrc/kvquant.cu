@@ -30,9 +30,11 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
   JG_REQUIRE(d.page_size == 16 || d.page_size == 32 || d.page_size == 64, "kvq_create: page_size %d not in {16,32,64}", d.page_size);
   JG_REQUIRE(d.n_heads % d.n_kv_heads == 0 && d.n_heads / d.n_kv_heads <= 8,
              "kvq_create: %d query heads for %d kv heads: 1 to 8 to each are supported", d.n_heads, d.n_kv_heads);
+  // what 32-bit indexes hold: query rows of a chunk, tiles of an item's heads, rows of a layer's pool
   JG_REQUIRE(d.n_heads <= 4096, "kvq_create: %d heads", d.n_heads);
-  JG_REQUIRE((long long)d.max_batch * d.max_pages_per_seq <= 0x7fffffffLL && (long long)d.max_pages_per_seq * d.page_size <= 0x7fffffffLL,
-             "kvq_create: block table too large");
+  JG_REQUIRE((long long)d.max_batch * d.max_pages_per_seq <= 0x7fffffffLL && (long long)d.max_pages_per_seq * d.page_size <= (1 << 24),
+             "kvq_create: block table too large, or more than 2^24 positions to a slot");
+  JG_REQUIRE((unsigned long long)d.n_pages * d.n_kv_heads * d.page_size <= 0xffffffffull, "kvq_create: pool too large");
   JG_REQUIRE(!dev->capturing, "kvq_create: a graph capture is in progress");
   jg_kvq* kv = new jg_kvq();
   memset(kv, 0, sizeof(*kv));
@@ -255,7 +257,7 @@ JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint6
   JG_REQUIRE(kv != nullptr && kv->dev == dev, "kvq_read: cache belongs to another device");
   JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_read: layer %d out of range", layer);
   const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
-  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
+  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && step > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ld >= G * hd && ld % 8 == 0, "kvq_read: rows of %d elements are no multiple of 8 or too short", ld);
   JG_REQUIRE(jg_aligned(k, 16) && jg_aligned(v, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_read: null or misaligned pointer");

@@ -4,6 +4,7 @@
 // tensor cores (kvquant_chunk.cu).  Both compute o = sum_t w_t v_t / sum_t w_t with w_t = e^(s_t - max), s_t = q.k_t / sqrt(hd), in one pass with a
 // running maximum; w is rounded to fp16 for the product with V and summed as it was.
 #include <math.h>
+#include <stdlib.h>
 
 #include "kvquant_chunk.cuh"
 #include "kvquant_split.cuh"
@@ -38,7 +39,7 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_attn: layer %d out of range", layer);
   const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
   JG_REQUIRE(H == kv->d.n_heads, "kvq_attn: H=%d does not match the cache (n_heads %d)", H, kv->d.n_heads);
-  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_attn: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
+  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && step > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_attn: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
@@ -64,7 +65,7 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   a.pos = (const int32_t*)pos; a.count = (const int32_t*)count; a.first = (const int32_t*)first; a.seq = (const int32_t*)seq;
   a.ldq = ldq; a.ldo = ldo; a.R = R; a.B = B; a.n_rep = H / G; a.max_count = max_count; a.step = step;
   a.max_tiles = (int)(((long long)max_count * (H / G) + KC_ROWS - 1) / KC_ROWS);
-  a.grain = 1;
+  a.grain = getenv("JG_KC_GRAIN") ? atoi(getenv("JG_KC_GRAIN")) : 1;
   a.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
   a.part = kv->part; a.tickets = kv->tickets; a.err = dev->err_word;
   return kvq_chunk(dev, kv->format, hd, a);

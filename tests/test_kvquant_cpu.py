@@ -75,7 +75,8 @@ def kv(lib, dev):
 
 
 @pytest.mark.parametrize("kw,fmt", [({"head_dim": 96}, 0), ({"page_size": 48}, 0), ({"n_heads": 7}, 0), ({"n_heads": 18}, 0), ({"n_layers": 0}, 0), ({"n_pages": 0}, 1),
-                                    ({"max_batch": 1 << 20, "max_pages_per_seq": 1 << 12}, 0), ({"max_pages_per_seq": 1 << 28, "max_batch": 1}, 0), ({}, 2), ({}, -1)])
+                                    ({"max_batch": 1 << 20, "max_pages_per_seq": 1 << 12}, 0), ({"max_pages_per_seq": 1 << 28, "max_batch": 1}, 0), ({}, 2), ({}, -1),
+                                    ({"max_pages_per_seq": (1 << 20) + 1, "max_batch": 1}, 0), ({"n_pages": 1 << 30, "n_kv_heads": 8}, 0)])
 def test_create_refuses(lib, dev, kw, fmt):
     h = C.c_void_p()
     assert lib.jg_kvq_create(dev, C.byref(desc(**kw)), fmt, C.byref(h)) == ffi.JG_EINVAL
@@ -114,9 +115,9 @@ CALLS = {
     "decode": (dict(layer=1, out=P, ldo=512, qkv=P, ldx=768, table=P, table_rows=9, pos=P, seq=P, B=5, H=8),
                dict(layer=[-1, 2], out=[0, P + 2], ldo=[504, 513], qkv=[0, P + 8], ldx=[760, 772], table=[P + 4], table_rows=[0, -1], pos=[0, P + 1], seq=[P + 2], B=[0, -1, 65536], H=[4, 0])),
     "attn": (dict(layer=1, out=P, ldo=512, q=P, ldq=512, R=20, pos=P, count=P, first=P, seq=P, B=5, max_count=4, step=1, H=8),
-             dict(layer=[-1, 2], out=[0, P + 2], ldo=[504, 513], q=[0, P + 8], ldq=[504, 515], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 65], H=[4, 0])),
+             dict(layer=[-1, 2], out=[0, P + 2], ldo=[504, 513], q=[0, P + 8], ldq=[504, 515], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 65], step=[0, -1], H=[4, 0])),
     "read": (dict(layer=1, k=P, v=P, ld=128, R=20, pos=P, count=P, first=P, seq=P, B=5, max_count=4, step=1),
-             dict(layer=[-1, 2], k=[0, P + 2], v=[0, P + 8], ld=[120, 129], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 65, 2 ** 31 - 1])),
+             dict(layer=[-1, 2], k=[0, P + 2], v=[0, P + 8], ld=[120, 129], R=[0, -1], pos=[0, P + 1], count=[P + 1], first=[P + 2], seq=[P + 3], B=[0, -1, 65536], max_count=[0, -4, 65, 2 ** 31 - 1], step=[0, -1])),
 }
 
 
