@@ -4,7 +4,6 @@
 // tensor cores (kvquant_chunk.cu).  Both compute o = sum_t w_t v_t / sum_t w_t with w_t = e^(s_t - max), s_t = q.k_t / sqrt(hd), in one pass with a
 // running maximum; w is rounded to fp16 for the product with V and summed as it was.
 #include <math.h>
-#include <stdlib.h>
 
 #include "kvquant_chunk.cuh"
 #include "kvquant_split.cuh"
@@ -65,7 +64,7 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   a.pos = (const int32_t*)pos; a.count = (const int32_t*)count; a.first = (const int32_t*)first; a.seq = (const int32_t*)seq;
   a.ldq = ldq; a.ldo = ldo; a.R = R; a.B = B; a.n_rep = H / G; a.max_count = max_count; a.step = step;
   a.max_tiles = (int)(((long long)max_count * (H / G) + KC_ROWS - 1) / KC_ROWS);
-  a.grain = getenv("JG_KC_GRAIN") ? atoi(getenv("JG_KC_GRAIN")) : 1;
+  JG_REQUIRE((long long)B * a.max_tiles <= (1 << 26), "kvq_attn: B=%d sequences of up to %d positions are too many for one call", B, max_count);
   a.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
   a.part = kv->part; a.tickets = kv->tickets; a.err = dev->err_word;
   return kvq_chunk(dev, kv->format, hd, a);

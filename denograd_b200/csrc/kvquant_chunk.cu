@@ -27,6 +27,8 @@ constexpr int KC_THREADS = 640, KC_REGS = 96;                                 //
 constexpr int KC_SOFT_REGS = 144, KC_WIDEN_REGS = 72, KC_MMA_REGS = 48;       // and from then on, by warpgroup
 static_assert(2 * KC_SOFT_REGS + 2 * KC_WIDEN_REGS + KC_MMA_REGS <= 5 * KC_REGS, "register shares exceed what a CTA is launched with");
 constexpr int KC_PLAN = 4;  // pieces that the plan is ahead
+constexpr int KC_HALF = KC_KEYS / 2;  // keys of a step of the softmax
+constexpr int KC_WHOLE = 8, KC_GRAIN = 6;
 
 template <int HD>
 struct KcCfg {
@@ -70,25 +72,39 @@ __device__ __forceinline__ float kc_max3(float x, float y, float z) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
 }
-// the larger of m and v[0 .. N)
-template <int N>
-__device__ __forceinline__ float kc_max(float m, const float* v) {
-  float t0 = m, t1 = v[0];
+__device__ __forceinline__ float kc_max64(const float* v) {  // in four chains
+  float t0 = v[0], t1 = v[1], t2 = v[2], t3 = v[3];
 #pragma unroll
-  for (int c = 1; c + 3 < N; c += 4) { t0 = kc_max3(t0, v[c], v[c + 1]); t1 = kc_max3(t1, v[c + 2], v[c + 3]); }
-#pragma unroll
-  for (int c = (N - 1) / 4 * 4 + 1; c < N; c++) t0 = fmaxf(t0, v[c]);
-  return fmaxf(t0, t1);
+  for (int c = 4; c + 8 <= 60; c += 8) {
+    t0 = kc_max3(t0, v[c], v[c + 1]);
+    t1 = kc_max3(t1, v[c + 2], v[c + 3]);
+    t2 = kc_max3(t2, v[c + 4], v[c + 5]);
+    t3 = kc_max3(t3, v[c + 6], v[c + 7]);
+  }
+  t0 = kc_max3(t0, v[60], v[61]);
+  t1 = kc_max3(t1, v[62], v[63]);
+  return fmaxf(kc_max3(t0, t1, t2), t3);
 }
-// (x, y) * (s, s) + (t, t), and sums of pairs
-__device__ __forceinline__ float2 kc_fma2(float x, float y, float s, float t) {
-  float2 r;
-  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "=f"(r.x), "=f"(r.y) : "f"(x), "f"(y), "f"(s), "f"(t));
+// pairs of floats: packed operands stay in register pairs, made once where they do not change
+__device__ __forceinline__ uint64_t kc_pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
   return r;
 }
-__device__ __forceinline__ void kc_add2(float2& s, float x, float y) {
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "+f"(s.x), "+f"(s.y) : "f"(x), "f"(y));
+__device__ __forceinline__ float2 kc_split(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t kc_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t kc_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 // Sixteen codes as halves times their row's scale.  int8: (1024 + 128 + code) s - 1152 s is exact in one operation, as long as 1152 s
 // is a half (`small`).
@@ -121,16 +137,17 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   unsigned char* sQ = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(kc_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sK = sQ + 2 * Cfg::Q_BYTES;
   unsigned char* sV = sK + 2 * Cfg::KV_BYTES;
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_low[2], p_high[2], o_full[2], q_full[2], met, plan_full[KC_PLAN], plan_empty[KC_PLAN];
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2][2], q_full[2], met, plan_full[KC_PLAN], plan_empty[KC_PLAN];
   __shared__ KcPiece s_plan[KC_PLAN];
   __shared__ uint32_t s_tmem;
   __shared__ unsigned int s_ticket;
-  __shared__ long long s_sum[KC_THREADS / 32], s_find[2];
+  __shared__ long long s_sum[KC_THREADS / 32], s_at;
+  __shared__ int s_longest[KC_THREADS / 32], s_entry;
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp();
   if (tid == 0) {
     for (int i = 0; i < 2; i++) {
-      mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], 1); mbar_init(&s_full[i], 1);
-      mbar_init(&p_low[i], 4); mbar_init(&p_high[i], 4); mbar_init(&o_full[i], 1); mbar_init(&q_full[i], 4);
+      mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 4); mbar_init(&v_empty[i], 1); mbar_init(&s_full[i], 1); mbar_init(&q_full[i], 4);
+      for (int half = 0; half < 2; half++) { mbar_init(&p_full[i][half], 4); mbar_init(&o_full[i][half], 1); }  // [stream][half of a key tile]
     }
     mbar_init(&met, 8);
     for (int i = 0; i < KC_PLAN; i++) { mbar_init(&plan_full[i], 1); mbar_init(&plan_empty[i], 17); }  // all warps but the plan's own and the last two
@@ -148,46 +165,60 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   pdl_launch();  // only now: see tcgen05.cuh
   pdl_wait();
 
-  // ---- the line of tiles: how long it is, and where this CTA's stretch begins.  Entry e = (sequence, item of it), all kv heads.
-  const long long entries = (long long)a.B * a.max_tiles;
-  auto weight = [&](long long e) -> long long {
+  // ---- the line of tiles: how long it is, and where this CTA's stretch begins.  Entry e = (sequence, item of it), all kv heads.  Up to 32
+  // entries are the plan's own business; more are looked at by all threads.
+  const int entries = a.B * a.max_tiles;
+  auto tiles_of = [&](int e) -> int {
     KcPiece p;
-    if (e >= entries) return 0;
-    const int b = a.max_tiles == 1 ? (int)e : (int)(e / a.max_tiles);
-    return (long long)kc_item(a, b, (int)(e - (long long)b * a.max_tiles), p) * a.c.G;
+    return e < entries ? kc_item(a, e / a.max_tiles, e % a.max_tiles, p) : 0;
   };
-  const long long w_first = weight(tid);
-  long long total = w_first;
-  for (long long e = tid + KC_THREADS; e < entries; e += KC_THREADS) total += weight(e);
+  auto warp_sum64 = [&](long long v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) s_sum[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < KC_THREADS / 32; w++) total += s_sum[w];
-  const int ctas = (int)max(1ll, min((long long)gridDim.x, (total + a.grain - 1) / a.grain));
-  const long long u_lo = (int)blockIdx.x < ctas ? blockIdx.x * total / ctas : 0, u_hi = (int)blockIdx.x < ctas ? (blockIdx.x + 1) * total / ctas : 0;
-  long long before = 0;
-  for (long long base = 0; base < entries && u_lo < u_hi; base += KC_THREADS) {  // the same for all threads
-    const long long mine = base == 0 ? w_first : weight(base + tid);
-    long long sum = mine;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto scan64 = [&](long long v) {  // of this lane and those below it
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long below = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += below;
+      const long long below = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += below;
+    }
+    return v;
+  };
+  // Cutting an item costs its CTAs a trip through memory each, 2 to 4 us: short items are not cut, others not into less than KC_GRAIN tiles.
+  long long total = 0, u_lo = 0, u_hi = 0;
+  int longest = 0, ctas = 1;
+  auto share = [&]() {
+    const long long most = longest <= KC_WHOLE ? total : total / KC_GRAIN;
+    ctas = (int)max(1ll, min((long long)gridDim.x, most));
+    if ((int)blockIdx.x < ctas) { u_lo = blockIdx.x * total / ctas; u_hi = (blockIdx.x + 1) * total / ctas; }
+  };
+  if (entries > 32) {
+    for (int e = tid; e < entries; e += KC_THREADS) {
+      const int n = tiles_of(e);
+      total += (long long)n * a.c.G;
+      longest = max(longest, n);
+    }
+    total = warp_sum64(total);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) { s_sum[warp] = total; s_longest[warp] = longest; }
+    __syncthreads();
+    total = 0;
+    for (int w = 0; w < KC_THREADS / 32; w++) { total += s_sum[w]; longest = max(longest, s_longest[w]); }
+    share();
+    long long before = 0;
+    for (int base = 0; base < entries && u_lo < u_hi; base += KC_THREADS) {  // the same for all threads
+      const long long mine = (long long)tiles_of(base + tid) * a.c.G, sum = scan64(mine);
+      __syncthreads();
+      if (lane == 31) s_sum[warp] = sum;
+      __syncthreads();
+      long long ahead = before;
+      for (int w = 0; w < KC_THREADS / 32; w++) { ahead += w < warp ? s_sum[w] : 0; before += s_sum[w]; }
+      if (ahead + sum - mine <= u_lo && u_lo < ahead + sum) { s_at = ahead + sum - mine; s_entry = base + tid; }
+      if (before > u_lo) break;
     }
     __syncthreads();
-    if (lane == 31) s_sum[warp] = sum;
-    __syncthreads();
-    long long ahead = before;
-    for (int w = 0; w < warp; w++) ahead += s_sum[w];
-    if (ahead + sum - mine <= u_lo && u_lo < ahead + sum) { s_find[0] = ahead + sum - mine; s_find[1] = base + tid; }
-#pragma unroll
-    for (int w = 0; w < KC_THREADS / 32; w++) before += s_sum[w];
-    if (before > u_lo) break;
   }
-  __syncthreads();
 
   bool ok = true;
   uint32_t planned = 0;
@@ -205,35 +236,50 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KC_MMA_REGS));
     if (warp == 17) {
       // ---- the plan: a walk along this CTA's stretch of the line
-      long long u = u_lo, at = u_lo < u_hi ? s_find[0] : 0;  // at: first tile of (b, tile, head 0)
-      int b = 0, tile = 0;
-      if (u_lo < u_hi) { b = (int)(s_find[1] / a.max_tiles); tile = (int)(s_find[1] % a.max_tiles); }
+      long long at;  // first tile of (b, tile, head 0)
+      int entry;
+      if (entries > 32) {
+        at = s_at;
+        entry = s_entry;
+      } else {
+        longest = tiles_of(lane);
+        const long long mine = (long long)longest * a.c.G, sum = scan64(mine);
+        total = __shfl_sync(0xffffffffu, sum, 31);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        share();
+        entry = max(0, __ffs(__ballot_sync(0xffffffffu, sum > u_lo)) - 1);
+        at = __shfl_sync(0xffffffffu, sum - mine, entry);
+      }
+      const bool cut = longest > KC_WHOLE;
+      long long u = u_lo;
+      int b = entry / a.max_tiles, tile = entry % a.max_tiles;
       for (;; planned++) {
         const uint32_t slot = planned % KC_PLAN;
         if (planned >= KC_PLAN) ok = mbar_wait(&plan_empty[slot], (planned / KC_PLAN - 1) & 1);
         if (!ok) break;
         KcPiece p;
         p.b = -1;
-        if (u < u_hi) {
-          int n;
-          for (;;) {
-            n = kc_item(a, b, tile, p);
-            if (n == 0) { tile = 0; b++; continue; }  // the items of a sequence are its first ones
-            if (u < at + (long long)n * a.c.G) break;
+        while (u < u_hi) {
+          const int n = kc_item(a, b, tile, p);
+          if (n == 0) { tile = 0; b++; continue; }  // the items of a sequence are its first ones
+          if (u >= at + (long long)n * a.c.G) {
             at += (long long)n * a.c.G;
             if (++tile == a.max_tiles) { tile = 0; b++; }
+            continue;
           }
-          p.b = b; p.tile = tile; p.n_tiles = n;
           p.g = (int)(u - at) / n;  // both below 2^31: see the limits of the cache
           const long long item = at + (long long)p.g * n;
           p.j0 = (int)(u - item);
-          p.j1 = (int)min((long long)n, u_hi - item);
+          p.j1 = cut ? (int)min((long long)n, u_hi - item) : n;
           u = item + p.j1;
+          if (!cut && p.j0 > 0) continue;  // begun by the CTA before
+          p.b = b; p.tile = tile; p.n_tiles = n;
           p.c_lo = p.pieces = 0;
           if (p.j1 - p.j0 < n) {
             p.c_lo = (int)(((item + 1) * ctas - 1) / total);
             p.pieces = (int)(((item + n) * ctas - 1) / total) - p.c_lo + 1;
           }
+          break;
         }
         if (lane == 0) { s_plan[slot] = p; ft_arrive(&plan_full[slot]); }
         if (p.b < 0) break;
@@ -243,7 +289,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       // ---- products
       constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(KC_KEYS >> 3) << 17) | (8u << 24);
       constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);
-      uint32_t tiles = 0, loaded[2] = {0, 0}, made[2] = {0, 0};  // key tiles, items and score tiles so far
+      uint32_t tiles = 0, loaded[2] = {0, 0}, made[2] = {0, 0};  // key tiles, items, and key tiles of either stream so far
       auto commit = [&](uint64_t* bar) {
         if (elect_one()) umma_commit(bar);
       };
@@ -261,7 +307,6 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
               umma_f16(tmem + q * 128, da + c * (BLOCK >> 4) + 2 * k, db + c * (BLOCK >> 4) + 2 * k, id_s, (c > 0 || k > 0) ? 1u : 0u);
           umma_commit(&s_full[q]);
         }
-        made[q]++;
       };
       KcPiece p;
       while (next(p)) {
@@ -273,32 +318,27 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         commit(&k_empty[tiles & 1]);
         for (int j = 0; j < n && ok; j++, tiles++) {
           const uint32_t slot = tiles & 1, then = slot ^ 1;
+          const bool more = j + 1 < n;
           wait(&v_full[slot], (tiles >> 1) & 1);
           for (int q = 0; q < streams && ok; q++) {
             const uint64_t db = umma_desc_mn(sV + (size_t)slot * Cfg::KV_BYTES, BLOCK);
-            wait(&p_low[q], (made[q] - 1) & 1);  // the weights of the first 64 keys, then of the others
-            if (!ok) break;
-            if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < KC_KEYS / 32; k++)  // 16 rows of values = 2048 bytes further
-                umma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, db + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
-            }
-            wait(&p_high[q], (made[q] - 1) & 1);
-            if (!ok) break;
-            if (elect_one()) {
+            for (int half = 0; half < 2; half++) {  // a half of the tile's weights at a time
+              wait(&p_full[q][half], made[q] & 1);
+              if (ok && elect_one()) {
 #pragma unroll
-              for (int k = KC_KEYS / 32; k < KC_KEYS / 16; k++)
-                umma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, db + k * 128, id_o, 1u);
-              umma_commit(&o_full[q]);
+                for (int k = half * (KC_HALF / 16); k < (half + 1) * (KC_HALF / 16); k++)  // 16 rows of values = 2048 bytes further
+                  umma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, db + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
+                umma_commit(&o_full[q][half]);
+              }
             }
-            if (j + 1 < n) {
-              if (q == 0) wait(&k_full[then], ((tiles + 1) >> 1) & 1);
-              if (ok) qk(q, then);
-            }
+            if (more && q == 0) wait(&k_full[then], ((tiles + 1) >> 1) & 1);
+            if (more && ok) qk(q, then);
+            made[q]++;
           }
           if (!ok) break;
           commit(&v_empty[slot]);
-          if (j + 1 < n) commit(&k_empty[then]);
+          if (more) commit(&k_empty[then]);
         }
       }
       if (!ok && lane == 0) atomicCAS(a.err, 0, 2);
@@ -306,63 +346,61 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   } else if (warp >= 8) {
     // ---- keys, or values: codes to halves, into 128-byte swizzled rows
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KC_WIDEN_REGS));
-    constexpr int LPR = HD / 16, ROWS = 128 / LPR, N = 128 / ROWS;  // lanes to a row of codes; rows at a time; times
+    // Four lanes take a 64-column block of a row, lanes 4-7 the row behind it: in 128-byte swizzled rows the eight 16-byte pieces that they
+    // write at a time fall on different banks.  A warp has PER neighbouring rows of each of the N groups of ROWS.
+    constexpr int ROWS = HD == 128 ? 16 : 32, N = 128 / ROWS, PER = ROWS / 4;
     const bool values = warp >= 12;
-    const int u = tid & 127, sub = u % LPR, row = u / LPR;
-    const uint8_t* codes = values ? a.c.v : a.c.k;
+    const int u = tid & 127, sub = HD == 128 ? (u & 3) + ((u >> 3) & 1) * 4 : u & 3, row = HD == 128 ? (u >> 4) * 2 + ((u >> 2) & 1) : u >> 2;
+    const uint8_t* codes = (values ? a.c.v : a.c.k) + sub * 16;
     const __half* scales = reinterpret_cast<const __half*>(a.c.scales) + (values ? 1 : 0);
     uint64_t* full = values ? v_full : k_full;
     uint64_t* empty = values ? v_empty : k_empty;
-    unsigned char* tile = values ? sV : sK;
-    // a thread's pieces of a row: columns 16 sub .. are two 16-byte pieces of a block's row.  The upper block's lanes begin with the second,
-    // so that eight lanes write to eight different places of a row.
-    const int c0 = (sub & 3) * 2, flip = HD == 128 ? sub >> 2 : 0;
-    tile += (sub >> 2) * BLOCK + row * 128;
-    const uint32_t o0 = ((c0 + flip) ^ (row & 7)) << 4, o1 = ((c0 + 1 - flip) ^ (row & 7)) << 4;  // (row + 16 i keeps row & 7)
+    unsigned char* tile = (values ? sV : sK) + (sub >> 2) * BLOCK + row * 128;
+    const uint32_t o0 = (((sub & 3) * 2) ^ (row & 7)) << 4, o1 = (((sub & 3) * 2 + 1) ^ (row & 7)) << 4;  // (row + i * ROWS keeps row & 7)
     uint32_t tiles = 0;
     KcPiece p;
     while (next(p)) {
       const int32_t* bt = p.bt ? p.bt : a.c.block_table;  // (a slot outside the cache: some row, nobody sees it)
       const int mask = (1 << a.c.page_shift) - 1, last = max(p.T - 1, 0);
-      // lane l & 7: the page of the tile's positions 16 l ..; positions past the end are the last one, masked
-      auto pages_of = [&](int j) { return bt[min(j * KC_KEYS + (lane & 7) * 16, last) >> a.c.page_shift]; };
+      // Lane l & 7 looks after positions 16 (l & 7) .. of a tile, which lie in one page: its page, and the row of the pool where they begin.
+      // Positions past the end are the last one, masked.
+      auto page_of = [&](int j) { return bt[min(j * KC_KEYS + (lane & 7) * 16, last) >> a.c.page_shift]; };
+      auto first_row = [&](int j, int page) { return ((uint32_t)(page * a.c.G + p.g) << a.c.page_shift) + (uint32_t)(min(j * KC_KEYS + (lane & 7) * 16, last) & mask); };
       uint4 x[N];
-      __half s[N];
-      auto load = [&](int j, int pages) {
+      float s = 0.f;  // lane l: the scale of row (l / PER) * ROWS + l % PER of the warp's rows
+      auto load = [&](int j, int page) {
+        const uint32_t begin = first_row(j, page);
+        const int room = last - j * KC_KEYS;  // rows of the tile up to the last position
+        auto row_at = [&](int r) {  // row of the pool of the tile's row r
+          const uint32_t b0 = __shfl_sync(0xffffffffu, begin, r >> 4);
+          return b0 + (uint32_t)(room >= KC_KEYS - 1 ? r & 15 : max(0, min(r & 15, room - (r & ~15))));
+        };
+        s = __half2float(scales[2 * (size_t)row_at((lane / PER % N) * ROWS + (warp & 3) * PER + lane % PER)]);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-          const int page = __shfl_sync(0xffffffffu, pages, (row + i * ROWS) >> 4);
-          const uint32_t at = ((uint32_t)(page * a.c.G + p.g) << a.c.page_shift) + (uint32_t)(min(j * KC_KEYS + row + i * ROWS, last) & mask);
-          x[i] = ld_stream_128(codes + (size_t)at * HD + sub * 16);
-          s[i] = scales[2 * (size_t)at];
-        }
+        for (int i = 0; i < N; i++) x[i] = ld_stream_128(codes + (size_t)row_at(row + i * ROWS) * HD);
       };
-      int pages = pages_of(p.j0);
-      load(p.j0, pages);
-      if (p.j0 + 1 < p.j1) pages = pages_of(p.j0 + 1);
+      int page = page_of(p.j0);
+      load(p.j0, page);
+      if (p.j0 + 1 < p.j1) page = page_of(p.j0 + 1);
       for (int j = p.j0; j < p.j1; j++, tiles++) {
         const uint32_t slot = tiles & 1;
         if (tiles >= 2) ok = mbar_wait(&empty[slot], ((tiles >> 1) - 1) & 1);
         if (!ok) break;
         unsigned char* to = tile + (size_t)slot * Cfg::KV_BYTES;
-        bool small = true;
-#pragma unroll
-        for (int i = 0; i < N; i++) small = small && !(__half2float(s[i]) > 56.f);
-        small = FMT == KVQ_INT8 && __all_sync(0xffffffffu, small);
+        const bool small = FMT == KVQ_INT8 && __all_sync(0xffffffffu, !(s > 56.f));
 #pragma unroll
         for (int i = 0; i < N; i++) {
-          const __half2 sc = __half2half2(s[i]);
+          const __half2 sc = __float2half2_rn(__shfl_sync(0xffffffffu, s, i * PER + (row & (PER - 1))));
           __half2 h[8];
           kc_widen<FMT>(x[i], sc, __hmul2_rn(sc, __floats2half2_rn(-1152.f, -1152.f)), small, h);
-          const uint4 lo = *reinterpret_cast<const uint4*>(h), hi = *reinterpret_cast<const uint4*>(h + 4);
-          *reinterpret_cast<uint4*>(to + i * ROWS * 128 + o0) = flip ? hi : lo;
-          *reinterpret_cast<uint4*>(to + i * ROWS * 128 + o1) = flip ? lo : hi;
+          *reinterpret_cast<uint4*>(to + i * ROWS * 128 + o0) = *reinterpret_cast<const uint4*>(h);
+          *reinterpret_cast<uint4*>(to + i * ROWS * 128 + o1) = *reinterpret_cast<const uint4*>(h + 4);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) ft_arrive(&full[slot]);
-        if (j + 1 < p.j1) load(j + 1, pages);
-        if (j + 2 < p.j1) pages = pages_of(j + 2);
+        if (j + 1 < p.j1) load(j + 1, page);
+        if (j + 2 < p.j1) page = page_of(j + 2);
       }
     }
     if (!ok && lane == 0) atomicCAS(a.err, 0, 1);
@@ -372,6 +410,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     const int q = warp >> 2, r = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + q * 128, O = lanes + 256 + q * 128;
     unsigned char* rows_at = sQ + (size_t)q * Cfg::Q_BYTES + (warp & 3) * 32 * 128;  // this warp's 32 rows of queries, and of results behind them
+    const uint64_t scale2 = kc_pair(a.scale2, a.scale2);
     uint32_t made = 0, meetings = 0;  // score tiles so far, and times that the two streams have met
     auto meet = [&]() {  // of all softmax warps, with a limit: bar.sync would wait for a warp that gave up
       __syncwarp();
@@ -381,7 +420,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     KcPiece p;
     while (next(p)) {
       const int n = p.j1 - p.j0, rows = p.n * a.n_rep - p.tile * KC_ROWS, mine = q * 128 + r;  // rows of the item, and this thread's
-      const bool active = rows > q * 128;  // the stream has rows at all
+      const bool active = rows > q * 128, idle = rows <= mine - lane;  // the stream has rows at all; this warp has none
       const int i = (p.tile * KC_ROWS + mine) / a.n_rep, h = p.tile * KC_ROWS + mine - i * a.n_rep;
       const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step, pos = (long long)p.p0 + i;
       const bool there = mine < rows && row >= 0 && row < a.R;
@@ -389,25 +428,20 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       const int lim = !there ? p.T - 1 : (int)max(-1ll, min(pos, (long long)p.T - 1));  // last key that the row sees
       const int head = p.g * a.n_rep + h;
       float m = -INFINITY;
-      float2 l = make_float2(0.f, 0.f);
+      uint64_t l0 = kc_pair(0.f, 0.f), l1 = l0;  // the sum, in four parts
       if (active) {
         // the warp's 32 rows, HD / 8 lanes to a row
         const long long from = there ? row * a.ldq + head * HD : -1;
         constexpr int W = HD / 8, PER = 32 / W;
-#pragma unroll
-        for (int k = 0; k < 32; k += PER * 8) {
-          uint4 x[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const long long at = __shfl_sync(0xffffffffu, from, k + e * PER + lane / W);
-            x[e] = at < 0 ? make_uint4(0, 0, 0, 0) : ld_128(a.q + at + lane % W * 8);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const int rr = k + e * PER + lane / W, c = lane % W;
-            *reinterpret_cast<uint4*>(rows_at + (c >> 3) * BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = x[e];
-          }
+#pragma unroll 4
+        for (int k = 0; k < 32; k += PER) {
+          const int rr = k + lane / W, c = lane % W;
+          const long long at = __shfl_sync(0xffffffffu, from, rr);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(smem_u32(rows_at + (c >> 3) * BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4))), "l"(a.q + max(at, 0ll) + c * 8), "r"(at < 0 ? 0 : 16)
+                       : "memory");  // zeros for rows that there are not
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) ft_arrive(&q_full[q]);
@@ -415,82 +449,72 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           ok = mbar_wait(&s_full[q], made & 1);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          // the first 64 scores stay in registers, the others are read twice
-          float v[64], y[32];
-          tmem_ld32(S, v);
-          tmem_ld32(S + 32, v + 32);
-          kc_landed<64>(v);
-          tmem_ld32(S + 64, y);
+          if (idle) {  // whatever lies in the place of its weights concerns rows that nobody stores
+            if (lane == 0) { ft_arrive(&p_full[q][0]); ft_arrive(&p_full[q][1]); }
+            continue;
+          }
+          // Two halves of 64 keys, each a step of its own of the running maximum: the first one's product with V runs while the second is here.
           const int key = (p.j0 + j) * KC_KEYS;
           const bool all = __all_sync(0xffffffffu, key + KC_KEYS - 1 <= lim);
-          auto hide = [&](float* x, int k, int count) {
-            if (all) return;
+          float v[64];
+          tmem_ld32(S, v);
+          tmem_ld32(S + 32, v + 32);
 #pragma unroll
-            for (int c = 0; c < count; c++) x[c] = k + c <= lim ? x[c] : -INFINITY;
-          };
-          hide(v, key, 64);
-          float top = kc_max<64>(-INFINITY, v);
-          kc_landed<32>(y);
-          {
-            float z[32];
-            tmem_ld32(S + 96, z);
-            hide(y, key + 64, 32);
-            top = kc_max<32>(top, y);
-            kc_landed<32>(z);
-            hide(z, key + 96, 32);
-            top = kc_max<32>(top, z);
-          }
-          top *= a.scale2;
-          if (__any_sync(0xffffffffu, top > m + 8.f)) {
-            const float then = fmaxf(m, top), fade = then == m ? 1.f : ft_ex2(m - then);
-            m = then;
-            l.x *= fade;
-            l.y *= fade;
-            if (j > 0) {
-              ok = mbar_wait(&o_full[q], (made - 1) & 1);  // the product before has to be in O
-              if (!ok) break;
-              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          for (int half = 0; half < 2; half++) {
+            kc_landed<64>(v);
+            if (!all) {
+#pragma unroll
+              for (int c = 0; c < 64; c++) v[c] = key + half * 64 + c <= lim ? v[c] : -INFINITY;
+            }
+            const float top = kc_max64(v) * a.scale2;
+            if (__any_sync(0xffffffffu, top > m + 8.f)) {
+              const float then = fmaxf(m, top), fade = then == m ? 1.f : ft_ex2(m - then);
+              m = then;
+              const uint64_t f2 = kc_pair(fade, fade);
+              l0 = kc_fma2(l0, f2, kc_pair(0.f, 0.f));
+              l1 = kc_fma2(l1, f2, kc_pair(0.f, 0.f));
+              if (j > 0 || half > 0) {  // the product before has to be in O
+                ok = half == 0 ? mbar_wait(&o_full[q][1], (made - 1) & 1) : mbar_wait(&o_full[q][0], made & 1);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-              for (int c = 0; c < HD; c += 32) {
-                uint32_t w[32];
-                tmem_ld32(O + c, y);
-                kc_landed<32>(y);
+                for (int c = 0; c < HD; c += 32) {
+                  float y[32];
+                  uint32_t w[32];
+                  tmem_ld32(O + c, y);
+                  kc_landed<32>(y);
 #pragma unroll
-                for (int k = 0; k < 32; k++) w[k] = __float_as_uint(y[k] * fade);
-                tmem_st32(O + c, w);
+                  for (int k = 0; k < 32; k++) w[k] = __float_as_uint(y[k] * fade);
+                  tmem_st32(O + c, w);
+                }
               }
             }
-          }
-          const float base = m == -INFINITY ? 0.f : -m, sc = a.scale2;
-          auto weights = [&](const float* x, uint32_t* w, int count) {
+            const float base = m == -INFINITY ? 0.f : -m;
+            const uint64_t base2 = kc_pair(base, base);
+            uint32_t w[32];
 #pragma unroll
-            for (int k = 0; k < count; k += 2) {
-              const float2 e = kc_fma2(x[k], x[k + 1], sc, base);
-              const float e0 = ft_ex2(e.x), e1 = ft_ex2(e.y);
-              kc_add2(l, e0, e1);
-              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2]) : "f"(e1), "f"(e0));
+            for (int k = 0; k < 64; k += 4) {
+              const float2 x = kc_split(kc_fma2(kc_pair(v[k], v[k + 1]), scale2, base2)), y = kc_split(kc_fma2(kc_pair(v[k + 2], v[k + 3]), scale2, base2));
+              const float x0 = ft_ex2(x.x), x1 = ft_ex2(x.y), y0 = ft_ex2(y.x), y1 = ft_ex2(y.y);
+              l0 = kc_add2(l0, kc_pair(x0, x1));
+              l1 = kc_add2(l1, kc_pair(y0, y1));
+              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2]) : "f"(x1), "f"(x0));
+              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2 + 1]) : "f"(y1), "f"(y0));
             }
-          };
-          auto ready = [&](uint64_t* bar) {
+            tmem_st32(S + half * 32, w);
+            if (half == 0) {
+              tmem_ld32(S + 64, v);
+              tmem_ld32(S + 96, v + 32);
+            }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) ft_arrive(bar);
-          };
-          uint32_t w[32];
-          weights(v, w, 64);
-          tmem_st32(S, w);
-          tmem_ld32(S + 64, v);
-          tmem_ld32(S + 96, v + 32);
-          ready(&p_low[q]);
-          kc_landed<64>(v);
-          hide(v, key + 64, 64);
-          weights(v, w, 64);
-          tmem_st32(S + 32, w);
-          ready(&p_high[q]);
+            if (lane == 0) ft_arrive(&p_full[q][half]);
+          }
+          if (!ok) break;
         }
         if (ok) {
-          ok = mbar_wait(&o_full[q], (made - 1) & 1);
+          ok = mbar_wait(&o_full[q][1], (made - 1) & 1);
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
       }
@@ -524,8 +548,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         }
         __syncwarp();
       };
-      const float sum_here = l.x + l.y;
-      if (active && ok) {
+      const float2 la = kc_split(l0), lb = kc_split(l1);
+      const float sum_here = (la.x + la.y) + (lb.x + lb.y);
+      if (active && ok && !idle) {
         const float f = sum_here == 0.f ? 0.f : __fdiv_rn(1.f, sum_here);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
@@ -551,9 +576,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         if (s_ticket == (unsigned)(p.pieces - 1)) a.tickets[p.c_lo] = 0;
       }
       meet();
-      const bool last = s_ticket == (unsigned)(p.pieces - 1);
-      meet();  // read by all before the next item's
-      if (!last || !active || !ok) continue;
+      if (s_ticket != (unsigned)(p.pieces - 1) || !active || idle || !ok) continue;
       __threadfence();
       auto piece = [&](int k) -> const float* { return a.part + (size_t)(2 * (p.c_lo + k) + (k == 0 ? 1 : 0)) * kc_part_floats(HD); };
       float top = -INFINITY, sum = 0.f;

@@ -12,7 +12,6 @@ struct KvqChunkArgs {
   const int32_t* seq;
   int ldq, ldo, R, B, n_rep, max_count, step;
   int max_tiles;          // items that max_count positions make
-  int grain;              // key tiles that a CTA has at least, where there are so many
   float scale2;           // log2 e / sqrt(hd)
   float* part;            // [2 * CTAs][kc_part_floats]
   unsigned int* tickets;  // [CTAs], zero between launches
