@@ -26,7 +26,8 @@ struct jg_dev {
                     // launch is the one that has to allocate it, and read without a copy
   float* pair_slots;    // gemm_pair.cuh: accumulators of tiles that several CTA pairs share, and their flags; allocated on first use
   uint32_t* pair_flags;
-  void (*on_error)(jg_dev*);  // clears what a launch that gave up left behind (kvquant.cu), or null
+  float* kvq_part;           // kvquant.cu: pieces of results that several CTAs share, and who has arrived (zeros between launches); allocated
+  unsigned int* kvq_tickets; // with the first 8-bit cache, one of each: launches of a device follow one another
   bool tc_pending;  // such kernels were launched, or replayed from a graph, since the word was last checked
   bool tc_before_capture;  // tc_pending as it was when the capture in progress began
   bool peer_pending;  // peer-memory reductions (comm.cu) were launched since their error word was last checked
@@ -83,6 +84,7 @@ static inline int jg_after_launch(jg_dev* dev, const char* name) {
     JG_CUDA(cudaSetDevice((dev)->ordinal));                        \
   } while (0)
 
+static inline size_t jg_kvq_ticket_bytes(const jg_dev* dev) { return (size_t)2 * dev->sm_count * sizeof(unsigned int); }
 static inline bool jg_aligned(uint64_t p, uint64_t a) { return p != 0 && (p % a) == 0; }
 constexpr unsigned JG_FRESH_RING = 16;
 static inline void jg_mark_fresh(jg_dev* dev, uint64_t lo, uint64_t bytes) {

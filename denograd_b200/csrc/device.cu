@@ -91,6 +91,7 @@ JG_API int jg_device_close(jg_dev* dev) {
   cudaFreeHost(dev->pinned_stage);
   cudaFreeHost(dev->err_word);
   if (dev->pair_slots) cudaFree(dev->pair_slots);  // the flags lie behind the slots
+  if (dev->kvq_part) cudaFree(dev->kvq_part);      // the tickets likewise
   cudaStreamDestroy(dev->stream);
   delete dev;
   return JG_OK;
@@ -119,7 +120,7 @@ int jg_check_device_errors(jg_dev* dev) {
   if (code != 0) {
     *(volatile int*)dev->err_word = 0;
     jg_pair_reset(dev);
-    if (dev->on_error) dev->on_error(dev);
+    if (dev->kvq_tickets) cudaMemsetAsync(dev->kvq_tickets, 0, jg_kvq_ticket_bytes(dev), dev->stream);
     jg_set_error("a device-side wait gave up (code %d: 1 = TMA producer, 2 = MMA issuer, 3 = epilogue of a tensor-core "
                  "projection, 4 = grid barrier of the single-kernel decode step); results since the last synchronisation "
                  "are invalid", code);

@@ -8,15 +8,20 @@
 #include "kvquant_split.cuh"
 
 // ------------------------------------------------------------------------------------------------ the object
-static inline int kvq_tickets(const jg_dev* dev) { return ks_ctas(dev) > kc_ctas(dev) ? ks_ctas(dev) : kc_ctas(dev); }
-
-// Every cache, so that tickets which a launch that gave up left behind are cleared with its error.
-static std::mutex g_lock;
-static jg_kvq* g_all = nullptr;
-static void kvq_on_error(jg_dev* dev) {
-  std::lock_guard<std::mutex> lock(g_lock);
-  for (jg_kvq* kv = g_all; kv != nullptr; kv = kv->next)
-    if (kv->dev == dev) cudaMemsetAsync(kv->tickets, 0, kvq_tickets(dev) * sizeof(unsigned int), dev->stream);
+// The device's workspace for results that several CTAs share, for either kernel and any cache.
+static int kvq_workspace(jg_dev* dev) {
+  static std::mutex m;
+  std::lock_guard<std::mutex> lock(m);
+  if (dev->kvq_part != nullptr) return JG_OK;
+  const size_t few = (size_t)ks_slots(dev) * ks_part_floats(128), many = (size_t)kc_slots(dev) * kc_part_floats(128);
+  const size_t part = (few > many ? few : many) * sizeof(float), tickets = jg_kvq_ticket_bytes(dev);
+  void* p = nullptr;
+  JG_CUDA(cudaMalloc(&p, part + tickets));
+  const cudaError_t e = cudaMemsetAsync((char*)p + part, 0, tickets, dev->stream);
+  if (e != cudaSuccess) { cudaFree(p); return jg_cuda_fail(e, "kvq workspace", __FILE__, __LINE__); }
+  dev->kvq_tickets = (unsigned int*)((char*)p + part);
+  dev->kvq_part = (float*)p;
+  return JG_OK;
 }
 
 JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t format, jg_kvq** out) {
@@ -36,6 +41,8 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
              "kvq_create: block table too large, or more than 2^24 positions to a slot");
   JG_REQUIRE((unsigned long long)d.n_pages * d.n_kv_heads * d.page_size <= 0xffffffffull, "kvq_create: pool too large");
   JG_REQUIRE(!dev->capturing, "kvq_create: a graph capture is in progress");
+  const int rc = kvq_workspace(dev);
+  if (rc) return rc;
   jg_kvq* kv = new jg_kvq();
   memset(kv, 0, sizeof(*kv));
   kv->dev = dev;
@@ -48,11 +55,6 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
   if (e == cudaSuccess) e = cudaMalloc(&kv->v_codes, codes);
   if (e == cudaSuccess) e = cudaMalloc(&kv->scales, rows * sizeof(__half2));
   if (e == cudaSuccess) e = cudaMalloc(&kv->block_table, table);
-  // one workspace for both kernels: launches of a device follow one another, and each leaves the tickets at zero
-  const size_t few = (size_t)2 * ks_ctas(dev) * ks_part_floats(d.head_dim), many = (size_t)2 * kc_ctas(dev) * kc_part_floats(d.head_dim);
-  const size_t part = (few > many ? few : many) * sizeof(float), tickets = (size_t)kvq_tickets(dev) * sizeof(unsigned int);
-  if (e == cudaSuccess) e = cudaMalloc(&kv->part, part);
-  if (e == cudaSuccess) e = cudaMalloc(&kv->tickets, tickets);
   int32_t* ids = (int32_t*)malloc(table);
   if (e == cudaSuccess && ids == nullptr) e = cudaErrorMemoryAllocation;
   if (e == cudaSuccess) {
@@ -67,7 +69,6 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
     e = cudaMemsetAsync(kv->k_codes, zero, codes, dev->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(kv->v_codes, zero, codes, dev->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(kv->scales, 0, rows * sizeof(__half2), dev->stream);
-    if (e == cudaSuccess) e = cudaMemsetAsync(kv->tickets, 0, tickets, dev->stream);
     if (e == cudaSuccess) e = cudaMemcpyAsync(kv->block_table, ids, table, cudaMemcpyHostToDevice, dev->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(dev->stream);
   }
@@ -77,13 +78,7 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
     jg_kvq_destroy(kv);
     return jg_cuda_fail(e, "kvq_create", __FILE__, __LINE__);
   }
-  kv->bytes = 2 * codes + rows * sizeof(__half2) + table + part + tickets;
-  {
-    std::lock_guard<std::mutex> lock(g_lock);
-    kv->next = g_all;
-    g_all = kv;
-    dev->on_error = kvq_on_error;
-  }
+  kv->bytes = 2 * codes + rows * sizeof(__half2) + table;
   *out = kv;
   return JG_OK;
 }
@@ -93,15 +88,9 @@ static void kvq_destroy_now(void* p) { jg_kvq_destroy((jg_kvq*)p); }
 JG_API int jg_kvq_destroy(jg_kvq* kv) {
   if (!kv) return JG_OK;
   if (g_jg_capturing > 0) { jg_defer(kvq_destroy_now, kv); return JG_OK; }
-  {
-    std::lock_guard<std::mutex> lock(g_lock);
-    for (jg_kvq** at = &g_all; *at != nullptr; at = &(*at)->next)
-      if (*at == kv) { *at = kv->next; break; }
-  }
   cudaSetDevice(kv->dev->ordinal);
   cudaStreamSynchronize(kv->dev->stream);
   cudaFree(kv->k_codes); cudaFree(kv->v_codes); cudaFree(kv->scales); cudaFree(kv->block_table);
-  cudaFree(kv->part); cudaFree(kv->tickets);
   delete kv;
   return JG_OK;
 }

@@ -24,12 +24,9 @@ struct jg_kvq {
   uint8_t* v_codes;
   __half2* scales;   // [L][n_pages][G][page], (K, V)
   int32_t* block_table;
-  float* part;            // pieces of results that several CTAs share, and who has arrived (kvquant_split.cuh, kvquant_chunk.cu)
-  unsigned int* tickets;
   int max_ctx;
   size_t layer_rows;  // (position, kv head) rows of a layer
   uint64_t bytes;
-  jg_kvq* next;
 };
 
 // What the kernels see of one layer.

@@ -26,7 +26,7 @@ JG_API int jg_kvq_decode(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, i
   a.ldx = ldx; a.ldo = ldo; a.R = B; a.B = B; a.H = H; a.n_rep = H / G; a.max_count = 1; a.step = 1;
   a.limit = table && table_rows < kv->max_ctx ? table_rows : kv->max_ctx;
   a.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
-  a.part = kv->part; a.tickets = kv->tickets;
+  a.part = dev->kvq_part; a.tickets = dev->kvq_tickets;
   if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_split<KVQ_INT8, 64, 1, true>(dev, a) : launch_split<KVQ_INT8, 128, 1, true>(dev, a);
   return hd == 64 ? launch_split<KVQ_E4M3, 64, 1, true>(dev, a) : launch_split<KVQ_E4M3, 128, 1, true>(dev, a);
 }
@@ -50,7 +50,7 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
     s.ldx = ldq; s.ldo = ldo; s.R = R; s.B = B; s.H = H; s.n_rep = H / G; s.max_count = max_count; s.step = step;
     s.limit = kv->max_ctx;
     s.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
-    s.part = kv->part; s.tickets = kv->tickets;
+    s.part = dev->kvq_part; s.tickets = dev->kvq_tickets;
     const bool few = max_count * (H / G) <= 8;
     if (kv->format == JG_KVQ_INT8)
       return hd == 64 ? (few ? launch_split<KVQ_INT8, 64, 1, false>(dev, s) : launch_split<KVQ_INT8, 64, 2, false>(dev, s))
@@ -66,6 +66,6 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   a.max_tiles = (int)(((long long)max_count * (H / G) + KC_ROWS - 1) / KC_ROWS);
   JG_REQUIRE((long long)B * a.max_tiles <= (1 << 26), "kvq_attn: B=%d sequences of up to %d positions are too many for one call", B, max_count);
   a.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
-  a.part = kv->part; a.tickets = kv->tickets; a.err = dev->err_word;
+  a.part = dev->kvq_part; a.tickets = dev->kvq_tickets; a.err = dev->err_word;
   return kvq_chunk(dev, kv->format, hd, a);
 }

@@ -28,7 +28,7 @@ constexpr int KC_SOFT_REGS = 144, KC_WIDEN_REGS = 72, KC_MMA_REGS = 48;       //
 static_assert(2 * KC_SOFT_REGS + 2 * KC_WIDEN_REGS + KC_MMA_REGS <= 5 * KC_REGS, "register shares exceed what a CTA is launched with");
 constexpr int KC_PLAN = 4;  // pieces that the plan is ahead
 constexpr int KC_HALF = KC_KEYS / 2;  // keys of a step of the softmax
-constexpr int KC_WHOLE = 8, KC_GRAIN = 6;
+constexpr int KC_WHOLE = 8, KC_GRAIN = 6, KC_FIXED = 2;  // tiles: see the line of tiles
 
 template <int HD>
 struct KcCfg {
@@ -128,6 +128,9 @@ __device__ __forceinline__ void kc_widen(const uint4& x, __half2 s, __half2 bias
   }
 }
 
+// Whether an item has up to 128 rows: then its key tiles take turns between the two streams.
+__device__ __forceinline__ bool kc_split_item(const KvqChunkArgs& a, const KcPiece& p) { return p.n * a.n_rep - p.tile * KC_ROWS <= 128; }
+
 template <int FMT, int HD>
 __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunkArgs a) {
   constexpr int KB = HD / 64;                     // 64-column blocks of a tile's rows
@@ -141,6 +144,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   __shared__ KcPiece s_plan[KC_PLAN];
   __shared__ uint32_t s_tmem;
   __shared__ unsigned int s_ticket;
+  __shared__ float2 s_ml[2][128];
   __shared__ long long s_sum[KC_THREADS / 32], s_at;
   __shared__ int s_longest[KC_THREADS / 32], s_entry;
   const int tid = threadIdx.x, lane = tid & 31, warp = uniform_warp();
@@ -172,6 +176,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     KcPiece p;
     return e < entries ? kc_item(a, e / a.max_tiles, e % a.max_tiles, p) : 0;
   };
+  auto cost = [&](int n) { return n > 0 ? (long long)(n + KC_FIXED) * a.c.G : 0ll; };
   auto warp_sum64 = [&](long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -185,18 +190,26 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     }
     return v;
   };
-  // Cutting an item costs its CTAs a trip through memory each, 2 to 4 us: short items are not cut, others not into less than KC_GRAIN tiles.
+  // An item costs what KC_FIXED tiles do beside its own.  Cutting one costs its CTAs a trip through memory each, 2 to 4 us: short items are
+  // not cut, others not into less than KC_GRAIN tiles.
   long long total = 0, u_lo = 0, u_hi = 0;
   int longest = 0, ctas = 1;
   auto share = [&]() {
     const long long most = longest <= KC_WHOLE ? total : total / KC_GRAIN;
     ctas = (int)max(1ll, min((long long)gridDim.x, most));
-    if ((int)blockIdx.x < ctas) { u_lo = blockIdx.x * total / ctas; u_hi = (blockIdx.x + 1) * total / ctas; }
+    if ((int)blockIdx.x >= ctas) return;
+    if (total < (1 << 23)) {  // 512 CTAs at most: see the launch
+      u_lo = blockIdx.x * (uint32_t)total / (uint32_t)ctas;
+      u_hi = (blockIdx.x + 1) * (uint32_t)total / (uint32_t)ctas;
+    } else {
+      u_lo = blockIdx.x * total / ctas;
+      u_hi = (blockIdx.x + 1) * total / ctas;
+    }
   };
   if (entries > 32) {
     for (int e = tid; e < entries; e += KC_THREADS) {
       const int n = tiles_of(e);
-      total += (long long)n * a.c.G;
+      total += cost(n);
       longest = max(longest, n);
     }
     total = warp_sum64(total);
@@ -208,7 +221,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     share();
     long long before = 0;
     for (int base = 0; base < entries && u_lo < u_hi; base += KC_THREADS) {  // the same for all threads
-      const long long mine = (long long)tiles_of(base + tid) * a.c.G, sum = scan64(mine);
+      const long long mine = cost(tiles_of(base + tid)), sum = scan64(mine);
       __syncthreads();
       if (lane == 31) s_sum[warp] = sum;
       __syncthreads();
@@ -243,7 +256,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         entry = s_entry;
       } else {
         longest = tiles_of(lane);
-        const long long mine = (long long)longest * a.c.G, sum = scan64(mine);
+        const long long mine = cost(longest), sum = scan64(mine);
         total = __shfl_sync(0xffffffffu, sum, 31);
         longest = __reduce_max_sync(0xffffffffu, longest);
         share();
@@ -262,22 +275,32 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         while (u < u_hi) {
           const int n = kc_item(a, b, tile, p);
           if (n == 0) { tile = 0; b++; continue; }  // the items of a sequence are its first ones
-          if (u >= at + (long long)n * a.c.G) {
-            at += (long long)n * a.c.G;
+          const int span = n + KC_FIXED;  // of an item on the line; its tiles are behind its fixed cost
+          if (u >= at + (long long)span * a.c.G) {
+            at += (long long)span * a.c.G;
             if (++tile == a.max_tiles) { tile = 0; b++; }
             continue;
           }
-          p.g = (int)(u - at) / n;  // both below 2^31: see the limits of the cache
-          const long long item = at + (long long)p.g * n;
-          p.j0 = (int)(u - item);
-          p.j1 = cut ? (int)min((long long)n, u_hi - item) : n;
-          u = item + p.j1;
-          if (!cut && p.j0 > 0) continue;  // begun by the CTA before
+          p.g = (int)(u - at) / span;  // both below 2^31: see the limits of the cache
+          const long long item = at + (long long)p.g * span;
+          if (!cut) {  // the CTA in whose stretch it begins has all of it
+            const bool mine = u == item;
+            u = item + span;
+            if (!mine) continue;
+            p.j0 = 0;
+            p.j1 = n;
+          } else {
+            p.j0 = max(0, (int)(u - item) - KC_FIXED);
+            u = min(item + span, u_hi);
+            p.j1 = max(0, (int)(u - item) - KC_FIXED);
+            if (p.j0 == p.j1) continue;
+          }
           p.b = b; p.tile = tile; p.n_tiles = n;
           p.c_lo = p.pieces = 0;
           if (p.j1 - p.j0 < n) {
-            p.c_lo = (int)(((item + 1) * ctas - 1) / total);
-            p.pieces = (int)(((item + n) * ctas - 1) / total) - p.c_lo + 1;
+            const long long begin = item + KC_FIXED;
+            p.c_lo = (int)(((begin + 1) * ctas - 1) / total);
+            p.pieces = (int)(((begin + n) * ctas - 1) / total) - p.c_lo + 1;
           }
           break;
         }
@@ -297,8 +320,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         ok = ok && mbar_wait(bar, parity);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       };
-      auto qk = [&](int q, uint32_t slot) {
-        const uint64_t da = umma_desc(sQ + (size_t)q * Cfg::Q_BYTES), db = umma_desc(sK + (size_t)slot * Cfg::KV_BYTES);
+      auto qk = [&](int q, uint32_t slot, int rows) {  // scores of a stream: of which 128 rows, over which tile of keys
+        const uint64_t da = umma_desc(sQ + (size_t)rows * Cfg::Q_BYTES), db = umma_desc(sK + (size_t)slot * Cfg::KV_BYTES);
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < KB; c++)
@@ -308,33 +331,55 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           umma_commit(&s_full[q]);
         }
       };
+      auto pv = [&](int q, uint32_t slot, bool first) {  // its weights times a tile of values, half a tile at a time
+        const uint64_t db = umma_desc_mn(sV + (size_t)slot * Cfg::KV_BYTES, BLOCK);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          wait(&p_full[q][half], made[q] & 1);
+          if (ok && elect_one()) {
+#pragma unroll
+            for (int k = half * (KC_HALF / 16); k < (half + 1) * (KC_HALF / 16); k++)  // 16 rows of values = 2048 bytes further
+              umma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, db + k * 128, id_o, (!first || k > 0) ? 1u : 0u);
+            umma_commit(&o_full[q][half]);
+          }
+        }
+        made[q]++;
+      };
       KcPiece p;
       while (next(p)) {
-        const int n = p.j1 - p.j0, streams = p.n * a.n_rep - p.tile * KC_ROWS > 128 ? 2 : 1;
-        for (int q = 0; q < streams; q++) wait(&q_full[q], loaded[q]++ & 1);
+        const int n = p.j1 - p.j0;
+        if (kc_split_item(a, p)) {
+          wait(&q_full[0], loaded[0]++ & 1);
+          auto scores = [&](int j) {  // of tile j, for the stream whose turn it is
+            const uint32_t slot = (tiles + j) & 1;
+            wait(&k_full[slot], ((tiles + j) >> 1) & 1);
+            if (ok) qk(j & 1, slot, 0);
+            if (ok) commit(&k_empty[slot]);
+          };
+          for (int j = 0; j < 2 && j < n; j++) scores(j);
+          for (int j = 0; j < n && ok; j++) {
+            const uint32_t slot = (tiles + j) & 1;
+            wait(&v_full[slot], ((tiles + j) >> 1) & 1);
+            if (ok) pv(j & 1, slot, j < 2);
+            if (ok) commit(&v_empty[slot]);
+            if (j + 2 < n) scores(j + 2);
+          }
+          tiles += n;
+          continue;
+        }
+        for (int q = 0; q < 2; q++) wait(&q_full[q], loaded[q]++ & 1);
         wait(&k_full[tiles & 1], (tiles >> 1) & 1);
         if (!ok) break;
-        for (int q = 0; q < streams; q++) qk(q, tiles & 1);
+        for (int q = 0; q < 2; q++) qk(q, tiles & 1, q);
         commit(&k_empty[tiles & 1]);
         for (int j = 0; j < n && ok; j++, tiles++) {
           const uint32_t slot = tiles & 1, then = slot ^ 1;
           const bool more = j + 1 < n;
           wait(&v_full[slot], (tiles >> 1) & 1);
-          for (int q = 0; q < streams && ok; q++) {
-            const uint64_t db = umma_desc_mn(sV + (size_t)slot * Cfg::KV_BYTES, BLOCK);
-#pragma unroll
-            for (int half = 0; half < 2; half++) {  // a half of the tile's weights at a time
-              wait(&p_full[q][half], made[q] & 1);
-              if (ok && elect_one()) {
-#pragma unroll
-                for (int k = half * (KC_HALF / 16); k < (half + 1) * (KC_HALF / 16); k++)  // 16 rows of values = 2048 bytes further
-                  umma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, db + k * 128, id_o, (j > 0 || k > 0) ? 1u : 0u);
-                umma_commit(&o_full[q][half]);
-              }
-            }
+          for (int q = 0; q < 2 && ok; q++) {
+            pv(q, slot, j == 0);
             if (more && q == 0) wait(&k_full[then], ((tiles + 1) >> 1) & 1);
-            if (more && ok) qk(q, then);
-            made[q]++;
+            if (more && ok) qk(q, then, q);
           }
           if (!ok) break;
           commit(&v_empty[slot]);
@@ -379,11 +424,23 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
 #pragma unroll
         for (int i = 0; i < N; i++) x[i] = ld_stream_128(codes + (size_t)row_at(row + i * ROWS) * HD);
       };
-      int page = page_of(p.j0);
+      // the rows of a tile on their way into L2, one to a thread, where a tile of few rows is done before another comes from HBM
+      const bool hurry = kc_split_item(a, p);
+      auto ahead = [&](int j, int page) {
+        const uint32_t begin = first_row(j, page);
+        const int r = u;
+        const size_t at = __shfl_sync(0xffffffffu, begin, r >> 4) + (uint32_t)(j * KC_KEYS + r <= last ? r & 15 : 0);
+        prefetch_l2(codes - sub * 16 + at * HD);
+        if ((r & 15) == 0) prefetch_l2(scales + 2 * at);
+      };
+      int page = page_of(p.j0), page2 = page_of(p.j0 + 1);
       load(p.j0, page);
-      if (p.j0 + 1 < p.j1) page = page_of(p.j0 + 1);
+      page = page2;
+      page2 = page_of(p.j0 + 2);
+      if (hurry && p.j0 + 1 < p.j1) ahead(p.j0 + 1, page);
       for (int j = p.j0; j < p.j1; j++, tiles++) {
         const uint32_t slot = tiles & 1;
+        if (hurry && j + 2 < p.j1) ahead(j + 2, page2);
         if (tiles >= 2) ok = mbar_wait(&empty[slot], ((tiles >> 1) - 1) & 1);
         if (!ok) break;
         unsigned char* to = tile + (size_t)slot * Cfg::KV_BYTES;
@@ -400,7 +457,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         __syncwarp();
         if (lane == 0) ft_arrive(&full[slot]);
         if (j + 1 < p.j1) load(j + 1, page);
-        if (j + 2 < p.j1) page = page_of(j + 2);
+        page = page2;
+        page2 = page_of(j + 3);
       }
     }
     if (!ok && lane == 0) atomicCAS(a.err, 0, 1);
@@ -411,117 +469,165 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), S = lanes + q * 128, O = lanes + 256 + q * 128;
     unsigned char* rows_at = sQ + (size_t)q * Cfg::Q_BYTES + (warp & 3) * 32 * 128;  // this warp's 32 rows of queries, and of results behind them
     const uint64_t scale2 = kc_pair(a.scale2, a.scale2);
-    uint32_t made = 0, meetings = 0;  // score tiles so far, and times that the two streams have met
+    uint32_t made = 0, meetings = 0, turn = 0;  // score tiles so far, times that the two streams have met, split items
     auto meet = [&]() {  // of all softmax warps, with a limit: bar.sync would wait for a warp that gave up
       __syncwarp();
       if (lane == 0) ft_arrive(&met);
       ok = mbar_wait(&met, meetings++ & 1) && ok;
     };
-    KcPiece p;
-    while (next(p)) {
-      const int n = p.j1 - p.j0, rows = p.n * a.n_rep - p.tile * KC_ROWS, mine = q * 128 + r;  // rows of the item, and this thread's
-      const bool active = rows > q * 128, idle = rows <= mine - lane;  // the stream has rows at all; this warp has none
-      const int i = (p.tile * KC_ROWS + mine) / a.n_rep, h = p.tile * KC_ROWS + mine - i * a.n_rep;
-      const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step, pos = (long long)p.p0 + i;
-      const bool there = mine < rows && row >= 0 && row < a.R;
-      const bool outside = p.bt == nullptr || pos < 0 || pos >= a.c.max_ctx;
-      const int lim = !there ? p.T - 1 : (int)max(-1ll, min(pos, (long long)p.T - 1));  // last key that the row sees
-      const int head = p.g * a.n_rep + h;
+    // What this thread's row is, worked out from the plan where it is needed: the loop over tiles has no registers to keep it in.
+    auto mine_of = [&](const KcPiece& p) { return kc_split_item(a, p) ? r : q * 128 + r; };  // of the item's rows
+    auto row_of = [&](const KcPiece& p, int& head, int& i) -> long long {  // row of queries and results, or -1
+      const int at = p.tile * KC_ROWS + mine_of(p);
+      i = at / a.n_rep;
+      head = p.g * a.n_rep + at - i * a.n_rep;
+      const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step;
+      return at < p.n * a.n_rep && row >= 0 && row < a.R ? row : -1;
+    };
+    for (;; planned++) {
+      const uint32_t planned_slot = planned % KC_PLAN;
+      ok = ok && mbar_wait(&plan_full[planned_slot], (planned / KC_PLAN) & 1);
+      if (!ok) break;
+      const KcPiece& p = s_plan[planned_slot];
+      if (p.b < 0) break;
+      auto release = [&]() {
+        __syncwarp();
+        if (lane == 0) ft_arrive(&plan_empty[planned_slot]);
+      };
+      const bool split = kc_split_item(a, p), idle = p.n * a.n_rep - p.tile * KC_ROWS <= mine_of(p) - lane;  // this warp has no rows
+      const int n = split ? (p.j1 - p.j0 + 1 - q) / 2 : p.j1 - p.j0;  // tiles of this stream
+      int lim;  // last key that the row sees
       float m = -INFINITY;
       uint64_t l0 = kc_pair(0.f, 0.f), l1 = l0;  // the sum, in four parts
-      if (active) {
-        // the warp's 32 rows, HD / 8 lanes to a row
-        const long long from = there ? row * a.ldq + head * HD : -1;
-        constexpr int W = HD / 8, PER = 32 / W;
+      {
+        int head, i;
+        const long long row = row_of(p, head, i);
+        lim = row < 0 ? p.T - 1 : (int)max(-1ll, min((long long)p.p0 + i, (long long)p.T - 1));
+        if (!split || q == 0) {
+          const long long from = row < 0 ? -1 : row * a.ldq + head * HD;
+          // the warp's 32 rows, HD / 8 lanes to a row
+          constexpr int W = HD / 8, PER = 32 / W;
 #pragma unroll 4
-        for (int k = 0; k < 32; k += PER) {
-          const int rr = k + lane / W, c = lane % W;
-          const long long at = __shfl_sync(0xffffffffu, from, rr);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                       ::"r"(smem_u32(rows_at + (c >> 3) * BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4))), "l"(a.q + max(at, 0ll) + c * 8), "r"(at < 0 ? 0 : 16)
-                       : "memory");  // zeros for rows that there are not
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) ft_arrive(&q_full[q]);
-        for (int j = 0; j < n; j++, made++) {
-          ok = mbar_wait(&s_full[q], made & 1);
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          if (idle) {  // whatever lies in the place of its weights concerns rows that nobody stores
-            if (lane == 0) { ft_arrive(&p_full[q][0]); ft_arrive(&p_full[q][1]); }
-            continue;
+          for (int k = 0; k < 32; k += PER) {
+            const int rr = k + lane / W, c = lane % W;
+            const long long at = __shfl_sync(0xffffffffu, from, rr);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                         ::"r"(smem_u32(rows_at + (c >> 3) * BLOCK + rr * 128 + (((c & 7) ^ (rr & 7)) << 4))), "l"(a.q + max(at, 0ll) + c * 8), "r"(at < 0 ? 0 : 16)
+                         : "memory");  // zeros for rows that there are not
           }
-          // Two halves of 64 keys, each a step of its own of the running maximum: the first one's product with V runs while the second is here.
-          const int key = (p.j0 + j) * KC_KEYS;
-          const bool all = __all_sync(0xffffffffu, key + KC_KEYS - 1 <= lim);
-          float v[64];
-          tmem_ld32(S, v);
-          tmem_ld32(S + 32, v + 32);
-#pragma unroll
-          for (int half = 0; half < 2; half++) {
-            kc_landed<64>(v);
-            if (!all) {
-#pragma unroll
-              for (int c = 0; c < 64; c++) v[c] = key + half * 64 + c <= lim ? v[c] : -INFINITY;
-            }
-            const float top = kc_max64(v) * a.scale2;
-            if (__any_sync(0xffffffffu, top > m + 8.f)) {
-              const float then = fmaxf(m, top), fade = then == m ? 1.f : ft_ex2(m - then);
-              m = then;
-              const uint64_t f2 = kc_pair(fade, fade);
-              l0 = kc_fma2(l0, f2, kc_pair(0.f, 0.f));
-              l1 = kc_fma2(l1, f2, kc_pair(0.f, 0.f));
-              if (j > 0 || half > 0) {  // the product before has to be in O
-                ok = half == 0 ? mbar_wait(&o_full[q][1], (made - 1) & 1) : mbar_wait(&o_full[q][0], made & 1);
-                if (!ok) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
-                  float y[32];
-                  uint32_t w[32];
-                  tmem_ld32(O + c, y);
-                  kc_landed<32>(y);
-#pragma unroll
-                  for (int k = 0; k < 32; k++) w[k] = __float_as_uint(y[k] * fade);
-                  tmem_st32(O + c, w);
-                }
-              }
-            }
-            const float base = m == -INFINITY ? 0.f : -m;
-            const uint64_t base2 = kc_pair(base, base);
-            uint32_t w[32];
-#pragma unroll
-            for (int k = 0; k < 64; k += 4) {
-              const float2 x = kc_split(kc_fma2(kc_pair(v[k], v[k + 1]), scale2, base2)), y = kc_split(kc_fma2(kc_pair(v[k + 2], v[k + 3]), scale2, base2));
-              const float x0 = ft_ex2(x.x), x1 = ft_ex2(x.y), y0 = ft_ex2(y.x), y1 = ft_ex2(y.y);
-              l0 = kc_add2(l0, kc_pair(x0, x1));
-              l1 = kc_add2(l1, kc_pair(y0, y1));
-              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2]) : "f"(x1), "f"(x0));
-              asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2 + 1]) : "f"(y1), "f"(y0));
-            }
-            tmem_st32(S + half * 32, w);
-            if (half == 0) {
-              tmem_ld32(S + 64, v);
-              tmem_ld32(S + 96, v + 32);
-            }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) ft_arrive(&p_full[q][half]);
-          }
-          if (!ok) break;
-        }
-        if (ok) {
-          ok = mbar_wait(&o_full[q][1], (made - 1) & 1);
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) ft_arrive(&q_full[q]);
         }
       }
+      int key = (p.j0 + (split ? q : 0)) * KC_KEYS;
+      for (int j = 0; j < n; j++, made++, key += split ? 2 * KC_KEYS : KC_KEYS) {
+        ok = mbar_wait(&s_full[q], made & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (idle) {  // whatever lies in the place of its weights concerns rows that nobody stores
+          if (lane == 0) { ft_arrive(&p_full[q][0]); ft_arrive(&p_full[q][1]); }
+          continue;
+        }
+        // Two halves of 64 keys, each a step of its own of the running maximum: the first one's product with V runs while the second is here.
+        const bool all = __all_sync(0xffffffffu, key + KC_KEYS - 1 <= lim);
+        float v[64];
+        tmem_ld32(S, v);
+        tmem_ld32(S + 32, v + 32);
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+          kc_landed<64>(v);
+          if (!all) {
+#pragma unroll
+            for (int c = 0; c < 64; c++) v[c] = key + half * 64 + c <= lim ? v[c] : -INFINITY;
+          }
+          const float top = kc_max64(v) * a.scale2;
+          if (__any_sync(0xffffffffu, top > m + 8.f)) {
+            const float then = fmaxf(m, top), fade = then == m ? 1.f : ft_ex2(m - then);
+            m = then;
+            const uint64_t f2 = kc_pair(fade, fade);
+            l0 = kc_fma2(l0, f2, kc_pair(0.f, 0.f));
+            l1 = kc_fma2(l1, f2, kc_pair(0.f, 0.f));
+            if (j > 0 || half > 0) {  // the product before has to be in O
+              ok = half == 0 ? mbar_wait(&o_full[q][1], (made - 1) & 1) : mbar_wait(&o_full[q][0], made & 1);
+              if (!ok) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 32) {
+                float y[32];
+                uint32_t w[32];
+                tmem_ld32(O + c, y);
+                kc_landed<32>(y);
+#pragma unroll
+                for (int k = 0; k < 32; k++) w[k] = __float_as_uint(y[k] * fade);
+                tmem_st32(O + c, w);
+              }
+            }
+          }
+          const float base = m == -INFINITY ? 0.f : -m;
+          const uint64_t base2 = kc_pair(base, base);
+          uint32_t w[32];
+#pragma unroll
+          for (int k = 0; k < 64; k += 4) {
+            const float2 x = kc_split(kc_fma2(kc_pair(v[k], v[k + 1]), scale2, base2)), y = kc_split(kc_fma2(kc_pair(v[k + 2], v[k + 3]), scale2, base2));
+            const float x0 = ft_ex2(x.x), x1 = ft_ex2(x.y), y0 = ft_ex2(y.x), y1 = ft_ex2(y.y);
+            l0 = kc_add2(l0, kc_pair(x0, x1));
+            l1 = kc_add2(l1, kc_pair(y0, y1));
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2]) : "f"(x1), "f"(x0));
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2 + 1]) : "f"(y1), "f"(y0));
+          }
+          tmem_st32(S + half * 32, w);
+          if (half == 0) {
+            tmem_ld32(S + 64, v);
+            tmem_ld32(S + 96, v + 32);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) ft_arrive(&p_full[q][half]);
+        }
+        if (!ok) break;
+      }
+      if (ok && n > 0) {
+        ok = mbar_wait(&o_full[q][1], (made - 1) & 1);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      const float2 la = kc_split(l0), lb = kc_split(l1);
+      float sum = (la.x + la.y) + (lb.x + lb.y), own = 1.f, others = 0.f;  // the shares of the two streams' outputs
+      // ---- the streams of a split item: a row's two outputs lie in the same lane of tensor memory
+      if (split && p.n_tiles > 1) {
+        float2* ml = s_ml[turn++ & 1] + r;  // two in turn: a stream without tiles would be ahead of the other
+        if (q == 1) *ml = make_float2(m, sum);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        meet();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (q == 0) {
+          const float2 o = *ml;
+          const float then = fmaxf(m, o.x), base = then == -INFINITY ? 0.f : then;
+          own = ft_ex2(m - base);
+          others = ft_ex2(o.x - base);
+          sum = sum * own + o.y * others;
+          m = then;
+        }
+      }
+      const bool both = split && p.j1 - p.j0 > 1, absent = split && q == 1;  // the other stream has outputs; this one's are the other's to store
+      auto outputs = [&](int c, float* o) {  // 32 columns of the row
+        tmem_ld32(O + c, o);
+        kc_landed<32>(o);
+        if (!both) return;
+        float x[32];
+        tmem_ld32(O + 128 + c, x);
+        kc_landed<32>(x);
+#pragma unroll
+        for (int k = 0; k < 32; k++) o[k] = o[k] * own + x[k] * others;
+      };
       // ---- the result, or a piece of it
-      const bool whole = n == p.n_tiles;
+      const bool whole = p.j1 - p.j0 == p.n_tiles;
       float* part = a.part + (size_t)(2 * blockIdx.x + (p.j0 == 0 ? 1 : 0)) * kc_part_floats(HD);  // [hd / 4][256][4], maxima, sums
-      const long long to = there ? row * a.ldo + head * HD : -1;
+      int head, i;
+      const long long row = row_of(p, head, i), to = row < 0 ? -1 : row * a.ldo + head * HD;
+      const bool outside = p.bt == nullptr || (long long)p.p0 + i < 0 || (long long)p.p0 + i >= a.c.max_ctx;
       // 32 columns from c on of the warp's rows, as halves in the place of its queries (whose products are done)
       auto gather = [&](int c, const float* o, float f) {
 #pragma unroll
@@ -548,26 +654,28 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         }
         __syncwarp();
       };
-      const float2 la = kc_split(l0), lb = kc_split(l1);
-      const float sum_here = (la.x + la.y) + (lb.x + lb.y);
-      if (active && ok && !idle) {
-        const float f = sum_here == 0.f ? 0.f : __fdiv_rn(1.f, sum_here);
+      const int at = q * 128 + r;
+      if (ok && !idle && !absent) {
+        const float f = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           float o[32];
-          tmem_ld32(O + c, o);
-          kc_landed<32>(o);
+          outputs(c, o);
           if (whole) {
             gather(c, o, f);
           } else {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) __stcg(reinterpret_cast<float4*>(part) + (size_t)((c + k) / 4) * KC_ROWS + mine, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+            for (int k = 0; k < 32; k += 4) __stcg(reinterpret_cast<float4*>(part) + (size_t)((c + k) / 4) * KC_ROWS + at, make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
           }
         }
-        if (whole) store();
-        else { __stcg(part + HD * KC_ROWS + mine, m); __stcg(part + HD * KC_ROWS + KC_ROWS + mine, sum_here); }
+        if (whole) {
+          store();
+        } else {
+          __stcg(part + HD * KC_ROWS + at, m);
+          __stcg(part + HD * KC_ROWS + KC_ROWS + at, sum);
+        }
       }
-      if (whole) continue;
+      if (whole) { release(); continue; }
       // ---- an item that CTAs c_lo .. share: the last to arrive adds its pieces up in this order
       __threadfence();
       meet();
@@ -576,35 +684,39 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         if (s_ticket == (unsigned)(p.pieces - 1)) a.tickets[p.c_lo] = 0;
       }
       meet();
-      if (s_ticket != (unsigned)(p.pieces - 1) || !active || idle || !ok) continue;
+      if (s_ticket != (unsigned)(p.pieces - 1) || idle || absent || !ok) { release(); continue; }
       __threadfence();
       auto piece = [&](int k) -> const float* { return a.part + (size_t)(2 * (p.c_lo + k) + (k == 0 ? 1 : 0)) * kc_part_floats(HD); };
-      float top = -INFINITY, sum = 0.f;
+      float top = -INFINITY;
 #pragma unroll 4
-      for (int k = 0; k < p.pieces; k++) top = fmaxf(top, __ldcg(piece(k) + HD * KC_ROWS + mine));
+      for (int k = 0; k < p.pieces; k++) top = fmaxf(top, __ldcg(piece(k) + HD * KC_ROWS + at));
       const float base = top == -INFINITY ? 0.f : top;
+      sum = 0.f;
 #pragma unroll 4
-      for (int k = 0; k < p.pieces; k++)
-        sum = fmaf(__ldcg(piece(k) + HD * KC_ROWS + KC_ROWS + mine), ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + mine) - base), sum);
+      for (int k = 0; k < p.pieces; k++) sum = fmaf(__ldcg(piece(k) + HD * KC_ROWS + KC_ROWS + at), ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base), sum);
       const float f = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
 #pragma unroll
         for (int k = 0; k < 32; k++) o[k] = 0.f;
-#pragma unroll 2
+#pragma unroll 1
         for (int k = 0; k < p.pieces; k++) {
-          const float w = ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + mine) - base);
+          const float4* from = reinterpret_cast<const float4*>(piece(k)) + (size_t)(c / 4) * KC_ROWS + at;
+          float4 y[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) y[e] = __ldcg(from + (size_t)e * KC_ROWS);
+          const float w = ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base);
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(piece(k)) + (size_t)(c / 4 + e) * KC_ROWS + mine);
-            o[4 * e] = fmaf(y.x, w, o[4 * e]); o[4 * e + 1] = fmaf(y.y, w, o[4 * e + 1]);
-            o[4 * e + 2] = fmaf(y.z, w, o[4 * e + 2]); o[4 * e + 3] = fmaf(y.w, w, o[4 * e + 3]);
+            o[4 * e] = fmaf(y[e].x, w, o[4 * e]); o[4 * e + 1] = fmaf(y[e].y, w, o[4 * e + 1]);
+            o[4 * e + 2] = fmaf(y[e].z, w, o[4 * e + 2]); o[4 * e + 3] = fmaf(y[e].w, w, o[4 * e + 3]);
           }
         }
         gather(c, o, f);
       }
       store();
+      release();
     }
     if (!ok && lane == 0) atomicCAS(a.err, 0, 3);
   }

@@ -13,13 +13,14 @@ struct KvqChunkArgs {
   int ldq, ldo, R, B, n_rep, max_count, step;
   int max_tiles;          // items that max_count positions make
   float scale2;           // log2 e / sqrt(hd)
-  float* part;            // [2 * CTAs][kc_part_floats]
+  float* part;            // [kc_slots][kc_part_floats]
   unsigned int* tickets;  // [CTAs], zero between launches
   int* err;
 };
 
 constexpr int KC_ROWS = 256, KC_KEYS = 128;  // query rows of an item, keys of a tile
-static inline int kc_ctas(const jg_dev* dev) { return dev->sm_count; }
+static inline int kc_ctas(const jg_dev* dev) { return dev->sm_count < 512 ? dev->sm_count : 512; }
+static inline int kc_slots(const jg_dev* dev) { return 2 * kc_ctas(dev); }  // pieces in the workspace
 __host__ __device__ constexpr size_t kc_part_floats(int hd) { return (size_t)KC_ROWS * (hd + 2); }  // outputs, maxima, sums
 
 int kvq_chunk(jg_dev* dev, int format, int hd, const KvqChunkArgs& a);

@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
   }
 }
 
-// CTAs that a device runs at once, which is also how many pieces and tickets the workspace has.
-static inline int ks_ctas(const jg_dev* dev) { return 2 * dev->sm_count; }
+static inline int ks_ctas(const jg_dev* dev) { return 2 * dev->sm_count; }  // that a device runs at once; as many tickets: jg_kvq_ticket_bytes
+static inline int ks_slots(const jg_dev* dev) { return 2 * ks_ctas(dev); }  // pieces in the workspace
 static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 2>::PART : KsCfg<128, 2>::PART; }
 
 template <int FMT, int HD, int NT, bool NEW>
