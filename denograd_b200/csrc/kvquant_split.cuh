@@ -4,15 +4,14 @@
 //   scores^T [16 positions x columns] = K [16 x hd] . q^T        weights in 16 bits, turned by movmatrix
 //   out^T [hd x columns] += V^T [hd x 16 positions] . w^T        mma.sync.m16n8k16, 32-bit sums
 // The inner index of a product and the order of its rows are free as long as both operands agree, so a lane's fragments are 16
-// neighbouring codes of a row: of K as they lie, of V two rows at a time with their bytes interleaved.  A lane copies the bytes that it
-// will itself read (cp.async into a ring of its own in shared memory), so nothing is shared between lanes and nobody waits for a
-// barrier in the loop.  V is multiplied by its scale as it is widened (exact), K's scale goes to the finished scores.
+// neighbouring codes of a row: of K as they lie, of V two rows at a time with their bytes interleaved.  So a lane loads just what it
+// multiplies, 16 bytes at a time and a tile ahead, straight into registers.  V is multiplied by its scale as it is widened (exact), K's scale goes to the finished scores.
 //
 // The running maximum is a reference that scores may pass by 2^6 before sums and outputs are rescaled: a vote a tile instead of three
 // rounds of shuffles.
 //
-// The positions of all (sequence, kv head)s are one line of units of 16 * KS_WARPS, cut evenly over the CTAs: long and short
-// conversations of a batch cost what they hold.  A CTA's stretch holds pieces of several (sequence, kv head)s; those that others
+// The positions of all (sequence, kv head)s are one line of units of 16 * KS_WARPS, with some more for what each costs by itself, cut
+// evenly over the CTAs: long and short conversations of a batch cost what they hold.  A CTA's stretch holds pieces of several (sequence, kv head)s; those that others
 // share are left in a workspace (at most two a CTA: its first and its last), and the last to arrive puts them together in order.
 #pragma once
 #include "kvquant.cuh"
@@ -32,16 +31,14 @@ struct KvqSplitArgs {
   unsigned int* tickets;                                 // [CTAs], zero between launches
 };
 
-constexpr int KS_WARPS = 8, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_STAGES = 2;
+constexpr int KS_WARPS = 4, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_CTAS = 3;  // CTAs to an SM
+constexpr int KS_FIXED = 3;  // units that a (sequence, kv head) costs beside its own
 
 template <int HD, int NT>
 struct KsCfg {
   static constexpr int COLS = 8 * NT, KJ = HD / 64;             // 16-byte pieces of a K row that a lane holds
   static constexpr int VB = HD / 8;                             // bytes of a V row that a lane holds
-  static constexpr int K_BYTES = 2 * KJ * 512, V_BYTES = 4 * VB * 32, S_BYTES = 24 * 32, STAGE = K_BYTES + V_BYTES + S_BYTES;
-  static constexpr int RING = KS_WARPS * KS_STAGES * STAGE;
-  static constexpr int MERGE = KS_WARPS * COLS * HD * 4;        // the warps' outputs, over the ring
-  static constexpr size_t SMEM = RING > MERGE ? RING : MERGE;
+  static constexpr size_t MERGE = KS_WARPS * COLS * HD * 4;     // the warps' outputs when they meet
   static constexpr int PART = COLS * (HD + 2);                  // floats of a piece: outputs, maxima, sums
 };
 
@@ -61,15 +58,10 @@ __device__ __forceinline__ uint32_t ks_transpose(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-template <int BYTES>
-__device__ __forceinline__ void ks_copy(uint32_t dst, const void* src) {
-  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
-}
 __device__ __forceinline__ uint32_t ks_half2(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
 template <int FMT, int HD, int NT, bool NEW>
-__global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(const KvqSplitArgs a) {
+__global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_kernel(const KvqSplitArgs a) {
   using Cfg = KsCfg<HD, NT>;
   constexpr int COLS = Cfg::COLS, KJ = Cfg::KJ, VB = Cfg::VB, MT = HD / 16;
   extern __shared__ __align__(16) unsigned char ks_raw[];
@@ -100,17 +92,24 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
   };
   // this CTA's stretch of the line of units, and the sequence that it begins in; every warp works it out for itself
   long long total = 0;
-  for (int b = lane; b < a.B; b += 32) total += units(b);
+  for (int b = lane; b < a.B; b += 32) total += units(b) + KS_FIXED;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= a.c.G;
   const long long ctas = min((long long)gridDim.x, total);
   if (blockIdx.x >= ctas) return;
-  const long long u_lo = blockIdx.x * total / ctas, u_hi = (blockIdx.x + 1) * total / ctas;
+  long long u_lo, u_hi;
+  if (total < (1 << 20)) {  // up to 4096 CTAs
+    u_lo = blockIdx.x * (uint32_t)total / (uint32_t)ctas;
+    u_hi = (blockIdx.x + 1) * (uint32_t)total / (uint32_t)ctas;
+  } else {
+    u_lo = blockIdx.x * total / ctas;
+    u_hi = (blockIdx.x + 1) * total / ctas;
+  }
   int b = 0;
   long long at = 0;  // first unit of (b, head 0)
   for (int base = 0;; base += 32) {
-    const int n = base + lane < a.B ? units(base + lane) : 0;
+    const int n = base + lane < a.B ? units(base + lane) + KS_FIXED : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -127,77 +126,94 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
     at += (long long)__shfl_sync(0xffffffffu, sum, 31) * a.c.G;
   }
 
-  unsigned char* ring = ks_raw + warp * (KS_STAGES * Cfg::STAGE);
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   for (long long u = u_lo; u < u_hi; b++) {
     int p0, n_new;
     const int32_t* bt;
     const int T = sequence(b, p0, n_new, bt);
-    const int n_units = max(1, (T + KS_UNIT - 1) / KS_UNIT);
+    const int n_units = max(1, (T + KS_UNIT - 1) / KS_UNIT), span = n_units + KS_FIXED;  // its units lie behind its fixed cost
     const bool stored = NEW && bt != nullptr;  // there is a new token, at p0
     const long long row0 = NEW ? b : (a.first ? a.first[b] : b);
     const int n_cols = n_new * a.n_rep;
-    for (int g = (int)((u - at) / n_units); g < a.c.G && u < u_hi; g++) {
-      const long long item = at + (long long)g * n_units;
-      const int j0 = (int)(u - item), j1 = (int)min((long long)n_units, u_hi - item);
-      u = item + j1;
+    for (int g = (int)((u - at) / span); g < a.c.G && u < u_hi; g++) {
+      const long long item = at + (long long)g * span;
+      const int j0 = max(0, (int)(u - item) - KS_FIXED);
+      u = min(item + span, u_hi);
+      const int j1 = max(0, (int)(u - item) - KS_FIXED);
+      if (j0 == j1) continue;
       const int t_lo = j0 * KS_UNIT, t_hi = min(T, j1 * KS_UNIT);
       const int n_tiles = t_hi > t_lo + warp * 16 ? (t_hi - t_lo - warp * 16 + KS_UNIT - 1) / KS_UNIT : 0;  // of this warp
 
-      // ---- copies of a tile: the lane's own pieces of 16 positions
-      int pages = 0;  // lane l: page of the warp's tile 32 i + l
-      auto request = [&](int i) {
+      // ---- a tile: the lane's own pieces of 16 positions
+      struct Tile {
+        uint4 k[2][KJ];              // of rows r and r + 8
+        uint32_t v[4][VB / 4];       // of rows 2c, 2c + 1, 2c + 8, 2c + 9
+        __half2 s0, s1;              // scales of rows r and r + 8
+        uint2 sv0, sv1;              // and of 2c, 2c + 1; 2c + 8, 2c + 9
+      };
+      auto pages_of = [&](int i) { return i + lane < n_tiles ? bt[(t_lo + (i + lane) * KS_UNIT + warp * 16) >> a.c.page_shift] : 0; };
+      int pages = pages_of(0);  // lane l: page of the warp's tile 32 i + l
+      auto load = [&](int i, Tile& t) {
         const int t0 = t_lo + i * KS_UNIT + warp * 16;
-        if ((i & 31) == 0) pages = i + lane < n_tiles ? bt[(t0 + lane * KS_UNIT) >> a.c.page_shift] : 0;
+        if (i > 0 && (i & 31) == 0) pages = pages_of(i);
         const int page = __shfl_sync(0xffffffffu, pages, i & 31);
         const size_t row = (((size_t)page * a.c.G + g) << a.c.page_shift) + (t0 & ((1 << a.c.page_shift) - 1));
-        uint32_t to = ring_at + (i % KS_STAGES) * Cfg::STAGE + lane * 16;
         const uint8_t* k = a.c.k + (row + r) * HD + c * 16;
+        const uint8_t* v = a.c.v + (row + 2 * c) * HD + r * VB;
+        const __half2* s = a.c.scales + row;
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-          for (int j = 0; j < KJ; j++, to += 512) ks_copy<16>(to, k + h * 8 * HD + j * 64);
-        const uint8_t* v = a.c.v + (row + 2 * c) * HD + r * VB;
-        to += lane * (VB - 16);
+          for (int j = 0; j < KJ; j++) t.k[h][j] = ld_128(k + h * 8 * HD + j * 64);
 #pragma unroll
-        for (int h = 0; h < 4; h++, to += VB * 32) ks_copy<VB>(to, v + ((h >> 1) * 8 + (h & 1)) * HD);
-        to += lane * (8 - VB);
-        const __half2* s = a.c.scales + row;
-        ks_copy<8>(to, s + 2 * c);
-        ks_copy<8>(to + 256, s + 2 * c + 8);
-        to -= lane * 4;
-        ks_copy<4>(to + 512, s + r);
-        ks_copy<4>(to + 640, s + r + 8);
-      };
-#pragma unroll
-      for (int i = 0; i < KS_STAGES - 1; i++) {
-        if (i < n_tiles) request(i);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      }
-
-      // ---- fragments of q^T: the lane's column is nt * 8 + r
-      uint32_t qf[NT][KJ * 4][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        const int col = nt * 8 + r, i = col / a.n_rep;
-        const long long row = row0 + (long long)i * a.step;
-        const bool have = col < n_cols && row >= 0 && row < a.R;
-        const __half* q = a.x + (size_t)(have ? row : 0) * a.ldx + (size_t)(g * a.n_rep + col % a.n_rep) * HD + c * 16;
-#pragma unroll
-        for (int j = 0; j < KJ; j++) {
-          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-          if (have) {
-            lo = ld_128(q + j * 64);
-            hi = ld_128(q + j * 64 + 8);
-            if (NEW && a.table && stored) {
-              const __half* turn = a.table + (size_t)p0 * HD + c * 16 + j * 64;
-              lo = kvq_rotate(lo, ld_128(turn));
-              hi = kvq_rotate(hi, ld_128(turn + 8));
-            }
+        for (int h = 0; h < 4; h++) {
+          const uint8_t* from = v + ((h >> 1) * 8 + (h & 1)) * HD;
+          if (VB == 16) {
+            const uint4 x = ld_128(from);
+            t.v[h][0] = x.x; t.v[h][1] = x.y; t.v[h][VB / 4 - 2] = x.z; t.v[h][VB / 4 - 1] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(from);
+            t.v[h][0] = x.x; t.v[h][1] = x.y;
           }
-          qf[nt][j * 4][0] = lo.x; qf[nt][j * 4][1] = lo.y; qf[nt][j * 4 + 1][0] = lo.z; qf[nt][j * 4 + 1][1] = lo.w;
-          qf[nt][j * 4 + 2][0] = hi.x; qf[nt][j * 4 + 2][1] = hi.y; qf[nt][j * 4 + 3][0] = hi.z; qf[nt][j * 4 + 3][1] = hi.w;
         }
+        t.s0 = s[r];
+        t.s1 = s[r + 8];
+        t.sv0 = *reinterpret_cast<const uint2*>(s + 2 * c);
+        t.sv1 = *reinterpret_cast<const uint2*>(s + 2 * c + 8);
+      };
+      // ---- fragments of q^T: the lane's column is nt * 8 + r.  Everything is asked for before anything is waited for.
+      uint32_t qf[NT][KJ * 4][2];
+      Tile tile;
+      {
+        uint4 x[NT][KJ][2], turn[KJ][2];
+        bool have[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          const int col = nt * 8 + r, i = col / a.n_rep;
+          const long long row = row0 + (long long)i * a.step;
+          have[nt] = col < n_cols && row >= 0 && row < a.R;
+          const __half* q = a.x + (size_t)(have[nt] ? row : 0) * a.ldx + (size_t)(g * a.n_rep + (have[nt] ? col - i * a.n_rep : 0)) * HD + c * 16;
+#pragma unroll
+          for (int j = 0; j < KJ; j++) { x[nt][j][0] = ld_128(q + j * 64); x[nt][j][1] = ld_128(q + j * 64 + 8); }
+        }
+        const bool turned = NEW && a.table && stored;
+        if (turned)
+#pragma unroll
+          for (int j = 0; j < KJ; j++) {
+            const __half* from = a.table + (size_t)p0 * HD + c * 16 + j * 64;
+            turn[j][0] = ld_128(from);
+            turn[j][1] = ld_128(from + 8);
+          }
+        if (n_tiles > 0) load(0, tile);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int j = 0; j < KJ; j++) {
+            uint4 lo = x[nt][j][0], hi = x[nt][j][1];
+            if (turned) { lo = kvq_rotate(lo, turn[j][0]); hi = kvq_rotate(hi, turn[j][1]); }
+            if (!have[nt]) lo = hi = make_uint4(0, 0, 0, 0);
+            qf[nt][j * 4][0] = lo.x; qf[nt][j * 4][1] = lo.y; qf[nt][j * 4 + 1][0] = lo.z; qf[nt][j * 4 + 1][1] = lo.w;
+            qf[nt][j * 4 + 2][0] = hi.x; qf[nt][j * 4 + 2][1] = hi.y; qf[nt][j * 4 + 3][0] = hi.z; qf[nt][j * 4 + 3][1] = hi.w;
+          }
       }
       // ---- the new token, by the CTA with the end of its sequence: stored, and an entry of its own when the warps' sums meet
       const bool entry = stored && j1 == n_units;
@@ -253,19 +269,16 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
         }
       }
       for (int i = 0; i < n_tiles; i++) {
-        if (i + KS_STAGES - 1 < n_tiles) request(i + KS_STAGES - 1);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group %0;" ::"n"(KS_STAGES - 1) : "memory");
-        const unsigned char* stage = ring + (i % KS_STAGES) * Cfg::STAGE;
+        const Tile t = tile;
+        if (i + 1 < n_tiles) load(i + 1, tile);
         const int t0 = t_lo + i * KS_UNIT + warp * 16;
         // scores
-        float s[NT][4];
+        float s[NT][4], s_[NT][4];  // in two chains of products
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s_[nt][0] = s_[nt][1] = s_[nt][2] = s_[nt][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < KJ; j++) {
-          const uint4 k0 = *reinterpret_cast<const uint4*>(stage + j * 512 + lane * 16), k1 = *reinterpret_cast<const uint4*>(stage + (KJ + j) * 512 + lane * 16);
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          const uint32_t w0[4] = {t.k[0][j].x, t.k[0][j].y, t.k[0][j].z, t.k[0][j].w}, w1[4] = {t.k[1][j].x, t.k[1][j].y, t.k[1][j].z, t.k[1][j].w};
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             __half2 a0, a1, a2, a3;
@@ -273,12 +286,12 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
             kvq_widen<FMT>(w1[e], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
-              ks_mma(s[nt], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), qf[nt][j * 4 + e][0], qf[nt][j * 4 + e][1]);
+              ks_mma(e & 1 ? s_[nt] : s[nt], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), qf[nt][j * 4 + e][0], qf[nt][j * 4 + e][1]);
           }
         }
-        const unsigned char* sc = stage + Cfg::K_BYTES + Cfg::V_BYTES;
-        const float ks0 = __low2float(*reinterpret_cast<const __half2*>(sc + 512 + lane * 4)) * a.scale2;
-        const float ks1 = __low2float(*reinterpret_cast<const __half2*>(sc + 640 + lane * 4)) * a.scale2;
+        const float ks0 = __low2float(t.s0) * a.scale2, ks1 = __low2float(t.s1) * a.scale2;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) { s[nt][0] += s_[nt][0]; s[nt][1] += s_[nt][1]; s[nt][2] += s_[nt][2]; s[nt][3] += s_[nt][3]; }
         bool over = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -316,26 +329,13 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
           w[nt][1] = ks_transpose(ks_half2(__floats2half2_rn(e2, e3)));
         }
         // outputs
-        const unsigned char* vs = stage + Cfg::K_BYTES + lane * VB;
-        const uint2 sv0 = *reinterpret_cast<const uint2*>(sc + lane * 8), sv1 = *reinterpret_cast<const uint2*>(sc + 256 + lane * 8);
-        const uint32_t p0_ = __byte_perm(sv0.x, sv0.y, 0x7632), p1_ = __byte_perm(sv1.x, sv1.y, 0x7632);
+        const uint32_t p0_ = __byte_perm(t.sv0.x, t.sv0.y, 0x7632), p1_ = __byte_perm(t.sv1.x, t.sv1.y, 0x7632);
         const __half2 scale0 = *reinterpret_cast<const __half2*>(&p0_), scale1 = *reinterpret_cast<const __half2*>(&p1_);
-        uint32_t v[4][VB / 4];
-#pragma unroll
-        for (int h = 0; h < 4; h++) {
-          if (VB == 16) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vs + h * VB * 32);
-            v[h][0] = x.x; v[h][1] = x.y; v[h][VB / 4 - 2] = x.z; v[h][VB / 4 - 1] = x.w;
-          } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(vs + h * VB * 32);
-            v[h][0] = x.x; v[h][1] = x.y;
-          }
-        }
 #pragma unroll
         for (int e = 0; e < VB / 4; e++)
 #pragma unroll
           for (int half = 0; half < 2; half++) {
-            const uint32_t lo = __byte_perm(v[0][e], v[1][e], half ? 0x7362 : 0x5140), hi = __byte_perm(v[2][e], v[3][e], half ? 0x7362 : 0x5140);
+            const uint32_t lo = __byte_perm(t.v[0][e], t.v[1][e], half ? 0x7362 : 0x5140), hi = __byte_perm(t.v[2][e], t.v[3][e], half ? 0x7362 : 0x5140);
             __half2 a0, a1, a2, a3;
             kvq_widen<FMT>(lo, a0, a1);
             kvq_widen<FMT>(hi, a2, a3);
@@ -346,9 +346,8 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
               ks_mma(o[nt][2 * e + half], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), w[nt][0], w[nt][1]);
           }
       }
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-      // ---- the warps' sums meet (their outputs lie over the ring)
+      // ---- the warps' sums meet 
       float* so = reinterpret_cast<float*>(ks_raw);  // [warp][column][hd]
       __syncthreads();
 #pragma unroll
@@ -408,8 +407,8 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
       }
       if (whole) { __syncthreads(); continue; }
       // ---- pieces of a (sequence, kv head) that CTAs c_lo .. c_hi share: the last to arrive adds them up in this order
-      const long long last = item + n_units - 1;
-      const int c_lo = (int)(((item + 1) * ctas - 1) / total), c_hi = (int)(((last + 1) * ctas - 1) / total), pieces = c_hi - c_lo + 1;
+      const long long begin = item + KS_FIXED, last = begin + n_units - 1;
+      const int c_lo = (int)(((begin + 1) * ctas - 1) / total), c_hi = (int)(((last + 1) * ctas - 1) / total), pieces = c_hi - c_lo + 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) s_ticket = atomicAdd(&a.tickets[c_lo], 1u);
@@ -418,53 +417,66 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? 2 : 1) kvq_split_kernel(
       __threadfence();
       if (tid == 0) a.tickets[c_lo] = 0;
       auto piece = [&](int p) -> const float* { return a.part + (size_t)(2 * (c_lo + p) + (p == 0 ? 1 : 0)) * Cfg::PART; };
-      float* weight = so;  // [column][pieces], at most 2^13 of them: see the launch
-      for (int col = warp; col < COLS; col += KS_WARPS) {
-        float top = -INFINITY, sum = 0.f;
-        for (int p = lane; p < pieces; p += 32) top = fmaxf(top, __ldcg(piece(p) + COLS * HD + col));
-        top = warp_max(top);
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int p = lane; p < pieces; p += 32) {
-          const float f = ks_ex2(__ldcg(piece(p) + COLS * HD + col) - base);
-          weight[col * pieces + p] = f;
-          sum = fmaf(__ldcg(piece(p) + COLS * HD + COLS + col), f, sum);
+      constexpr int NI = COLS * HD / (KS_THREADS * 4), BATCH = NI > 2 ? 2 : NI > 1 ? 4 : 8;  // groups of four values of a thread; pieces whose loads are in flight together
+      float x[NI][4], top[NI], sum[NI];
+#pragma unroll
+      for (int e = 0; e < NI; e++) { x[e][0] = x[e][1] = x[e][2] = x[e][3] = sum[e] = 0.f; top[e] = -INFINITY; }
+#pragma unroll 1
+      for (int p = 0; p < pieces; p += BATCH) {
+        float4 y[BATCH][NI];
+        float pm[BATCH][NI], pl[BATCH][NI];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+          const float* from = piece(min(p + k, pieces - 1));
+#pragma unroll
+          for (int e = 0; e < NI; e++) {
+            const int idx = (tid + e * KS_THREADS) * 4;
+            y[k][e] = __ldcg(reinterpret_cast<const float4*>(from + idx));
+            pm[k][e] = __ldcg(from + COLS * HD + idx / HD);
+            pl[k][e] = __ldcg(from + COLS * HD + COLS + idx / HD);
+          }
         }
-        sum = warp_sum(sum);
-        if (lane == 0) s_l[0][col] = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+#pragma unroll
+        for (int k = 0; k < BATCH; k++)
+#pragma unroll
+          for (int e = 0; e < NI; e++) {
+            if (p + k >= pieces) continue;
+            const float then = fmaxf(top[e], pm[k][e]), base = then == -INFINITY ? 0.f : then, fade = ks_ex2(top[e] - base), f = ks_ex2(pm[k][e] - base);
+            top[e] = then;
+            sum[e] = sum[e] * fade + pl[k][e] * f;
+            x[e][0] = x[e][0] * fade + y[k][e].x * f;
+            x[e][1] = x[e][1] * fade + y[k][e].y * f;
+            x[e][2] = x[e][2] * fade + y[k][e].z * f;
+            x[e][3] = x[e][3] * fade + y[k][e].w * f;
+          }
       }
-      __syncthreads();
-      for (int idx = tid * 4; idx < COLS * HD; idx += KS_THREADS * 4) {
-        const int col = idx / HD;
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int p = 0; p < pieces; p++) {
-          const float f = weight[col * pieces + p];
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(piece(p) + idx));
-          x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
-        }
-        const float inv = s_l[0][col];
-        x[0] *= inv; x[1] *= inv; x[2] *= inv; x[3] *= inv;
-        store(idx, x);
+#pragma unroll
+      for (int e = 0; e < NI; e++) {
+        const float inv = sum[e] == 0.f ? 0.f : __fdiv_rn(1.f, sum[e]);
+        x[e][0] *= inv; x[e][1] *= inv; x[e][2] *= inv; x[e][3] *= inv;
+        store((tid + e * KS_THREADS) * 4, x[e]);
       }
       __syncthreads();
     }
-    at += (long long)n_units * a.c.G;
+    at += (long long)span * a.c.G;
   }
 }
 
-static inline int ks_ctas(const jg_dev* dev) { return 2 * dev->sm_count; }  // that a device runs at once; as many tickets: jg_kvq_ticket_bytes
+static inline int ks_ctas(const jg_dev* dev) { return KS_CTAS * dev->sm_count; }  // that a device runs at once; as many tickets: jg_kvq_ticket_bytes
 static inline int ks_slots(const jg_dev* dev) { return 2 * ks_ctas(dev); }  // pieces in the workspace
 static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 2>::PART : KsCfg<128, 2>::PART; }
 
 template <int FMT, int HD, int NT, bool NEW>
 static int launch_split(jg_dev* dev, const KvqSplitArgs& a) {
   auto kern = kvq_split_kernel<FMT, HD, NT, NEW>;
+  using Cfg = KsCfg<HD, NT>;
+  const size_t smem = Cfg::MERGE;
   static bool attr_set[8] = {};
   if (!attr_set[dev->ordinal & 7]) {
-    JG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)KsCfg<HD, NT>::SMEM));
+    JG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attr_set[dev->ordinal & 7] = true;
   }
   const long long most = (long long)a.B * a.c.G * ((a.c.max_ctx + KS_UNIT - 1) / KS_UNIT);
-  return jg_launch(dev, NEW ? "kvq_decode" : "kvq_attn", kern, dim3((unsigned)(most < ks_ctas(dev) ? most : ks_ctas(dev))), dim3(KS_THREADS), KsCfg<HD, NT>::SMEM, a);
+  return jg_launch(dev, NEW ? "kvq_decode" : "kvq_attn", kern, dim3((unsigned)(most < ks_ctas(dev) ? most : ks_ctas(dev))), dim3(KS_THREADS), smem, a);
 }
 #endif
