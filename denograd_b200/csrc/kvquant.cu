@@ -126,42 +126,59 @@ struct KvqWriteArgs {
 
 constexpr int KW_THREADS = 256;
 
-// A thread for each eight values of a row's Q heads, and of its K heads together with V.
-template <int FMT, int HD>
+// A thread for each eight values of a row's Q heads, and of its K heads together with V, of U neighbouring rows: all their loads
+// are on their way before any is waited for (positions and slots are not needed for the values, only for where they go).
+template <int FMT, int HD, int U>
 __global__ void __launch_bounds__(KW_THREADS) kvq_write_kernel(const KvqWriteArgs a) {
   constexpr int LPR = HD / 8;
   pdl_launch();
   pdl_wait();
-  const unsigned per_row = (unsigned)(a.H + a.c.G) * LPR, at = blockIdx.x * (unsigned)KW_THREADS + threadIdx.x;
-  const unsigned row = at / per_row;
-  const int piece = (int)(at - row * per_row), head = piece / LPR, sub = piece % LPR;
-  int t = -1;
-  const int32_t* bt_row = nullptr;
-  if (row < (unsigned)a.R) {
-    const int sq = a.seq ? a.seq[row] : (int)row;
-    t = a.pos[row];
-    if ((unsigned)sq >= (unsigned)a.c.n_seq || (unsigned)t >= (unsigned)a.c.max_ctx || (a.table && t >= a.table_rows)) t = -1;
-    else bt_row = a.c.block_table + (size_t)sq * a.c.max_pages;
+  const unsigned per_row = (unsigned)(a.H + a.c.G) * LPR, at = blockIdx.x * (unsigned)KW_THREADS + threadIdx.x, group = at / per_row;
+  const int piece = (int)(at - group * per_row), head = piece / LPR, sub = piece % LPR;
+  const bool is_q = head < a.H;
+  const int row0 = (int)group * U;
+  uint4 v[U], w[U], turn[U];
+  int t[U], sq[U];
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    const bool in = row0 + k < a.R;
+    const __half* x = a.qkv + (size_t)(in ? row0 + k : 0) * a.ldx + (size_t)head * HD + sub * 8;
+    t[k] = in ? a.pos[row0 + k] : -1;
+    sq[k] = in ? (a.seq ? a.seq[row0 + k] : row0 + k) : -1;
+    v[k] = w[k] = turn[k] = make_uint4(0, 0, 0, 0);
+    if (in && (!is_q || a.q_out)) v[k] = ld_128(x);
+    if (in && !is_q) w[k] = ld_128(x + (size_t)a.c.G * HD);
   }
-  const __half* x = a.qkv + (size_t)row * a.ldx + (size_t)head * HD + sub * 8;
-  const bool live = t >= 0, is_q = head < a.H;
-  uint4 v = make_uint4(0, 0, 0, 0), w = v;
-  if (live && (!is_q || a.q_out)) {
-    v = ld_128(x);
-    if (!is_q) w = ld_128(x + (size_t)a.c.G * HD);
-    if (a.table) v = kvq_rotate(v, ld_128(a.table + (size_t)t * HD + sub * 8));
-    if (is_q) *reinterpret_cast<uint4*>(a.q_out + (size_t)row * a.ldq + (size_t)head * HD + sub * 8) = v;
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    if ((unsigned)sq[k] >= (unsigned)a.c.n_seq || (unsigned)t[k] >= (unsigned)a.c.max_ctx || (a.table && t[k] >= a.table_rows)) t[k] = -1;
+    if (a.table && t[k] >= 0) turn[k] = ld_128(a.table + (size_t)t[k] * HD + sub * 8);
   }
-  if (__all_sync(0xffffffffu, is_q || !live)) return;
-  uint2 kc, vc;
-  __half2 scale;
-  kvq_quantise<FMT, LPR>(v, w, kc, vc, scale);
-  if (live && !is_q) {
-    const size_t to = kvq_row(a.c, bt_row, t, head - a.H);
-    *reinterpret_cast<uint2*>(a.c.k + to * HD + sub * 8) = kc;
-    *reinterpret_cast<uint2*>(a.c.v + to * HD + sub * 8) = vc;
-    if (sub == 0) a.c.scales[to] = scale;
+  size_t to[U];
+#pragma unroll
+  for (int k = 0; k < U; k++) to[k] = !is_q && t[k] >= 0 ? kvq_row(a.c, a.c.block_table + (size_t)sq[k] * a.c.max_pages, t[k], head - a.H) : 0;
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    if (a.table) v[k] = kvq_rotate(v[k], turn[k]);
+    if (is_q && a.q_out && t[k] >= 0) *reinterpret_cast<uint4*>(a.q_out + (size_t)(row0 + k) * a.ldq + (size_t)head * HD + sub * 8) = v[k];
+    if (__all_sync(0xffffffffu, is_q || t[k] < 0)) continue;
+    uint2 kc, vc;
+    __half2 scale;
+    kvq_quantise<FMT, LPR>(v[k], w[k], kc, vc, scale);
+    if (!is_q && t[k] >= 0) {
+      *reinterpret_cast<uint2*>(a.c.k + to[k] * HD + sub * 8) = kc;
+      *reinterpret_cast<uint2*>(a.c.v + to[k] * HD + sub * 8) = vc;
+      if (sub == 0) a.c.scales[to[k]] = scale;
+    }
   }
+}
+
+template <int FMT, int HD>
+static int launch_write(jg_dev* dev, const KvqWriteArgs& a) {
+  // four rows to a thread where that leaves every SM eight CTAs; below, one
+  const unsigned long long per_row = (unsigned long long)(a.H + a.c.G) * (HD / 8), four = ((a.R + 3) / 4 * per_row + KW_THREADS - 1) / KW_THREADS;
+  if (four >= 8ull * dev->sm_count) return jg_launch(dev, "kvq_write", kvq_write_kernel<FMT, HD, 4>, dim3((unsigned)four), dim3(KW_THREADS), 0, a);
+  return jg_launch(dev, "kvq_write", kvq_write_kernel<FMT, HD, 1>, dim3((unsigned)((a.R * per_row + KW_THREADS - 1) / KW_THREADS)), dim3(KW_THREADS), 0, a);
 }
 
 JG_API int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, int32_t ldq, uint64_t qkv, int32_t ldx, uint64_t table,
@@ -183,12 +200,8 @@ JG_API int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, 
   a.q_out = (__half*)q_out; a.qkv = (const __half*)qkv; a.table = (const __half*)table;
   a.pos = (const int32_t*)pos; a.seq = (const int32_t*)seq;
   a.ldq = ldq; a.ldx = ldx; a.table_rows = table_rows; a.R = R; a.H = H;
-  const dim3 grid((unsigned)((pieces + KW_THREADS - 1) / KW_THREADS)), block(KW_THREADS);
-  if (kv->format == JG_KVQ_INT8)
-    return hd == 64 ? jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_INT8, 64>, grid, block, 0, a)
-                    : jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_INT8, 128>, grid, block, 0, a);
-  return hd == 64 ? jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_E4M3, 64>, grid, block, 0, a)
-                  : jg_launch(dev, "kvq_write", kvq_write_kernel<KVQ_E4M3, 128>, grid, block, 0, a);
+  if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_write<KVQ_INT8, 64>(dev, a) : launch_write<KVQ_INT8, 128>(dev, a);
+  return hd == 64 ? launch_write<KVQ_E4M3, 64>(dev, a) : launch_write<KVQ_E4M3, 128>(dev, a);
 }
 
 // ------------------------------------------------------------------------------------------------ reading back
@@ -205,39 +218,65 @@ struct KvqReadArgs {
 
 constexpr int KR_THREADS = 256;
 
-// A thread for each eight values of K and the eight of V beside them.
-template <int FMT, int HD>
+// A thread for each eight values of K and the eight of V beside them, of U neighbouring positions, whose loads are in flight together.
+template <int FMT, int HD, int U>
 __global__ void __launch_bounds__(KR_THREADS) kvq_read_kernel(const KvqReadArgs a) {
   constexpr int LPR = HD / 8;
   pdl_launch();
   pdl_wait();
   const int b = blockIdx.y;
-  const unsigned per_row = (unsigned)a.c.G * LPR, at = blockIdx.x * (unsigned)KR_THREADS + threadIdx.x, i = at / per_row;
-  const int n = a.count ? min(a.count[b], a.max_count) : a.max_count;
-  if ((long long)i >= n) return;
-  const int piece = (int)(at - i * per_row), g = piece / LPR, sub = piece % LPR;
-  const long long row = (long long)(a.first ? a.first[b] : b) + (long long)i * a.step, t = (long long)a.pos[b] + i;
-  if (row < 0 || row >= a.R) return;
-  const int sq = a.seq ? a.seq[b] : b;
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if ((unsigned)sq < (unsigned)a.c.n_seq && t >= 0 && t < a.c.max_ctx) {
-    const size_t from = kvq_row(a.c, a.c.block_table + (size_t)sq * a.c.max_pages, (int)t, g);
-    const uint2 kc = *reinterpret_cast<const uint2*>(a.c.k + from * HD + sub * 8), vc = *reinterpret_cast<const uint2*>(a.c.v + from * HD + sub * 8);
-    const __half2 scale = a.c.scales[from];
-    const __half2 sk = __low2half2(scale), sv = __hisnan(__low2half(scale)) ? sk : __high2half2(scale);
+  const unsigned per_row = (unsigned)a.c.G * LPR, at = blockIdx.x * (unsigned)KR_THREADS + threadIdx.x, group = at / per_row;
+  const int count = a.count ? a.count[b] : a.max_count, first = a.first ? a.first[b] : b, p0 = a.pos[b], sq = a.seq ? a.seq[b] : b;
+  const int n = min(count, a.max_count);
+  const long long i0 = (long long)group * U;
+  if (i0 >= n) return;
+  const int piece = (int)(at - group * per_row), g = piece / LPR, sub = piece % LPR;
+  const bool known = (unsigned)sq < (unsigned)a.c.n_seq;
+  const int32_t* bt_row = a.c.block_table + (size_t)(known ? sq : 0) * a.c.max_pages;
+  size_t from[U];
+  bool live[U];
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    const long long t = p0 + i0 + k;
+    live[k] = known && i0 + k < n && t >= 0 && t < a.c.max_ctx;
+    from[k] = live[k] ? kvq_row(a.c, bt_row, (int)t, g) : 0;
+  }
+  uint2 kc[U], vc[U];
+  __half2 scale[U];
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    kc[k] = vc[k] = make_uint2(KVQ_ZERO<FMT>, KVQ_ZERO<FMT>);
+    scale[k] = __half2half2(__ushort_as_half(0));
+    if (live[k]) {
+      kc[k] = *reinterpret_cast<const uint2*>(a.c.k + from[k] * HD + sub * 8);
+      vc[k] = *reinterpret_cast<const uint2*>(a.c.v + from[k] * HD + sub * 8);
+      scale[k] = a.c.scales[from[k]];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    const long long row = first + (i0 + k) * a.step;
+    if (i0 + k >= n || row < 0 || row >= a.R) continue;
+    const __half2 sk = __low2half2(scale[k]), sv = __hisnan(__low2half(scale[k])) ? sk : __high2half2(scale[k]);
     __half2 h[4], w[4];
-    kvq_widen<FMT>(kc.x, h[0], h[1]);
-    kvq_widen<FMT>(kc.y, h[2], h[3]);
-    kvq_widen<FMT>(vc.x, w[0], w[1]);
-    kvq_widen<FMT>(vc.y, w[2], w[3]);
+    kvq_widen<FMT>(kc[k].x, h[0], h[1]);
+    kvq_widen<FMT>(kc[k].y, h[2], h[3]);
+    kvq_widen<FMT>(vc[k].x, w[0], w[1]);
+    kvq_widen<FMT>(vc[k].y, w[2], w[3]);
 #pragma unroll
     for (int j = 0; j < 4; j++) { h[j] = __hmul2_rn(h[j], sk); w[j] = __hmul2_rn(w[j], sv); }
-    k = *reinterpret_cast<const uint4*>(h);
-    v = *reinterpret_cast<const uint4*>(w);
+    const size_t to = (size_t)row * a.ld + (size_t)g * HD + sub * 8;
+    *reinterpret_cast<uint4*>(a.k + to) = *reinterpret_cast<const uint4*>(h);
+    *reinterpret_cast<uint4*>(a.v + to) = *reinterpret_cast<const uint4*>(w);
   }
-  const size_t to = (size_t)row * a.ld + (size_t)g * HD + sub * 8;
-  *reinterpret_cast<uint4*>(a.k + to) = k;
-  *reinterpret_cast<uint4*>(a.v + to) = v;
+}
+
+template <int FMT, int HD>
+static int launch_read(jg_dev* dev, const KvqReadArgs& a, int B) {
+  // four positions to a thread where that leaves every SM eight CTAs; below, one
+  const unsigned long long per_row = (unsigned long long)a.c.G * (HD / 8), four = ((a.max_count + 3) / 4 * per_row + KR_THREADS - 1) / KR_THREADS;
+  if (four * B >= 8ull * dev->sm_count) return jg_launch(dev, "kvq_read", kvq_read_kernel<FMT, HD, 4>, dim3((unsigned)four, (unsigned)B), dim3(KR_THREADS), 0, a);
+  return jg_launch(dev, "kvq_read", kvq_read_kernel<FMT, HD, 1>, dim3((unsigned)((a.max_count * per_row + KR_THREADS - 1) / KR_THREADS), (unsigned)B), dim3(KR_THREADS), 0, a);
 }
 
 JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint64_t v, int32_t ld, int32_t R, uint64_t pos, uint64_t count,
@@ -257,10 +296,6 @@ JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint6
   a.k = (__half*)k; a.v = (__half*)v;
   a.pos = (const int32_t*)pos; a.count = (const int32_t*)count; a.first = (const int32_t*)first; a.seq = (const int32_t*)seq;
   a.ld = ld; a.R = R; a.max_count = max_count; a.step = step;
-  const dim3 grid((unsigned)((pieces + KR_THREADS - 1) / KR_THREADS), (unsigned)B), block(KR_THREADS);
-  if (kv->format == JG_KVQ_INT8)
-    return hd == 64 ? jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_INT8, 64>, grid, block, 0, a)
-                    : jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_INT8, 128>, grid, block, 0, a);
-  return hd == 64 ? jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_E4M3, 64>, grid, block, 0, a)
-                  : jg_launch(dev, "kvq_read", kvq_read_kernel<KVQ_E4M3, 128>, grid, block, 0, a);
+  if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_read<KVQ_INT8, 64>(dev, a, B) : launch_read<KVQ_INT8, 128>(dev, a, B);
+  return hd == 64 ? launch_read<KVQ_E4M3, 64>(dev, a, B) : launch_read<KVQ_E4M3, 128>(dev, a, B);
 }

@@ -5,8 +5,8 @@
 //   e4m3   scale = the least 2^e with max|x| / 2^e <= 448, e >= -15,                                  code = e4m3(x / scale)
 // A code has at most 7 significant bits (int8) or 4 (e4m3), so code * scale has at most 11 and is an fp16 number: what
 // attends to the cache multiplies fp16 values, exact, and needs no scale inside a sum.  Rounding int8's scale up costs up to an
-// eighth of a step (0.5 dB), which is the price of that.  The quotients are computed in 32 bits and never round across a border:
-// max|x| has 11 significant bits, so a quotient that is not on a border is at least 2^-12 of itself away from it.
+// eighth of a step (0.5 dB), which is the price of that.  The scales' quotients are computed in 32 bits and never round across a
+// border: max|x| has 11 significant bits, so a quotient that is not on a border is at least 2^-12 of itself away from it.
 // A value beyond 65504 (rounded up from just below) becomes the next lower code.
 // A row with a NaN or an infinity in its K or V has no codes that could stand for it: its K scale is NaN and the V row zero.
 // Scores against it are NaN, so every query that sees the position becomes NaN, and no other: a masked NaN is replaced, but a
@@ -95,21 +95,36 @@ __device__ __forceinline__ float kvq_scale(float a) {
   const uint32_t s = (__float_as_uint(__fdiv_rn(a, 448.f)) + 0x7FFFFFu) & ~0x7FFFFFu;  // the next power of two
   return fmaxf(__uint_as_float(s), 3.0517578125e-05f);
 }
-// Four values as a word of codes.
+// What a row's values are multiplied by to be codes, and the largest code.
 template <int FMT>
-__device__ __forceinline__ uint32_t kvq_codes(const float (&x)[4], float scale) {
+__device__ __forceinline__ float kvq_inverse(float scale) {
+  if (FMT == KVQ_INT8) return __fdiv_rn(1.f, scale);
+  return __uint_as_float(0x7F000000u - __float_as_uint(scale));  // 2^-e
+}
+// Four values as a word of codes.
+// int8: x times the rounded 1 / scale is off by less than 2^-16 from x / scale, which is at most 127.  A quotient that is no tie is at least
+// 2^-12 away from one (x has 11 significant bits, scale 4), so rounding to multiples of 2^-13 first makes ties of the ties and of
+// nothing else.  Adding 1536 is that rounding, adding 1.5 2^23 the one to whole numbers, and 128 more the code's bias.
+template <int FMT>
+__device__ __forceinline__ uint32_t kvq_codes(const float (&x)[4], float scale, float inverse) {
   if (!(scale > 0.f)) return KVQ_ZERO<FMT>;
   if (FMT == KVQ_INT8) {
-    const float top = fminf(127.f, floorf(__fdiv_rn(65504.f, scale)));
-    uint32_t w = 0;
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) w |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x[i], scale)), -top), top) + 128u) << (8 * i);
-    return w;
+    for (int i = 0; i < 4; i++) {
+      float q = __fmul_rn(x[i], inverse);
+      if (scale >= 512.f) {  // values may pass 65504: the next lower code
+        const float top = floorf(__fdiv_rn(65504.f, scale));
+        q = fminf(fmaxf(q, -top), top);
+      }
+      w[i] = __float_as_uint(__fadd_rn(__fadd_rn(__fadd_rn(q, 1536.f), -1536.f), 12583040.f));
+    }
+    return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
   }
-  const float up = __uint_as_float(0x7F000000u - __float_as_uint(scale)), top = scale < 256.f ? 448.f : 240.f;  // 1 / 2^e
+  const float top = scale < 256.f ? 448.f : 240.f;
   float y[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) y[i] = fminf(fmaxf(x[i] * up, -top), top);
+  for (int i = 0; i < 4; i++) y[i] = fminf(fmaxf(x[i] * inverse, -top), top);
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
@@ -132,33 +147,33 @@ __device__ __forceinline__ uint4 kvq_rotate(const uint4& x, const uint4& t) {
 // A K and a V row spread over LPR neighbouring lanes, eight values each (K rotated already): their codes and scales.
 template <int FMT, int LPR>
 __device__ __forceinline__ void kvq_quantise(const uint4& k, const uint4& v, uint2& kc, uint2& vc, __half2& scale) {
-  float x[8], y[8];
-  unpack8(k, x);
-  unpack8(v, y);
-  float a = 0.f, b = 0.f;
-  bool fine = true;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    a = fmaxf(a, fabsf(x[i]));
-    b = fmaxf(b, fabsf(y[i]));
-    fine = fine && fabsf(x[i]) <= 65504.f && fabsf(y[i]) <= 65504.f;
-  }
-  if (!fine) a = INFINITY;
+  // the largest magnitudes, K's and V's as one pair of halves; a NaN stays
+  const auto top = [](const uint4& v) {
+    const uint32_t w[4] = {v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu, v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu};
+    const __half2* h = reinterpret_cast<const __half2*>(w);
+    return __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  };
+  const __half2 tk = top(k), tv = top(v);
+  __half2 t = __hmax2_nan(__lows2half2(tk, tv), __highs2half2(tk, tv));
 #pragma unroll
   for (int o = LPR / 2; o > 0; o >>= 1) {
-    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&t), o);
+    t = __hmax2_nan(t, *reinterpret_cast<const __half2*>(&other));
   }
-  if (a == INFINITY) {
+  const float a = __low2float(t), b = __high2float(t);
+  if (!(a <= 65504.f) || !(b <= 65504.f)) {
     kc = vc = make_uint2(KVQ_ZERO<FMT>, KVQ_ZERO<FMT>);
     scale = __halves2half2(__ushort_as_half(0x7FFF), __ushort_as_half(0));
     return;
   }
-  const float sk = kvq_scale<FMT>(a), sv = kvq_scale<FMT>(b);
-  kc.x = kvq_codes<FMT>({x[0], x[1], x[2], x[3]}, sk);
-  kc.y = kvq_codes<FMT>({x[4], x[5], x[6], x[7]}, sk);
-  vc.x = kvq_codes<FMT>({y[0], y[1], y[2], y[3]}, sv);
-  vc.y = kvq_codes<FMT>({y[4], y[5], y[6], y[7]}, sv);
+  float x[8], y[8];
+  unpack8(k, x);
+  unpack8(v, y);
+  const float sk = kvq_scale<FMT>(a), sv = kvq_scale<FMT>(b), ik = kvq_inverse<FMT>(sk), iv = kvq_inverse<FMT>(sv);
+  kc.x = kvq_codes<FMT>({x[0], x[1], x[2], x[3]}, sk, ik);
+  kc.y = kvq_codes<FMT>({x[4], x[5], x[6], x[7]}, sk, ik);
+  vc.x = kvq_codes<FMT>({y[0], y[1], y[2], y[3]}, sv, iv);
+  vc.y = kvq_codes<FMT>({y[4], y[5], y[6], y[7]}, sv, iv);
   scale = __floats2half2_rn(sk, sv);
 }
 #endif

@@ -21,26 +21,29 @@ from .device import CUDA, Tensor
 FORMATS = {"int8": ffi.KVQ_INT8, "fp8": ffi.KVQ_E4M3}
 
 
-def _ints(name: str, t: Tensor | None, n: int | None = None) -> int:
+def _ints(name: str, t: Tensor | None, n: int) -> int:
+    """Its address, or 0 where it is not given."""
     if t is None:
         return 0
-    if t.dtype != "int32":
-        raise TypeError(f"{name} is {t.dtype}, not int32")
-    if n is not None and t.numel() < n:
-        raise ValueError(f"{name} has {t.numel()} entries, {n} are needed")
-    return t.ptr
+    buf = t.buf
+    if buf.dtype != "int32":
+        raise TypeError(f"{name} is {buf.dtype}, not int32")
+    if buf.size < n:
+        raise ValueError(f"{name} has {buf.size} entries, {n} are needed")
+    return buf.ptr
 
 
-def _rows(name: str, t: Tensor, columns: int, rows: int | None = None) -> int:
-    """The row stride of a tensor of fp16 rows."""
-    if t.dtype != "float16":
-        raise TypeError(f"{name} is {t.dtype}, not float16")
-    ld = t.shape[-1]
+def _rows(name: str, t: Tensor, columns: int, rows: int = 0) -> tuple[int, int, int]:
+    """(address, row stride, rows) of a tensor of fp16 rows."""
+    buf, ld = t.buf, t.shape[-1]
+    if buf.dtype != "float16":
+        raise TypeError(f"{name} is {buf.dtype}, not float16")
     if ld < columns:
         raise ValueError(f"{name} has rows of {ld}, {columns} are needed")
-    if rows is not None and t.numel() // ld < rows:
-        raise ValueError(f"{name} has {t.numel() // ld} rows, {rows} are needed")
-    return ld
+    have = buf.size // ld
+    if have < rows:
+        raise ValueError(f"{name} has {have} rows, {rows} are needed")
+    return buf.ptr, ld, have
 
 
 class QuantKVCache:
@@ -56,6 +59,7 @@ class QuantKVCache:
         self.max_pages_per_seq = (max_context + page_size - 1) // page_size
         self.n_pages = n_pages if n_pages is not None else self.max_pages_per_seq * max_batch
         self.max_batch = max_batch
+        self._q, self._kv, self._qkv = n_heads * head_dim, n_kv_heads * head_dim, (n_heads + 2 * n_kv_heads) * head_dim  # columns
         d = ffi.KvDesc(n_layers, n_kv_heads, head_dim, page_size, self.n_pages, max_batch, self.max_pages_per_seq, n_heads, 0)
         self.handle = C.c_void_p()
         ffi.call("jg_kvq_create", dev.handle, C.byref(d), FORMATS[dtype], C.byref(self.handle))
@@ -76,24 +80,21 @@ class QuantKVCache:
               q_out: Tensor | None = None) -> None:
         """Rotates Q and K of every row of `qkv` (by `freqs_cis`, or not at all) and stores K and V: row r is position pos[r] of slot
         seq[r] (None: slot r).  Rotated Q goes to `q_out`, which may be `qkv`.  The rows name different positions."""
-        hd, H = self.head_dim, self.n_heads
-        ldx = _rows("qkv", qkv, (H + 2 * self.n_kv_heads) * hd)
-        R = qkv.numel() // ldx
-        self.dev.call("jg_kvq_write", self.handle, layer, q_out.ptr if q_out is not None else 0,
-                      _rows("q_out", q_out, H * hd, R) if q_out is not None else 0, qkv.ptr, ldx, *self._table(freqs_cis), _ints("pos", pos, R),
-                      _ints("seq", seq, R), R, H)
+        x, ldx, R = _rows("qkv", qkv, self._qkv)
+        to, ldq, _ = _rows("q_out", q_out, self._q, R) if q_out is not None else (0, 0, 0)
+        table, n = self._table(freqs_cis)
+        self.dev.call("jg_kvq_write", self.handle, layer, to, ldq, x, ldx, table, n, _ints("pos", pos, R), _ints("seq", seq, R), R, self.n_heads)
 
     def decode(self, layer: int, qkv: Tensor, pos: Tensor, freqs_cis: Tensor | None = None, seq: Tensor | None = None,
                out: Tensor | None = None) -> Tensor:
         """One new token for each row of `qkv`, rows in different slots: stores it as `write` does and attends to positions 0 .. pos[b].
         `qkv` is left as it is.  A row whose position lies outside the cache gets zeros."""
-        hd, H = self.head_dim, self.n_heads
-        ldx = _rows("qkv", qkv, (H + 2 * self.n_kv_heads) * hd)
-        B = qkv.numel() // ldx
+        x, ldx, B = _rows("qkv", qkv, self._qkv)
         if out is None:
-            out = Tensor.empty((B, H * hd), "float16", self.dev)
-        self.dev.call("jg_kvq_decode", self.handle, layer, out.ptr, _rows("out", out, H * hd, B), qkv.ptr, ldx, *self._table(freqs_cis),
-                      _ints("pos", pos, B), _ints("seq", seq, B), B, H)
+            out = Tensor.empty((B, self._q), "float16", self.dev)
+        to, ldo, _ = _rows("out", out, self._q, B)
+        table, n = self._table(freqs_cis)
+        self.dev.call("jg_kvq_decode", self.handle, layer, to, ldo, x, ldx, table, n, _ints("pos", pos, B), _ints("seq", seq, B), B, self.n_heads)
         return out
 
     def attend(self, layer: int, q: Tensor, pos: Tensor, count: Tensor | None = None, first: Tensor | None = None,
@@ -102,51 +103,49 @@ class QuantKVCache:
         count[b], is row first[b] + i * step of `q` (rotated) and of `out`, and sees positions 0 .. pos[b] + i of slot seq[b].
         Defaults: max_count positions each (all rows, dealt evenly), in position-major order (row i * B + b).  A ragged batch has
         running sums in `first`, step=1, and the largest count as `max_count`.  Rows that no sequence names stay as they are (zeros where `out` is not given)."""
-        hd, H = self.head_dim, self.n_heads
-        ldq = _rows("q", q, H * hd)
-        R = q.numel() // ldq
-        where, B, most, step = self._where(R, pos, count, first, seq, max_count, step)
+        x, ldq, R = _rows("q", q, self._q)
         if out is None:
-            out = Tensor.zeros((R, H * hd), "float16", self.dev)
-        self.dev.call("jg_kvq_attn", self.handle, layer, out.ptr, _rows("out", out, H * hd, R), q.ptr, ldq, R, *where, B, most, step, H)
+            out = Tensor.zeros((R, self._q), "float16", self.dev)
+        to, ldo, _ = _rows("out", out, self._q, R)
+        self.dev.call("jg_kvq_attn", self.handle, layer, to, ldo, x, ldq, R, *self._where(R, pos, count, first, seq, max_count, step), self.n_heads)
         return out
 
     def read(self, layer: int, pos: Tensor, count: Tensor | None = None, first: Tensor | None = None, seq: Tensor | None = None,
              max_count: int | None = None, step: int | None = None, k: Tensor | None = None, v: Tensor | None = None,
              rows: int | None = None) -> tuple[Tensor, Tensor]:
         """K and V of stretches of the cache as fp16 rows, named as in `attend`; `rows` of them are made where `k` and `v` are not given."""
-        width = self.n_kv_heads * self.head_dim
         if (k is None) != (v is None):
             raise ValueError("k and v are given together")
         if k is None:
             if rows is None:
                 raise ValueError("give k and v, or the number of rows")
-            k, v = (Tensor.zeros((rows, width), "float16", self.dev) for _ in range(2))
-        ld = _rows("k", k, width)
-        R = k.numel() // ld
-        if _rows("v", v, width, R) != ld:
-            raise ValueError(f"k has rows of {ld}, v of {v.shape[-1]}")
-        where, B, most, step = self._where(R, pos, count, first, seq, max_count, step)
-        self.dev.call("jg_kvq_read", self.handle, layer, k.ptr, v.ptr, ld, R, *where, B, most, step)
+            k, v = (Tensor.zeros((rows, self._kv), "float16", self.dev) for _ in range(2))
+        to_k, ld, R = _rows("k", k, self._kv)
+        to_v, ldv, _ = _rows("v", v, self._kv, R)
+        if ldv != ld:
+            raise ValueError(f"k has rows of {ld}, v of {ldv}")
+        self.dev.call("jg_kvq_read", self.handle, layer, to_k, to_v, ld, R, *self._where(R, pos, count, first, seq, max_count, step))
         return k, v
 
     def _table(self, freqs_cis: Tensor | None) -> tuple[int, int]:
         if freqs_cis is None:
             return 0, 0
-        if freqs_cis.dtype != "float16" or tuple(freqs_cis.shape[1:]) != (self.head_dim // 2, 2):
-            raise ValueError(f"freqs_cis is {freqs_cis.dtype} {tuple(freqs_cis.shape)}, not float16 [positions, {self.head_dim // 2}, 2]")
-        return freqs_cis.ptr, freqs_cis.shape[0]
+        shape = freqs_cis.shape
+        if freqs_cis.buf.dtype != "float16" or len(shape) != 3 or shape[2] != 2 or shape[1] * 2 != self.head_dim:
+            raise ValueError(f"freqs_cis is {freqs_cis.dtype} {tuple(shape)}, not float16 [positions, {self.head_dim // 2}, 2]")
+        return freqs_cis.buf.ptr, shape[0]
 
     @staticmethod
-    def _where(R: int, pos: Tensor, count, first, seq, max_count: int | None, step: int | None):
-        B = pos.numel()
+    def _where(R: int, pos: Tensor, count, first, seq, max_count: int | None, step: int | None) -> tuple:
+        """(pos, count, first, seq, sequences, max_count, step) of a call."""
+        B = pos.buf.size
         if max_count is None:
             if R % B or count is not None or first is not None:
                 raise ValueError("max_count is needed where sequences have different numbers of rows")
             max_count = R // B
         if step is None:
             step = B if first is None else 1
-        return (_ints("pos", pos), _ints("count", count, B), _ints("first", first, B), _ints("seq", seq, B)), B, max_count, step
+        return _ints("pos", pos, B), _ints("count", count, B), _ints("first", first, B), _ints("seq", seq, B), B, max_count, step
 
     def close(self) -> None:
         if self.handle:
