@@ -84,7 +84,7 @@ static inline int jg_after_launch(jg_dev* dev, const char* name) {
     JG_CUDA(cudaSetDevice((dev)->ordinal));                        \
   } while (0)
 
-static inline size_t jg_kvq_ticket_bytes(const jg_dev* dev) { return (size_t)4 * dev->sm_count * sizeof(unsigned int); }
+static inline size_t jg_kvq_ticket_bytes(const jg_dev* dev) { return (size_t)6 * dev->sm_count * sizeof(unsigned int); }
 static inline bool jg_aligned(uint64_t p, uint64_t a) { return p != 0 && (p % a) == 0; }
 constexpr unsigned JG_FRESH_RING = 16;
 static inline void jg_mark_fresh(jg_dev* dev, uint64_t lo, uint64_t bytes) {

@@ -5,8 +5,8 @@
 //   e4m3   scale = the least 2^e with max|x| / 2^e <= 448, e >= -15,                                  code = e4m3(x / scale)
 // A code has at most 7 significant bits (int8) or 4 (e4m3), so code * scale has at most 11 and is an fp16 number: what
 // attends to the cache multiplies fp16 values, exact, and needs no scale inside a sum.  Rounding int8's scale up costs up to an
-// eighth of a step (0.5 dB), which is the price of that.  The scales' quotients are computed in 32 bits and never round across a
-// border: max|x| has 11 significant bits, so a quotient that is not on a border is at least 2^-12 of itself away from it.
+// eighth of a step (0.5 dB), which is the price of that.  A quotient that is not on a border between two scales is at least
+// 2^-12 of itself away from it, since max|x| has 11 significant bits: 32 bits are enough to be exact.
 // A value beyond 65504 (rounded up from just below) becomes the next lower code.
 // A row with a NaN or an infinity in its K or V has no codes that could stand for it: its K scale is NaN and the V row zero.
 // Scores against it are NaN, so every query that sees the position becomes NaN, and no other: a masked NaN is replaced, but a
@@ -83,50 +83,46 @@ __device__ __forceinline__ void kvq_widen(uint32_t w, __half2& lo, __half2& hi) 
   }
 }
 
-// The scale of a row whose largest magnitude is a (finite).
+// The scale of a row whose largest magnitude is a (finite).  The quotient is a product with a constant that is 2^-20 of itself too
+// small: less than a quotient beyond a border is away from it, more than the roundings, so one on a border is rounded up to it.
 template <int FMT>
 __device__ __forceinline__ float kvq_scale(float a) {
   if (a == 0.f) return 0.f;
   if (FMT == KVQ_INT8) {
-    const float s = __fdiv_rn(a, 127.f);
-    if (s < 4.76837158203125e-07f) return ceilf(s * 16777216.f) * 5.9604644775390625e-08f;  // below 2^-21: multiples of 2^-24
-    return __uint_as_float((__float_as_uint(s) + 0xFFFFFu) & ~0xFFFFFu);                      // 3 bits behind the leading one
+    const float s = a * (float)((1.0 - 0x1p-20) / 127.0);
+    if (s < 0x1p-21f) return ceilf(s * 0x1p24f) * 0x1p-24f;                // multiples of 2^-24
+    return __uint_as_float((__float_as_uint(s) + 0xFFFFFu) & ~0xFFFFFu);  // 3 bits behind the leading one
   }
-  const uint32_t s = (__float_as_uint(__fdiv_rn(a, 448.f)) + 0x7FFFFFu) & ~0x7FFFFFu;  // the next power of two
-  return fmaxf(__uint_as_float(s), 3.0517578125e-05f);
+  const uint32_t s = (__float_as_uint(a * (float)((1.0 - 0x1p-20) / 448.0)) + 0x7FFFFFu) & ~0x7FFFFFu;  // the next power of two
+  return fmaxf(__uint_as_float(s), 0x1p-15f);
 }
-// What a row's values are multiplied by to be codes, and the largest code.
+// What a row's values are multiplied by to be codes.
 template <int FMT>
 __device__ __forceinline__ float kvq_inverse(float scale) {
-  if (FMT == KVQ_INT8) return __fdiv_rn(1.f, scale);
-  return __uint_as_float(0x7F000000u - __float_as_uint(scale));  // 2^-e
+  if (FMT != KVQ_INT8) return __uint_as_float(0x7F000000u - __float_as_uint(scale));  // 2^-e
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));  // to 2^-23
+  return r;
 }
-// Four values as a word of codes.
-// int8: x times the rounded 1 / scale is off by less than 2^-16 from x / scale, which is at most 127.  A quotient that is no tie is at least
-// 2^-12 away from one (x has 11 significant bits, scale 4), so rounding to multiples of 2^-13 first makes ties of the ties and of
-// nothing else.  Adding 1536 is that rounding, adding 1.5 2^23 the one to whole numbers, and 128 more the code's bias.
+// Four values as a word of codes.  A scale beyond 512 (256) has codes whose values pass 65504: the largest that does not is 113 (240).
+// int8: the product is off by less than 2^-15 from x / scale, which is at most 127.  A quotient that is no tie is at least 2^-12 away
+// from one (x has 11 significant bits, scale 4), so rounding to multiples of 2^-13 first makes ties of the ties and of nothing
+// else.  Adding 1536 is that rounding, adding 1.5 2^23 the one to whole numbers, and 128 more the code's bias.
 template <int FMT>
 __device__ __forceinline__ uint32_t kvq_codes(const float (&x)[4], float scale, float inverse) {
   if (!(scale > 0.f)) return KVQ_ZERO<FMT>;
+  const float top = FMT == KVQ_INT8 ? (scale > 512.f ? 113.f : 127.f) : (scale < 256.f ? 448.f : 240.f);
+  float q[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) q[i] = fminf(fmaxf(__fmul_rn(x[i], inverse), -top), top);
   if (FMT == KVQ_INT8) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float q = __fmul_rn(x[i], inverse);
-      if (scale >= 512.f) {  // values may pass 65504: the next lower code
-        const float top = floorf(__fdiv_rn(65504.f, scale));
-        q = fminf(fmaxf(q, -top), top);
-      }
-      w[i] = __float_as_uint(__fadd_rn(__fadd_rn(__fadd_rn(q, 1536.f), -1536.f), 12583040.f));
-    }
+    for (int i = 0; i < 4; i++) w[i] = __float_as_uint(__fadd_rn(__fadd_rn(__fadd_rn(q[i], 1536.f), -1536.f), 12583040.f));
     return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
   }
-  const float top = scale < 256.f ? 448.f : 240.f;
-  float y[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) y[i] = fminf(fmaxf(x[i] * inverse, -top), top);
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
 

@@ -28,11 +28,13 @@ struct KvqSplitArgs {
   int ldx, ldo, R, B, H, n_rep, max_count, step, limit;  // positions from `limit` on are outside
   float scale2;                                          // log2 e / sqrt(hd)
   float* part;                                           // [2 * CTAs][columns * (hd + 2)]
-  unsigned int* tickets;                                 // [CTAs], zero between launches
+  unsigned int* tickets;                                 // [2 * CTAs], zero between launches
 };
 
 constexpr int KS_WARPS = 4, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_CTAS = 3;  // CTAs to an SM
 constexpr int KS_FIXED = 3;  // units that a (sequence, kv head) costs beside its own
+constexpr int KS_AHEAD = 3;  // tiles of a warp that are asked into L2 when it begins
+constexpr int KS_GROUP = 8;  // pieces that are added up ahead of the others, where there are many
 
 template <int HD, int NT>
 struct KsCfg {
@@ -152,11 +154,13 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
       };
       auto pages_of = [&](int i) { return i + lane < n_tiles ? bt[(t_lo + (i + lane) * KS_UNIT + warp * 16) >> a.c.page_shift] : 0; };
       int pages = pages_of(0);  // lane l: page of the warp's tile 32 i + l
+      auto row_of = [&](int i) -> size_t {  // of the pool, where tile i begins
+        const int t0 = t_lo + i * KS_UNIT + warp * 16, page = __shfl_sync(0xffffffffu, pages, i & 31);
+        return (((size_t)page * a.c.G + g) << a.c.page_shift) + (t0 & ((1 << a.c.page_shift) - 1));
+      };
       auto load = [&](int i, Tile& t) {
-        const int t0 = t_lo + i * KS_UNIT + warp * 16;
         if (i > 0 && (i & 31) == 0) pages = pages_of(i);
-        const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-        const size_t row = (((size_t)page * a.c.G + g) << a.c.page_shift) + (t0 & ((1 << a.c.page_shift) - 1));
+        const size_t row = row_of(i);
         const uint8_t* k = a.c.k + (row + r) * HD + c * 16;
         const uint8_t* v = a.c.v + (row + 2 * c) * HD + r * VB;
         const __half2* s = a.c.scales + row;
@@ -183,6 +187,10 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
       // ---- fragments of q^T: the lane's column is nt * 8 + r.  Everything is asked for before anything is waited for.
       uint32_t qf[NT][KJ * 4][2];
       Tile tile;
+      // The new token is an entry of its own when the warps' sums meet, made by the CTA with the end of its sequence and stored on the way.  Its
+      // last warp has a tile less than the others at most times.
+      const bool entry = stored && j1 == n_units, fresh = NEW && entry && warp == KS_WARPS - 1;
+      uint4 kx, vx, kt;
       {
         uint4 x[NT][KJ][2], turn[KJ][2];
         bool have[NT];
@@ -203,7 +211,17 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
             turn[j][0] = ld_128(from);
             turn[j][1] = ld_128(from + 8);
           }
+        if (fresh) {
+          const __half* k = a.x + (size_t)b * a.ldx + (size_t)(a.H + g) * HD + lane % (HD / 8) * 8;
+          kx = ld_128(k);
+          vx = ld_128(k + (size_t)a.c.G * HD);
+          if (a.table) kt = ld_128(a.table + (size_t)p0 * HD + lane % (HD / 8) * 8);
+        }
         if (n_tiles > 0) load(0, tile);
+        // the next tiles on their way into L2, a line to a lane: at the start nothing else keeps HBM busy
+#pragma unroll
+        for (int i = 1; i <= KS_AHEAD; i++)
+          if (i < n_tiles) prefetch_l2((lane < 16 ? a.c.k : a.c.v) + (row_of(i) + (lane & 15)) * HD);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -215,14 +233,11 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
             qf[nt][j * 4 + 2][0] = hi.x; qf[nt][j * 4 + 2][1] = hi.y; qf[nt][j * 4 + 3][0] = hi.z; qf[nt][j * 4 + 3][1] = hi.w;
           }
       }
-      // ---- the new token, by the CTA with the end of its sequence: stored, and an entry of its own when the warps' sums meet
-      const bool entry = stored && j1 == n_units;
-      if (NEW && entry && warp == 0) {
+      // ---- the new token
+      if (fresh) {
         constexpr int LPR = HD / 8;
         const int sub = lane % LPR;
-        const __half* k = a.x + (size_t)b * a.ldx + (size_t)(a.H + g) * HD + sub * 8;
-        uint4 kx = ld_128(k), vx = ld_128(k + (size_t)a.c.G * HD);
-        if (a.table) kx = kvq_rotate(kx, ld_128(a.table + (size_t)p0 * HD + sub * 8));
+        if (a.table) kx = kvq_rotate(kx, kt);
         uint2 kc, vc;
         __half2 scale;
         kvq_quantise<FMT, LPR>(kx, vx, kc, vc, scale);
@@ -406,50 +421,74 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         }
       }
       if (whole) { __syncthreads(); continue; }
-      // ---- pieces of a (sequence, kv head) that CTAs c_lo .. c_hi share: the last to arrive adds them up in this order
+      // ---- pieces of a (sequence, kv head) that CTAs c_lo .. c_hi share: the last to arrive adds them up in this order.  Many are added up in
+      // groups of neighbours first, as these are done: one CTA reads 30 pieces in 10 us.
       const long long begin = item + KS_FIXED, last = begin + n_units - 1;
       const int c_lo = (int)(((begin + 1) * ctas - 1) / total), c_hi = (int)(((last + 1) * ctas - 1) / total), pieces = c_hi - c_lo + 1;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) s_ticket = atomicAdd(&a.tickets[c_lo], 1u);
-      __syncthreads();
-      if (s_ticket != (unsigned)(pieces - 1)) continue;
-      __threadfence();
-      if (tid == 0) a.tickets[c_lo] = 0;
-      auto piece = [&](int p) -> const float* { return a.part + (size_t)(2 * (c_lo + p) + (p == 0 ? 1 : 0)) * Cfg::PART; };
+      auto arrive = [&](unsigned int* ticket, int of) -> bool {  // whether this CTA is the last
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();
+          s_ticket = atomicAdd(ticket, 1u);
+          if (s_ticket == (unsigned)(of - 1)) *ticket = 0;
+          __threadfence();
+        }
+        __syncthreads();
+        return s_ticket == (unsigned)(of - 1);
+      };
+      auto piece = [&](int p) -> float* { return a.part + (size_t)(2 * (c_lo + p) + (p == 0 ? 1 : 0)) * Cfg::PART; };
       constexpr int NI = COLS * HD / (KS_THREADS * 4), BATCH = NI > 2 ? 2 : NI > 1 ? 4 : 8;  // groups of four values of a thread; pieces whose loads are in flight together
       float x[NI][4], top[NI], sum[NI];
+      auto add_up = [&](int from, int to, int step) {
 #pragma unroll
-      for (int e = 0; e < NI; e++) { x[e][0] = x[e][1] = x[e][2] = x[e][3] = sum[e] = 0.f; top[e] = -INFINITY; }
+        for (int e = 0; e < NI; e++) { x[e][0] = x[e][1] = x[e][2] = x[e][3] = sum[e] = 0.f; top[e] = -INFINITY; }
 #pragma unroll 1
-      for (int p = 0; p < pieces; p += BATCH) {
-        float4 y[BATCH][NI];
-        float pm[BATCH][NI], pl[BATCH][NI];
+        for (int p = from; p < to; p += BATCH * step) {
+          float4 y[BATCH][NI];
+          float pm[BATCH][NI], pl[BATCH][NI];
 #pragma unroll
-        for (int k = 0; k < BATCH; k++) {
-          const float* from = piece(min(p + k, pieces - 1));
+          for (int k = 0; k < BATCH; k++) {
+            const float* src = piece(p + k * step < to ? p + k * step : from);
 #pragma unroll
-          for (int e = 0; e < NI; e++) {
-            const int idx = (tid + e * KS_THREADS) * 4;
-            y[k][e] = __ldcg(reinterpret_cast<const float4*>(from + idx));
-            pm[k][e] = __ldcg(from + COLS * HD + idx / HD);
-            pl[k][e] = __ldcg(from + COLS * HD + COLS + idx / HD);
+            for (int e = 0; e < NI; e++) {
+              const int idx = (tid + e * KS_THREADS) * 4;
+              y[k][e] = __ldcg(reinterpret_cast<const float4*>(src + idx));
+              pm[k][e] = __ldcg(src + COLS * HD + idx / HD);
+              pl[k][e] = __ldcg(src + COLS * HD + COLS + idx / HD);
+            }
           }
+#pragma unroll
+          for (int k = 0; k < BATCH; k++)
+#pragma unroll
+            for (int e = 0; e < NI; e++) {
+              if (p + k * step >= to) continue;
+              const float then = fmaxf(top[e], pm[k][e]), base = then == -INFINITY ? 0.f : then, fade = ks_ex2(top[e] - base), f = ks_ex2(pm[k][e] - base);
+              top[e] = then;
+              sum[e] = sum[e] * fade + pl[k][e] * f;
+              x[e][0] = x[e][0] * fade + y[k][e].x * f;
+              x[e][1] = x[e][1] * fade + y[k][e].y * f;
+              x[e][2] = x[e][2] * fade + y[k][e].z * f;
+              x[e][3] = x[e][3] * fade + y[k][e].w * f;
+            }
         }
+      };
+      int step = 1;
+      if (pieces > KS_GROUP + KS_GROUP / 2) {
+        step = KS_GROUP;
+        const int from = ((int)blockIdx.x - c_lo) / KS_GROUP * KS_GROUP, to = min(from + KS_GROUP, pieces);
+        if (!arrive(&a.tickets[c_lo + from], to - from)) continue;
+        add_up(from, to, 1);
+        __syncthreads();  // all have read what is written over now
+        float* dst = piece(from);
 #pragma unroll
-        for (int k = 0; k < BATCH; k++)
-#pragma unroll
-          for (int e = 0; e < NI; e++) {
-            if (p + k >= pieces) continue;
-            const float then = fmaxf(top[e], pm[k][e]), base = then == -INFINITY ? 0.f : then, fade = ks_ex2(top[e] - base), f = ks_ex2(pm[k][e] - base);
-            top[e] = then;
-            sum[e] = sum[e] * fade + pl[k][e] * f;
-            x[e][0] = x[e][0] * fade + y[k][e].x * f;
-            x[e][1] = x[e][1] * fade + y[k][e].y * f;
-            x[e][2] = x[e][2] * fade + y[k][e].z * f;
-            x[e][3] = x[e][3] * fade + y[k][e].w * f;
-          }
+        for (int e = 0; e < NI; e++) {
+          const int idx = (tid + e * KS_THREADS) * 4;
+          __stcg(reinterpret_cast<float4*>(dst + idx), make_float4(x[e][0], x[e][1], x[e][2], x[e][3]));
+          if (idx % HD == 0) { __stcg(dst + COLS * HD + idx / HD, top[e]); __stcg(dst + COLS * HD + COLS + idx / HD, sum[e]); }
+        }
       }
+      if (!arrive(&a.tickets[gridDim.x + c_lo], (pieces + step - 1) / step)) continue;
+      add_up(0, pieces, step);
 #pragma unroll
       for (int e = 0; e < NI; e++) {
         const float inv = sum[e] == 0.f ? 0.f : __fdiv_rn(1.f, sum[e]);
@@ -462,7 +501,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
   }
 }
 
-static inline int ks_ctas(const jg_dev* dev) { return KS_CTAS * dev->sm_count; }  // that a device runs at once; as many tickets: jg_kvq_ticket_bytes
+static inline int ks_ctas(const jg_dev* dev) { return KS_CTAS * dev->sm_count; }  // that a device runs at once; twice as many tickets: jg_kvq_ticket_bytes
 static inline int ks_slots(const jg_dev* dev) { return 2 * ks_ctas(dev); }  // pieces in the workspace
 static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 2>::PART : KsCfg<128, 2>::PART; }
 
