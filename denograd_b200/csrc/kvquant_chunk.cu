@@ -411,19 +411,19 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       // Positions past the end are the last one, masked.
       auto page_of = [&](int j) { return bt[min(j * KC_KEYS + (lane & 7) * 16, last) >> a.c.page_shift]; };
       auto first_row = [&](int j, int page) { return ((uint32_t)(page * a.c.G + p.g) << a.c.page_shift) + (uint32_t)(min(j * KC_KEYS + (lane & 7) * 16, last) & mask); };
+      // A piece of a row is asked for as soon as the one of the tile before it is done with, so that all have a tile's time to come.
       uint4 x[N];
-      float s = 0.f;  // lane l: the scale of row (l / PER) * ROWS + l % PER of the warp's rows
-      auto load = [&](int j, int page) {
-        const uint32_t begin = first_row(j, page);
-        const int room = last - j * KC_KEYS;  // rows of the tile up to the last position
-        auto row_at = [&](int r) {  // row of the pool of the tile's row r
-          const uint32_t b0 = __shfl_sync(0xffffffffu, begin, r >> 4);
-          return b0 + (uint32_t)(room >= KC_KEYS - 1 ? r & 15 : max(0, min(r & 15, room - (r & ~15))));
-        };
-        s = __half2float(scales[2 * (size_t)row_at((lane / PER % N) * ROWS + (warp & 3) * PER + lane % PER)]);
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = ld_stream_128(codes + (size_t)row_at(row + i * ROWS) * HD);
+      uint32_t begin = 0;  // of the tile whose rows are asked for: first_row
+      int room = 0;        // its rows up to the last position
+      auto row_at = [&](int r) {  // row of the pool of the tile's row r
+        const uint32_t b0 = __shfl_sync(0xffffffffu, begin, r >> 4);
+        return b0 + (uint32_t)(room >= KC_KEYS - 1 ? r & 15 : max(0, min(r & 15, room - (r & ~15))));
       };
+      auto tile_at = [&](int j, int page) { begin = first_row(j, page); room = last - j * KC_KEYS; };
+      auto scale_at = [&]() {  // lane l: the scale of row (l / PER) * ROWS + l % PER of the warp's rows
+        return __half2float(scales[2 * (size_t)row_at((lane / PER % N) * ROWS + (warp & 3) * PER + lane % PER)]);
+      };
+      auto codes_at = [&](int i) { return ld_stream_128(codes + (size_t)row_at(row + i * ROWS) * HD); };
       // the rows of a tile on their way into L2, one to a thread, where a tile of few rows is done before another comes from HBM
       const bool hurry = kc_split_item(a, p);
       auto ahead = [&](int j, int page) {
@@ -434,7 +434,10 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         if ((r & 15) == 0) prefetch_l2(scales + 2 * at);
       };
       int page = page_of(p.j0), page2 = page_of(p.j0 + 1);
-      load(p.j0, page);
+      tile_at(p.j0, page);
+      float s = scale_at();
+#pragma unroll
+      for (int i = 0; i < N; i++) x[i] = codes_at(i);
       page = page2;
       page2 = page_of(p.j0 + 2);
       if (hurry && p.j0 + 1 < p.j1) ahead(p.j0 + 1, page);
@@ -444,19 +447,25 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         if (tiles >= 2) ok = mbar_wait(&empty[slot], ((tiles >> 1) - 1) & 1);
         if (!ok) break;
         unsigned char* to = tile + (size_t)slot * Cfg::KV_BYTES;
-        const bool small = FMT == KVQ_INT8 && __all_sync(0xffffffffu, !(s > 56.f));
+        const bool small = FMT == KVQ_INT8 && __all_sync(0xffffffffu, !(s > 56.f)), more = j + 1 < p.j1;
+        float then = 0.f;
+        if (more) {
+          tile_at(j + 1, page);
+          then = scale_at();
+        }
 #pragma unroll
         for (int i = 0; i < N; i++) {
           const __half2 sc = __float2half2_rn(__shfl_sync(0xffffffffu, s, i * PER + (row & (PER - 1))));
           __half2 h[8];
           kc_widen<FMT>(x[i], sc, __hmul2_rn(sc, __floats2half2_rn(-1152.f, -1152.f)), small, h);
+          if (more) x[i] = codes_at(i);
           *reinterpret_cast<uint4*>(to + i * ROWS * 128 + o0) = *reinterpret_cast<const uint4*>(h);
           *reinterpret_cast<uint4*>(to + i * ROWS * 128 + o1) = *reinterpret_cast<const uint4*>(h + 4);
         }
+        s = then;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) ft_arrive(&full[slot]);
-        if (j + 1 < p.j1) load(j + 1, page);
         page = page2;
         page2 = page_of(j + 3);
       }

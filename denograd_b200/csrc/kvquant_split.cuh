@@ -515,7 +515,8 @@ static int launch_split(jg_dev* dev, const KvqSplitArgs& a) {
     JG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     attr_set[dev->ordinal & 7] = true;
   }
+  const int ctas = NT == 1 ? ks_ctas(dev) : 2 * dev->sm_count;  // that run at once
   const long long most = (long long)a.B * a.c.G * ((a.c.max_ctx + KS_UNIT - 1) / KS_UNIT);
-  return jg_launch(dev, NEW ? "kvq_decode" : "kvq_attn", kern, dim3((unsigned)(most < ks_ctas(dev) ? most : ks_ctas(dev))), dim3(KS_THREADS), smem, a);
+  return jg_launch(dev, NEW ? "kvq_decode" : "kvq_attn", kern, dim3((unsigned)(most < ctas ? most : ctas)), dim3(KS_THREADS), smem, a);
 }
 #endif
