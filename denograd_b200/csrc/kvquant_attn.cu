@@ -42,7 +42,9 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
-  if ((long long)max_count * (H / G) <= 16) {
+  // Up to 24 columns are read at HBM's pace or near it: 8 sequences of 5 positions behind 3001, 20 columns, 31 us (the tensor cores' form 38),
+  // 16 columns 22 us (38), 32 sequences 84 us (93).  Beyond that a lane's outputs do not fit its registers.
+  if ((long long)max_count * (H / G) <= 24) {
     KvqSplitArgs s = {};
     s.c = kvq_layer(kv, layer);
     s.x = (const __half*)q; s.out = (__half*)out;
@@ -51,12 +53,14 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
     s.limit = kv->max_ctx;
     s.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
     s.part = dev->kvq_part; s.tickets = dev->kvq_tickets;
-    const bool few = max_count * (H / G) <= 8;
-    if (kv->format == JG_KVQ_INT8)
-      return hd == 64 ? (few ? launch_split<KVQ_INT8, 64, 1, false>(dev, s) : launch_split<KVQ_INT8, 64, 2, false>(dev, s))
-                      : (few ? launch_split<KVQ_INT8, 128, 1, false>(dev, s) : launch_split<KVQ_INT8, 128, 2, false>(dev, s));
-    return hd == 64 ? (few ? launch_split<KVQ_E4M3, 64, 1, false>(dev, s) : launch_split<KVQ_E4M3, 64, 2, false>(dev, s))
-                    : (few ? launch_split<KVQ_E4M3, 128, 1, false>(dev, s) : launch_split<KVQ_E4M3, 128, 2, false>(dev, s));
+    const int columns = max_count * (H / G);
+#define KS_CASE(FMT_, FORMAT_, HD_)                                                      \
+  if (kv->format == FORMAT_ && hd == HD_)                                                \
+    return columns <= 8    ? launch_split<FMT_, HD_, 1, false>(dev, s)                   \
+           : columns <= 16 ? launch_split<FMT_, HD_, 2, false>(dev, s)                   \
+                           : launch_split<FMT_, HD_, 3, false>(dev, s);
+    KS_CASE(KVQ_INT8, JG_KVQ_INT8, 64) KS_CASE(KVQ_INT8, JG_KVQ_INT8, 128) KS_CASE(KVQ_E4M3, JG_KVQ_E4M3, 64) KS_CASE(KVQ_E4M3, JG_KVQ_E4M3, 128)
+#undef KS_CASE
   }
   KvqChunkArgs a = {};
   a.c = kvq_layer(kv, layer);

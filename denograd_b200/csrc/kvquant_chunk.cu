@@ -39,23 +39,27 @@ struct KcCfg {
 // A piece of work: the key tiles [j0, j1) of an item.
 struct KcPiece {
   const int32_t* bt;       // null: the slot lies outside the cache
-  int b, tile, g, j0, j1;  // b < 0: no more pieces
+  int b, g, j0, j1;        // b < 0: no more pieces
+  int row0;                // the item's first row of the sequence's
+  int left;                // its rows; up to 128: its key tiles take turns between the two streams
   int n_tiles;             // of the whole item
   int p0, n, T;            // first new position and number of new positions of the sequence; keys that the item looks at
   int c_lo, pieces;        // the CTAs that share the item
 };
 
 // What a sequence is, and how many key tiles item `tile` of it has (0: no such item).
-__device__ __forceinline__ int kc_item(const KvqChunkArgs& a, int b, int tile, KcPiece& p) {
+__device__ __forceinline__ int kc_item(const KvqChunkArgs& a, int b, int tile, int rows, KcPiece& p) {
+  p.row0 = tile * rows;
   const int sq = a.seq ? a.seq[b] : b, count = a.count ? a.count[b] : a.max_count;
   p.p0 = a.pos[b];
   p.n = max(0, min(count, a.max_count));
   const int first = a.first ? a.first[b] : b;
   if ((long long)first + (long long)(p.n - 1) * a.step >= a.R) p.n = first < a.R ? (int)(((long long)a.R - 1 - first) / a.step) + 1 : 0;  // rows there are
-  if ((long long)tile * KC_ROWS >= (long long)p.n * a.n_rep) return 0;
+  if ((long long)tile * rows >= (long long)p.n * a.n_rep) return 0;
+  p.left = min(rows, p.n * a.n_rep - p.row0);
   const bool have = (unsigned)sq < (unsigned)a.c.n_seq;
   p.bt = have ? a.c.block_table + (size_t)sq * a.c.max_pages : nullptr;
-  const int last = min(p.n, ((tile + 1) * KC_ROWS - 1) / a.n_rep + 1);  // positions up to the item's end
+  const int last = min(p.n, ((tile + 1) * rows - 1) / a.n_rep + 1);  // positions up to the item's end
   p.T = have ? (int)max(0ll, min((long long)p.p0 + last, (long long)a.c.max_ctx)) : 0;
   return max(1, (p.T + KC_KEYS - 1) / KC_KEYS);
 }
@@ -128,9 +132,6 @@ __device__ __forceinline__ void kc_widen(const uint4& x, __half2 s, __half2 bias
   }
 }
 
-// Whether an item has up to 128 rows: then its key tiles take turns between the two streams.
-__device__ __forceinline__ bool kc_split_item(const KvqChunkArgs& a, const KcPiece& p) { return p.n * a.n_rep - p.tile * KC_ROWS <= 128; }
-
 template <int FMT, int HD>
 __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunkArgs a) {
   constexpr int KB = HD / 64;                     // 64-column blocks of a tile's rows
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   const int entries = a.B * a.max_tiles;
   auto tiles_of = [&](int e) -> int {
     KcPiece p;
-    return e < entries ? kc_item(a, e / a.max_tiles, e % a.max_tiles, p) : 0;
+    return e < entries ? kc_item(a, e / a.max_tiles, e % a.max_tiles, KC_ROWS, p) : 0;
   };
   auto cost = [&](int n) { return n > 0 ? (long long)(n + KC_FIXED) * a.c.G : 0ll; };
   auto warp_sum64 = [&](long long v) {
@@ -250,22 +251,34 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     if (warp == 17) {
       // ---- the plan: a walk along this CTA's stretch of the line
       long long at;  // first tile of (b, tile, head 0)
-      int entry;
+      int entry, rows = KC_ROWS, per = a.max_tiles;  // of an item; items of a sequence
+      bool single = false;
       if (entries > 32) {
         at = s_at;
         entry = s_entry;
       } else {
-        longest = tiles_of(lane);
-        const long long mine = cost(longest), sum = scan64(mine);
+        int n = tiles_of(lane);
+        longest = __reduce_max_sync(0xffffffffu, n);
+        int items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
+        // Short items that leave half of the CTAs idle become items of half the rows, whose two streams share their keys (512 new positions of the
+        // 8B 16.6 us, 18.7 without); and where each CTA has one at most, they count alike (18.7 us, 19.3 without).
+        if (longest <= KC_WHOLE && entries <= 16 && 2 * items <= (int)gridDim.x) {
+          rows = KC_ROWS / 2;
+          per *= 2;
+          KcPiece p;
+          n = lane < a.B * per ? kc_item(a, lane / per, lane % per, rows, p) : 0;
+          items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
+        }
+        single = longest <= KC_WHOLE && items <= (int)gridDim.x;
+        const long long mine = single ? (n > 0 ? a.c.G : 0) : cost(n), sum = scan64(mine);
         total = __shfl_sync(0xffffffffu, sum, 31);
-        longest = __reduce_max_sync(0xffffffffu, longest);
         share();
         entry = max(0, __ffs(__ballot_sync(0xffffffffu, sum > u_lo)) - 1);
         at = __shfl_sync(0xffffffffu, sum - mine, entry);
       }
       const bool cut = longest > KC_WHOLE;
       long long u = u_lo;
-      int b = entry / a.max_tiles, tile = entry % a.max_tiles;
+      int b = entry / per, tile = entry % per;
       for (;; planned++) {
         const uint32_t slot = planned % KC_PLAN;
         if (planned >= KC_PLAN) ok = mbar_wait(&plan_empty[slot], (planned / KC_PLAN - 1) & 1);
@@ -273,12 +286,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         KcPiece p;
         p.b = -1;
         while (u < u_hi) {
-          const int n = kc_item(a, b, tile, p);
+          const int n = kc_item(a, b, tile, rows, p);
           if (n == 0) { tile = 0; b++; continue; }  // the items of a sequence are its first ones
-          const int span = n + KC_FIXED;  // of an item on the line; its tiles are behind its fixed cost
+          const int span = single ? 1 : n + KC_FIXED;  // of an item on the line; its tiles are behind its fixed cost
           if (u >= at + (long long)span * a.c.G) {
             at += (long long)span * a.c.G;
-            if (++tile == a.max_tiles) { tile = 0; b++; }
+            if (++tile == per) { tile = 0; b++; }
             continue;
           }
           p.g = (int)(u - at) / span;  // both below 2^31: see the limits of the cache
@@ -295,7 +308,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
             p.j1 = max(0, (int)(u - item) - KC_FIXED);
             if (p.j0 == p.j1) continue;
           }
-          p.b = b; p.tile = tile; p.n_tiles = n;
+          p.b = b; p.n_tiles = n;
           p.c_lo = p.pieces = 0;
           if (p.j1 - p.j0 < n) {
             const long long begin = item + KC_FIXED;
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       KcPiece p;
       while (next(p)) {
         const int n = p.j1 - p.j0;
-        if (kc_split_item(a, p)) {
+        if (p.left <= 128) {
           wait(&q_full[0], loaded[0]++ & 1);
           auto scores = [&](int j) {  // of tile j, for the stream whose turn it is
             const uint32_t slot = (tiles + j) & 1;
@@ -425,7 +438,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       };
       auto codes_at = [&](int i) { return ld_stream_128(codes + (size_t)row_at(row + i * ROWS) * HD); };
       // the rows of a tile on their way into L2, one to a thread, where a tile of few rows is done before another comes from HBM
-      const bool hurry = kc_split_item(a, p);
+      const bool hurry = p.left <= 128;
       auto ahead = [&](int j, int page) {
         const uint32_t begin = first_row(j, page);
         const int r = u;
@@ -485,9 +498,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       ok = mbar_wait(&met, meetings++ & 1) && ok;
     };
     // What this thread's row is, worked out from the plan where it is needed: the loop over tiles has no registers to keep it in.
-    auto mine_of = [&](const KcPiece& p) { return kc_split_item(a, p) ? r : q * 128 + r; };  // of the item's rows
+    auto mine_of = [&](const KcPiece& p) { return p.left <= 128 ? r : q * 128 + r; };  // of the item's rows
     auto row_of = [&](const KcPiece& p, int& head, int& i) -> long long {  // row of queries and results, or -1
-      const int at = p.tile * KC_ROWS + mine_of(p);
+      const int at = p.row0 + mine_of(p);
       i = at / a.n_rep;
       head = p.g * a.n_rep + at - i * a.n_rep;
       const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step;
@@ -503,7 +516,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         __syncwarp();
         if (lane == 0) ft_arrive(&plan_empty[planned_slot]);
       };
-      const bool split = kc_split_item(a, p), idle = p.n * a.n_rep - p.tile * KC_ROWS <= mine_of(p) - lane;  // this warp has no rows
+      const bool split = p.left <= 128, idle = p.left <= mine_of(p) - lane;  // this warp has no rows
       const int n = split ? (p.j1 - p.j0 + 1 - q) / 2 : p.j1 - p.j0;  // tiles of this stream
       int lim;  // last key that the row sees
       float m = -INFINITY;

@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
 
 static inline int ks_ctas(const jg_dev* dev) { return KS_CTAS * dev->sm_count; }  // that a device runs at once; twice as many tickets: jg_kvq_ticket_bytes
 static inline int ks_slots(const jg_dev* dev) { return 2 * ks_ctas(dev); }  // pieces in the workspace
-static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 2>::PART : KsCfg<128, 2>::PART; }
+static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 3>::PART : KsCfg<128, 3>::PART; }
 
 template <int FMT, int HD, int NT, bool NEW>
 static int launch_split(jg_dev* dev, const KvqSplitArgs& a) {

@@ -274,6 +274,28 @@ def test_attend_long_and_many(dev, H, G, hd, ahead, new, fmt):
     c.close()
 
 
+# Queries of a kv head on either side of 8, 16 and 24, where the kernel for few of them takes more columns, and beyond it; long caches, so that
+# (sequence, kv head)s are shared
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("H,G,hd,new", [(8, 1, 128, [2]), (8, 1, 128, [3, 3]), (8, 1, 64, [3]), (8, 1, 128, [4]), (12, 4, 64, [8, 7, 8]), (12, 4, 128, [6, 8]), (12, 4, 128, [9, 8]),
+                                        (2, 2, 64, [24]), (2, 2, 128, [25, 17]), (2, 1, 128, [9, 12])])
+def test_attend_few_queries(dev, H, G, hd, new, fmt):
+    ahead = [2907, 66, 0][:len(new)]
+    c = Cache(dev, H, G, hd, fmt, 32, max(a + n for a, n in zip(ahead, new)), len(new) + 1, np.random.default_rng(21))
+    attend(c, ahead, new, False, seed=13)
+    c.close()
+
+
+# Prompts that the tensor cores' form cuts into items of 128 rows where they leave half of the SMs idle, and into 256 where they do not: sequences and
+# rows on either side of the choice
+@pytest.mark.parametrize("H,G,hd,new,ahead", [(32, 8, 128, [300], 0), (32, 8, 64, [576], 0), (32, 8, 128, [577], 100), (32, 8, 64, [640], 0), (8, 1, 64, [129], 900), (4, 1, 64, [33] * 16, 0),
+                                              (4, 1, 64, [33] * 17, 0), (4, 4, 128, [128, 129, 256, 257], 40), (8, 1, 128, [700, 40], 200), (16, 8, 64, [64, 0, 65, 1, 200], 700)])
+def test_attend_prompts(dev, H, G, hd, new, ahead):
+    c = Cache(dev, H, G, hd, "int8", 64, ahead + max(new), len(new) + 1, np.random.default_rng(22))
+    attend(c, [ahead] * len(new), new, False, seed=14)
+    c.close()
+
+
 @pytest.mark.parametrize("most", [3, 40])  # short chunks and long ones have kernels of their own
 def test_attend_rows_outside(dev, most):
     rng = np.random.default_rng(10)
