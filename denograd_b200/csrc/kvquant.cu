@@ -3,6 +3,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <new>
 
 #include "kvquant_chunk.cuh"
 #include "kvquant_split.cuh"
@@ -43,8 +44,8 @@ JG_API int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t forma
   JG_REQUIRE(!dev->capturing, "kvq_create: a graph capture is in progress");
   const int rc = kvq_workspace(dev);
   if (rc) return rc;
-  jg_kvq* kv = new jg_kvq();
-  memset(kv, 0, sizeof(*kv));
+  jg_kvq* kv = new (std::nothrow) jg_kvq();
+  JG_REQUIRE(kv != nullptr, "kvq_create: out of memory");
   kv->dev = dev;
   kv->d = d;
   kv->format = format;

@@ -344,7 +344,14 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
           w[nt][1] = ks_transpose(ks_half2(__floats2half2_rn(e2, e3)));
         }
         // outputs
-        const uint32_t p0_ = __byte_perm(t.sv0.x, t.sv0.y, 0x7632), p1_ = __byte_perm(t.sv1.x, t.sv1.y, 0x7632);
+        uint32_t p0_ = __byte_perm(t.sv0.x, t.sv0.y, 0x7632), p1_ = __byte_perm(t.sv1.x, t.sv1.y, 0x7632);
+        if (NEW && t0 + 16 > T) {
+          // The row behind the last is being written by another warp: new codes times the scale that was there could be an infinity, and that
+          // times a weight of 0 a NaN.
+          const int left = T - t0 - 2 * c;
+          p0_ &= (left > 0 ? 0xFFFFu : 0u) | (left > 1 ? 0xFFFF0000u : 0u);
+          p1_ &= (left > 8 ? 0xFFFFu : 0u) | (left > 9 ? 0xFFFF0000u : 0u);
+        }
         const __half2 scale0 = *reinterpret_cast<const __half2*>(&p0_), scale1 = *reinterpret_cast<const __half2*>(&p1_);
 #pragma unroll
         for (int e = 0; e < VB / 4; e++)

@@ -2,7 +2,7 @@
 rows, attend to the cache and read it back (jg_kvq_* in include/jsgrad_cuda.h).
 
 The reference keeps K and V in the model's 16-bit type (Attention.cache_kv, jsgrad/models/llama.ts:78-90); ``KVCache`` in llama.py is
-that cache, ``QuantKVCache`` takes 0.51 of its memory (and of what a decode step reads) for an error of K and V of about 0.6 %
+that cache, ``QuantKVCache`` takes 0.51 of its memory (and of what a decode step reads) for an error of K and V of about 0.7 %
 ("int8") or 2.6 % ("fp8") of a normally distributed row.  ``Llama3(kv_dtype="int8")`` puts it under a model.
 
 Rows are fp16 tensors [rows, columns] whose first columns are used: wq|wk|wv outputs [(H + 2G) * hd], queries and results [H * hd],
@@ -21,11 +21,13 @@ from .device import CUDA, Tensor
 FORMATS = {"int8": ffi.KVQ_INT8, "fp8": ffi.KVQ_E4M3}
 
 
-def _ints(name: str, t: Tensor | None, n: int) -> int:
+def _ints(dev: CUDA, name: str, t: Tensor | None, n: int) -> int:
     """Its address, or 0 where it is not given."""
     if t is None:
         return 0
     buf = t.buf
+    if buf.dev is not dev:
+        raise ValueError(f"{name} lies on {buf.dev.device}, the cache on {dev.device}")
     if buf.dtype != "int32":
         raise TypeError(f"{name} is {buf.dtype}, not int32")
     if buf.size < n:
@@ -33,9 +35,11 @@ def _ints(name: str, t: Tensor | None, n: int) -> int:
     return buf.ptr
 
 
-def _rows(name: str, t: Tensor, columns: int, rows: int = 0) -> tuple[int, int, int]:
+def _rows(dev: CUDA, name: str, t: Tensor, columns: int, rows: int = 0) -> tuple[int, int, int]:
     """(address, row stride, rows) of a tensor of fp16 rows."""
     buf, ld = t.buf, t.shape[-1]
+    if buf.dev is not dev:
+        raise ValueError(f"{name} lies on {buf.dev.device}, the cache on {dev.device}")
     if buf.dtype != "float16":
         raise TypeError(f"{name} is {buf.dtype}, not float16")
     if ld < columns:
@@ -80,33 +84,34 @@ class QuantKVCache:
               q_out: Tensor | None = None) -> None:
         """Rotates Q and K of every row of `qkv` (by `freqs_cis`, or not at all) and stores K and V: row r is position pos[r] of slot
         seq[r] (None: slot r).  Rotated Q goes to `q_out`, which may be `qkv`.  The rows name different positions."""
-        x, ldx, R = _rows("qkv", qkv, self._qkv)
-        to, ldq, _ = _rows("q_out", q_out, self._q, R) if q_out is not None else (0, 0, 0)
+        x, ldx, R = _rows(self.dev, "qkv", qkv, self._qkv)
+        to, ldq, _ = _rows(self.dev, "q_out", q_out, self._q, R) if q_out is not None else (0, 0, 0)
         table, n = self._table(freqs_cis)
-        self.dev.call("jg_kvq_write", self.handle, layer, to, ldq, x, ldx, table, n, _ints("pos", pos, R), _ints("seq", seq, R), R, self.n_heads)
+        self.dev.call("jg_kvq_write", self.handle, layer, to, ldq, x, ldx, table, n, _ints(self.dev, "pos", pos, R), _ints(self.dev, "seq", seq, R), R, self.n_heads)
 
     def decode(self, layer: int, qkv: Tensor, pos: Tensor, freqs_cis: Tensor | None = None, seq: Tensor | None = None,
                out: Tensor | None = None) -> Tensor:
         """One new token for each row of `qkv`, rows in different slots: stores it as `write` does and attends to positions 0 .. pos[b].
         `qkv` is left as it is.  A row whose position lies outside the cache gets zeros."""
-        x, ldx, B = _rows("qkv", qkv, self._qkv)
+        x, ldx, B = _rows(self.dev, "qkv", qkv, self._qkv)
         if out is None:
             out = Tensor.empty((B, self._q), "float16", self.dev)
-        to, ldo, _ = _rows("out", out, self._q, B)
+        to, ldo, _ = _rows(self.dev, "out", out, self._q, B)
         table, n = self._table(freqs_cis)
-        self.dev.call("jg_kvq_decode", self.handle, layer, to, ldo, x, ldx, table, n, _ints("pos", pos, B), _ints("seq", seq, B), B, self.n_heads)
+        self.dev.call("jg_kvq_decode", self.handle, layer, to, ldo, x, ldx, table, n, _ints(self.dev, "pos", pos, B), _ints(self.dev, "seq", seq, B), B, self.n_heads)
         return out
 
     def attend(self, layer: int, q: Tensor, pos: Tensor, count: Tensor | None = None, first: Tensor | None = None,
                seq: Tensor | None = None, max_count: int | None = None, step: int | None = None, out: Tensor | None = None) -> Tensor:
         """Attention of a chunk of new positions of each of len(pos) sequences, whose K and V `write` has stored: position pos[b] + i, i <
         count[b], is row first[b] + i * step of `q` (rotated) and of `out`, and sees positions 0 .. pos[b] + i of slot seq[b].
-        Defaults: max_count positions each (all rows, dealt evenly), in position-major order (row i * B + b).  A ragged batch has
-        running sums in `first`, step=1, and the largest count as `max_count`.  Rows that no sequence names stay as they are (zeros where `out` is not given)."""
-        x, ldq, R = _rows("q", q, self._q)
+        Defaults: max_count positions each (all rows, dealt evenly), in position-major order (row i * B + b).  A ragged batch
+        has running sums in `first`, step=1, and the largest count as `max_count`.  Rows that no sequence names stay as they are (zeros where
+        `out` is not given); a row whose position or slot lies outside the cache gets zeros."""
+        x, ldq, R = _rows(self.dev, "q", q, self._q)
         if out is None:
             out = Tensor.zeros((R, self._q), "float16", self.dev)
-        to, ldo, _ = _rows("out", out, self._q, R)
+        to, ldo, _ = _rows(self.dev, "out", out, self._q, R)
         self.dev.call("jg_kvq_attn", self.handle, layer, to, ldo, x, ldq, R, *self._where(R, pos, count, first, seq, max_count, step), self.n_heads)
         return out
 
@@ -120,8 +125,8 @@ class QuantKVCache:
             if rows is None:
                 raise ValueError("give k and v, or the number of rows")
             k, v = (Tensor.zeros((rows, self._kv), "float16", self.dev) for _ in range(2))
-        to_k, ld, R = _rows("k", k, self._kv)
-        to_v, ldv, _ = _rows("v", v, self._kv, R)
+        to_k, ld, R = _rows(self.dev, "k", k, self._kv)
+        to_v, ldv, _ = _rows(self.dev, "v", v, self._kv, R)
         if ldv != ld:
             raise ValueError(f"k has rows of {ld}, v of {ldv}")
         self.dev.call("jg_kvq_read", self.handle, layer, to_k, to_v, ld, R, *self._where(R, pos, count, first, seq, max_count, step))
@@ -131,12 +136,13 @@ class QuantKVCache:
         if freqs_cis is None:
             return 0, 0
         shape = freqs_cis.shape
+        if freqs_cis.buf.dev is not self.dev:
+            raise ValueError(f"freqs_cis lies on {freqs_cis.buf.dev.device}, the cache on {self.dev.device}")
         if freqs_cis.buf.dtype != "float16" or len(shape) != 3 or shape[2] != 2 or shape[1] * 2 != self.head_dim:
             raise ValueError(f"freqs_cis is {freqs_cis.dtype} {tuple(shape)}, not float16 [positions, {self.head_dim // 2}, 2]")
         return freqs_cis.buf.ptr, shape[0]
 
-    @staticmethod
-    def _where(R: int, pos: Tensor, count, first, seq, max_count: int | None, step: int | None) -> tuple:
+    def _where(self, R: int, pos: Tensor, count, first, seq, max_count: int | None, step: int | None) -> tuple:
         """(pos, count, first, seq, sequences, max_count, step) of a call."""
         B = pos.buf.size
         if max_count is None:
@@ -145,7 +151,7 @@ class QuantKVCache:
             max_count = R // B
         if step is None:
             step = B if first is None else 1
-        return _ints("pos", pos, B), _ints("count", count, B), _ints("first", first, B), _ints("seq", seq, B), B, max_count, step
+        return _ints(self.dev, "pos", pos, B), _ints(self.dev, "count", count, B), _ints(self.dev, "first", first, B), _ints(self.dev, "seq", seq, B), B, max_count, step
 
     def close(self) -> None:
         if self.handle:

@@ -319,12 +319,12 @@ int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, int32_t
  * out: [B][H * hd]; a row whose slot or position lies outside the cache or the table gets zeros, and nothing is stored for it. */
 int jg_kvq_decode(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int32_t ldo, uint64_t qkv, int32_t ldx, uint64_t table,
                   int32_t table_rows, uint64_t pos, uint64_t seq, int32_t B, int32_t H);
-/* Chunks: sequence b, in slot seq[b] (0: slot b), has count[b] new positions (0: max_count each, which the
- * cache's context bounds; more are cut off), the first of them pos[b]; position pos[b] + i is row first[b] + i * step (first = 0: row b + i * step, so step = B is jg_attn_chunk's
- * position-major order and first = running sums with step = 1 a ragged batch).  Their K and V are in the cache already (jg_kvq_write) and
- * Q is rotated.  out[row] = attention of q[row] (the first H * hd columns) over positions [0, pos[b] + i].
- * Rows outside [0, R) are not followed; rows that no sequence names are left as they were; a position or a slot outside the cache
- * gives a row of zeros. */
+/* Chunks: sequence b, in slot seq[b] (0: slot b), has count[b] new positions (0: max_count each; more than max_count are cut off), the first of
+ * them pos[b]; position pos[b] + i is row first[b] + i * step (first = 0: row b + i * step, so step = B is jg_attn_chunk's position-major
+ * order and first = running sums with step = 1 a ragged batch).  1 <= max_count <= the cache's context, step >= 1.  Their K and V are
+ * in the cache already (jg_kvq_write) and Q is rotated.  out[row] = attention of q[row] (the first H * hd columns) over positions
+ * [0, pos[b] + i].  Rows outside [0, R) are not followed; rows that no sequence names are left as they were; a position or a slot
+ * outside the cache gives a row of zeros. */
 int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int32_t ldo, uint64_t q, int32_t ldq, int32_t R, uint64_t pos,
                 uint64_t count, uint64_t first, uint64_t seq, int32_t B, int32_t max_count, int32_t step, int32_t H);
 /* What the cache holds, as fp16 rows of G * hd: positions and rows are named as in jg_kvq_attn.  Positions and slots outside the cache read

@@ -204,6 +204,22 @@ def test_class_refuses(rec):
     assert rec.calls[-1][0] == "jg_kvq_attn" and rec.calls[-1][5:9] == (512, q.ptr, 520, 8) and rec.calls[-1][-4:] == (2, 4, 2, 8)
 
 
+def test_class_refuses_tensors_of_another_device(rec):
+    from denograd_b200.device import CUDA, Device, Tensor
+    from denograd_b200.kvquant import QuantKVCache
+    dev, other = Device["CUDA"], CUDA("CUDA:1")
+    kv = QuantKVCache(dev, 1, 8, 2, 64, 100, 3, page_size=16)
+    t = lambda where, *s: Tensor.empty(s, "float16", where)  # noqa: E731
+    i = lambda where, n: Tensor.empty((n,), "int32", where)  # noqa: E731
+    n = len(rec.calls)
+    for make in (lambda: kv.write(0, t(other, 3, 768), i(dev, 3)), lambda: kv.write(0, t(dev, 3, 768), i(other, 3)), lambda: kv.decode(0, t(dev, 3, 768), i(dev, 3), out=t(other, 3, 512)),
+                 lambda: kv.decode(0, t(dev, 3, 768), i(dev, 3), freqs_cis=t(other, 9, 32, 2)), lambda: kv.attend(0, t(dev, 6, 512), i(dev, 3), seq=i(other, 3)),
+                 lambda: kv.read(0, i(dev, 2), max_count=2, k=t(other, 4, 128), v=t(dev, 4, 128))):
+        with pytest.raises(ValueError, match="CUDA:1"):
+            make()
+    assert not [c for c in rec.calls[n:] if c[0].startswith("jg_kvq_")]
+
+
 @pytest.mark.parametrize("fused", [True, False])
 def test_a_model_uses_it(rec, fused, monkeypatch):
     from denograd_b200.llama3 import Llama3

@@ -231,11 +231,11 @@ def test_decode_rows_outside(dev):
 
 
 # ------------------------------------------------------------------------------------------------ chunks
-def attend(c, ahead, new, regular, seed, extra=3):
+def attend(c, ahead, new, regular, seed, extra=3, slots=None):
     rng = np.random.default_rng(seed)
     B = len(ahead)
-    seq = rng.permutation(B + 1)[:B]
-    held = np.zeros(B + 1, int)
+    seq = rng.permutation(slots or B + 1)[:B]
+    held = np.zeros(slots or B + 1, int)
     held[seq] = np.array(ahead) + np.array(new)
     c.fill(held)
     if regular:
@@ -418,6 +418,96 @@ def test_a_conversation(dev, fmt):
         out = c.kv.attend(0, xt, ints(dev, lens), seq=ints(dev, seqs))
         c.check(out.numpy(), c.note(x, pos, seq, cs), pos, seq, "draft")
         c.check_stored()
+    c.close()
+
+
+def test_graphs_share_a_workspace(dev):
+    """Captured calls of two caches whose (sequence, kv head)s are shared by many CTAs, replayed in turn and among eager ones: the same bits every time."""
+    rng = np.random.default_rng(23)
+    a, b = Cache(dev, 8, 2, 128, "int8", 64, 3200, 2, rng), Cache(dev, 4, 2, 64, "fp8", 16, 2100, 3, rng)
+    a.fill([2900, 3000])
+    b.fill([1900, 40, 1000])
+    xa, pa = Tensor(a.rows(200), device=dev), ints(dev, [2900, 3000])
+    xb, pb = Tensor(b.rows(3), device=dev), ints(dev, [1900, 40, 1000])
+    rows, seq = ints(dev, np.concatenate([2900 + np.arange(100), 3000 + np.arange(100)])), ints(dev, np.repeat([0, 1], 100))
+    first = ints(dev, [0, 100])
+    outs = [Tensor.zeros((200, 8 * 128), "float16", dev), Tensor.zeros((200, 8 * 128), "float16", dev), Tensor.zeros((3, 4 * 64), "float16", dev)]
+    ka, va = (Tensor.zeros((200, 2 * 128), "float16", dev) for _ in range(2))
+
+    def many():
+        a.kv.write(0, xa, rows, seq=seq)
+        a.kv.attend(0, xa, pa, first=first, max_count=100, out=outs[0])
+        a.kv.read(0, pa, first=first, max_count=100, k=ka, v=va)
+
+    def few():
+        b.kv.decode(0, xb, pb, out=outs[2])
+        a.kv.attend(0, xa, pa, first=first, max_count=3, out=outs[1])
+
+    many()
+    few()
+    want = [t.numpy().copy() for t in (*outs, ka, va)]
+    q = a.note(xa.numpy(), np.concatenate([2900 + np.arange(100), 3000 + np.arange(100)]), np.repeat([0, 1], 100))
+    some = [0, 50, 99, 100, 199]
+    a.check(want[0][some], q[some], [2900, 2950, 2999, 3000, 3099], [0, 0, 0, 1, 1])
+    b.check(want[2], b.note(xb.numpy(), np.array([1900, 40, 1000]), np.arange(3)), [1900, 40, 1000], [0, 1, 2])
+    with CUDAGraph(dev) as g1:
+        many()
+    with CUDAGraph(dev) as g2:
+        few()
+    for turn in ((g1.launch, g2.launch), (g2.launch, few, g1.launch), (many, g2.launch, g1.launch, g2.launch), (g1.launch, g1.launch, few)):
+        for t in (*outs, ka, va):
+            t.assign(np.zeros(t.shape, np.float16))
+        for call in turn:
+            call()
+        for got, w in zip((*outs, ka, va), want):
+            np.testing.assert_array_equal(got.numpy().view(np.uint16), w.view(np.uint16))
+    a.close()
+    b.close()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_pages_beyond_4_gib(dev, fmt):
+    """Pages at the end of pools of more than 2^32 codes."""
+    rng = np.random.default_rng(24)
+    H, G, hd, page, n_pages = 8, 8, 128, 64, 66000
+    c = Cache.__new__(Cache)
+    c.dev, c.H, c.G, c.hd, c.fmt, c.rng = dev, H, G, hd, fmt, rng
+    c.kv = QuantKVCache(dev, 1, H, G, hd, 512, 2, page_size=page, dtype=fmt, n_pages=n_pages)
+    c.kv.set_block_table(np.stack([n_pages - 1 - np.arange(8), 65536 - 4 + np.arange(8)]).astype(np.int32))
+    c.n = 512
+    c.k, c.v = (np.zeros((2, c.n, G, hd), np.float16) for _ in range(2))
+    attend(c, [250, 3], [140, 400], False, seed=15, slots=2)
+    c.check_stored()
+    pos = np.array([390, 403])
+    x = c.rows(2)
+    out = c.kv.decode(0, Tensor(x, device=dev), ints(dev, pos))
+    c.check(out.numpy(), c.note(x, pos, np.arange(2)), pos, np.arange(2))
+    c.check_stored()
+    c.close()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_a_slot_used_again(dev, fmt):
+    """Behind a conversation's end lie rows of an earlier one, of the largest scales and of none."""
+    rng = np.random.default_rng(25)
+    c = Cache(dev, 8, 2, 128, fmt, 16, 160, 2, rng)
+    x = c.rows(320)
+    old = c.split(x)
+    old[1][:] = np.where(rng.random(old[1].shape) < 0.5, 65504, -65504)
+    old[2][:] = np.where(rng.random(old[2].shape) < 0.5, 65504, -65504)
+    old[1][::3] = np.nan
+    c.kv.write(0, Tensor(x, device=dev), ints(dev, np.tile(np.arange(160), 2)), seq=ints(dev, np.repeat([0, 1], 160)))
+    c.fill([37, 90])
+    for i in range(20):
+        pos = np.array([37, 90]) + i
+        y = c.rows(2)
+        out = c.kv.decode(0, Tensor(y, device=dev), ints(dev, pos))
+        c.check(out.numpy(), c.note(y, pos, np.arange(2)), pos, np.arange(2), f"token {i}")
+    for most in (2, 9):  # few queries and many, over a tile with rows of both
+        q = rng.standard_normal((2 * most, 8 * 128)).astype(np.float16)
+        pos = np.array([57, 110]) - most
+        out = c.kv.attend(0, Tensor(q, device=dev), ints(dev, pos), first=ints(dev, [0, most]), max_count=most)
+        c.check(out.numpy(), q.reshape(-1, 8, 128), np.concatenate([pos[0] + np.arange(most), pos[1] + np.arange(most)]), np.repeat([0, 1], most), "chunk")
     c.close()
 
 
