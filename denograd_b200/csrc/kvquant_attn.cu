@@ -42,8 +42,8 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
-  // Up to 24 columns are read at HBM's pace or near it: 8 sequences of 5 positions behind 3001, 20 columns, 31 us (the tensor cores' form 38),
-  // 16 columns 22 us (38), 32 sequences 84 us (93).  Beyond that a lane's outputs do not fit its registers.
+  // Up to 24 columns are read at HBM's pace or near it: 8 sequences of 5 positions behind 3001, 20 columns, 29.5 us (the tensor cores' form 38),
+  // 16 columns 20.8 us (38), 32 sequences 84 us (93).  Beyond that a lane's outputs do not fit its registers.
   if ((long long)max_count * (H / G) <= 24) {
     KvqSplitArgs s = {};
     s.c = kvq_layer(kv, layer);

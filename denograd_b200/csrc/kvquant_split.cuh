@@ -32,7 +32,6 @@ struct KvqSplitArgs {
 };
 
 constexpr int KS_WARPS = 4, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_CTAS = 3;  // CTAs to an SM
-constexpr int KS_FIXED = 3;  // units that a (sequence, kv head) costs beside its own
 constexpr int KS_AHEAD = 3;  // tiles of a warp that are asked into L2 when it begins
 constexpr int KS_GROUP = 8;  // pieces that are added up ahead of the others, where there are many
 
@@ -42,6 +41,9 @@ struct KsCfg {
   static constexpr int VB = HD / 8;                             // bytes of a V row that a lane holds
   static constexpr size_t MERGE = KS_WARPS * COLS * HD * 4;     // the warps' outputs when they meet
   static constexpr int PART = COLS * (HD + 2);                  // floats of a piece: outputs, maxima, sums
+  // Units that a (sequence, kv head) costs beside its own.  One column group: 1, 3 and 6 within 1 %; more: 8 sequences of 5 positions behind 3001 of the
+  // 8B 30.9 us with 3, 29.5 with 5, 29.8 with 7 (30 ragged ones 25.5, 25.3, 27.1).
+  static constexpr int FIXED = NT == 1 ? 3 : 5;
 };
 
 #ifdef __CUDACC__
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
   };
   // this CTA's stretch of the line of units, and the sequence that it begins in; every warp works it out for itself
   long long total = 0;
-  for (int b = lane; b < a.B; b += 32) total += units(b) + KS_FIXED;
+  for (int b = lane; b < a.B; b += 32) total += units(b) + Cfg::FIXED;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   total *= a.c.G;
@@ -111,7 +113,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
   int b = 0;
   long long at = 0;  // first unit of (b, head 0)
   for (int base = 0;; base += 32) {
-    const int n = base + lane < a.B ? units(base + lane) + KS_FIXED : 0;
+    const int n = base + lane < a.B ? units(base + lane) + Cfg::FIXED : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -132,15 +134,15 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
     int p0, n_new;
     const int32_t* bt;
     const int T = sequence(b, p0, n_new, bt);
-    const int n_units = max(1, (T + KS_UNIT - 1) / KS_UNIT), span = n_units + KS_FIXED;  // its units lie behind its fixed cost
+    const int n_units = max(1, (T + KS_UNIT - 1) / KS_UNIT), span = n_units + Cfg::FIXED;  // its units lie behind its fixed cost
     const bool stored = NEW && bt != nullptr;  // there is a new token, at p0
     const long long row0 = NEW ? b : (a.first ? a.first[b] : b);
     const int n_cols = n_new * a.n_rep;
     for (int g = (int)((u - at) / span); g < a.c.G && u < u_hi; g++) {
       const long long item = at + (long long)g * span;
-      const int j0 = max(0, (int)(u - item) - KS_FIXED);
+      const int j0 = max(0, (int)(u - item) - Cfg::FIXED);
       u = min(item + span, u_hi);
-      const int j1 = max(0, (int)(u - item) - KS_FIXED);
+      const int j1 = max(0, (int)(u - item) - Cfg::FIXED);
       if (j0 == j1) continue;
       const int t_lo = j0 * KS_UNIT, t_hi = min(T, j1 * KS_UNIT);
       const int n_tiles = t_hi > t_lo + warp * 16 ? (t_hi - t_lo - warp * 16 + KS_UNIT - 1) / KS_UNIT : 0;  // of this warp
@@ -430,7 +432,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
       if (whole) { __syncthreads(); continue; }
       // ---- pieces of a (sequence, kv head) that CTAs c_lo .. c_hi share: the last to arrive adds them up in this order.  Many are added up in
       // groups of neighbours first, as these are done: one CTA reads 30 pieces in 10 us.
-      const long long begin = item + KS_FIXED, last = begin + n_units - 1;
+      const long long begin = item + Cfg::FIXED, last = begin + n_units - 1;
       const int c_lo = (int)(((begin + 1) * ctas - 1) / total), c_hi = (int)(((last + 1) * ctas - 1) / total), pieces = c_hi - c_lo + 1;
       auto arrive = [&](unsigned int* ticket, int of) -> bool {  // whether this CTA is the last
         __syncthreads();
