@@ -42,9 +42,10 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
              max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
-  // Up to 24 columns are read at HBM's pace or near it: 8 sequences of 5 positions behind 3001, 20 columns, 29.5 us (the tensor cores' form 38),
-  // 16 columns 20.8 us (38), 32 sequences 84 us (93).  Beyond that a lane's outputs do not fit its registers.
-  if ((long long)max_count * (H / G) <= 24) {
+  // Few columns are read at HBM's pace or near it: 8 sequences behind 3001 positions of the 8B, 16 columns 21.3 us (the tensor cores' form 38), 20
+  // columns 26.3 (38), 32 sequences of these 71 (93); 24 sequences behind 4000 of the 1B, 28 columns 54 (67).  A lane's outputs have to fit its
+  // registers: 32 columns of 128 values would take 42 us, against 38.
+  if ((long long)max_count * (H / G) <= (hd == 64 ? 32 : 24)) {
     KvqSplitArgs s = {};
     s.c = kvq_layer(kv, layer);
     s.x = (const __half*)q; s.out = (__half*)out;
@@ -58,7 +59,8 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   if (kv->format == FORMAT_ && hd == HD_)                                                \
     return columns <= 8    ? launch_split<FMT_, HD_, 1, false>(dev, s)                   \
            : columns <= 16 ? launch_split<FMT_, HD_, 2, false>(dev, s)                   \
-                           : launch_split<FMT_, HD_, 3, false>(dev, s);
+           : columns <= 24 ? launch_split<FMT_, HD_, 3, false>(dev, s)                   \
+                           : launch_split<FMT_, HD_, HD_ == 64 ? 4 : 3, false>(dev, s);
     KS_CASE(KVQ_INT8, JG_KVQ_INT8, 64) KS_CASE(KVQ_INT8, JG_KVQ_INT8, 128) KS_CASE(KVQ_E4M3, JG_KVQ_E4M3, 64) KS_CASE(KVQ_E4M3, JG_KVQ_E4M3, 128)
 #undef KS_CASE
   }

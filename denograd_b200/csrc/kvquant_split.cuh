@@ -5,14 +5,22 @@
 //   out^T [hd x columns] += V^T [hd x 16 positions] . w^T        mma.sync.m16n8k16, 32-bit sums
 // The inner index of a product and the order of its rows are free as long as both operands agree, so a lane's fragments are 16
 // neighbouring codes of a row: of K as they lie, of V two rows at a time with their bytes interleaved.  So a lane loads just what it
-// multiplies, 16 bytes at a time and a tile ahead, straight into registers.  V is multiplied by its scale as it is widened (exact), K's scale goes to the finished scores.
+// multiplies, 16 bytes at a time and a tile ahead, straight into registers (32 sequences of 4100 positions of the 8B 67 us; staged in shared
+// memory 81).  V is multiplied by its scale as it is widened (exact), K's scale goes to the finished scores.  The queries' fragments lie in
+// shared memory, each lane's own, which leaves the registers to outputs and tiles (20 columns 26.3 us, 29.5 with them in registers; one
+// column group 67.5, 68.2).
 //
 // The running maximum is a reference that scores may pass by 2^6 before sums and outputs are rescaled: a vote a tile instead of three
 // rounds of shuffles.
 //
 // The positions of all (sequence, kv head)s are one line of units of 16 * KS_WARPS, with some more for what each costs by itself, cut
-// evenly over the CTAs: long and short conversations of a batch cost what they hold.  A CTA's stretch holds pieces of several (sequence, kv head)s; those that others
-// share are left in a workspace (at most two a CTA: its first and its last), and the last to arrive puts them together in order.
+// evenly over the CTAs: long and short conversations of a batch cost what they hold.  A CTA's stretch holds pieces of several (sequence,
+// kv head)s; those that others share are left in a workspace (at most two a CTA: its first and its last), and the last to arrive puts them
+// together in order.
+//
+// What bounds it.  32 x 4100 positions, 274 MB: the loops run at about 6 TB/s; 4.5 us pass before them (positions, page, first tiles: three
+// trips through memory), 5 behind (the warps meet, the pieces), and a stretch with two pieces ends 4 us after one with one.  Three column
+// groups run on eight warps an SM, 255 registers each: there latency bounds the loops (3.1 TB/s, issue slots a third full).
 #pragma once
 #include "kvquant.cuh"
 
@@ -39,7 +47,8 @@ template <int HD, int NT>
 struct KsCfg {
   static constexpr int COLS = 8 * NT, KJ = HD / 64;             // 16-byte pieces of a K row that a lane holds
   static constexpr int VB = HD / 8;                             // bytes of a V row that a lane holds
-  static constexpr size_t MERGE = KS_WARPS * COLS * HD * 4;     // the warps' outputs when they meet
+  static constexpr size_t Q_BYTES = NT * KJ * 1024;             // a warp's fragments of q
+  static constexpr size_t MERGE = KS_WARPS * COLS * HD * 4;     // the warps' outputs when they meet, in the place of these
   static constexpr int PART = COLS * (HD + 2);                  // floats of a piece: outputs, maxima, sums
   // Units that a (sequence, kv head) costs beside its own.  One column group: 1, 3 and 6 within 1 %; more: 8 sequences of 5 positions behind 3001 of the
   // 8B 30.9 us with 3, 29.5 with 5, 29.8 with 7 (30 ragged ones 25.5, 25.3, 27.1).
@@ -61,6 +70,14 @@ __device__ __forceinline__ uint32_t ks_transpose(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+__device__ __forceinline__ void ks_put(uint32_t at, const uint4& x) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+}
+__device__ __forceinline__ uint4 ks_get(uint32_t at, int turn) {  // anew in each turn of a loop: not to be kept in registers
+  uint4 x;
+  asm("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4]; // %5" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at), "r"(turn));
+  return x;
 }
 __device__ __forceinline__ uint32_t ks_half2(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
@@ -187,7 +204,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         t.sv1 = *reinterpret_cast<const uint2*>(s + 2 * c + 8);
       };
       // ---- fragments of q^T: the lane's column is nt * 8 + r.  Everything is asked for before anything is waited for.
-      uint32_t qf[NT][KJ * 4][2];
+      uint32_t q_at = (uint32_t)__cvta_generic_to_shared(ks_raw) + (uint32_t)(warp * Cfg::Q_BYTES + lane * 16);  // the lane's own, [nt][j][2] 512 bytes apart
       Tile tile;
       // The new token is an entry of its own when the warps' sums meet, made by the CTA with the end of its sequence and stored on the way.  Its
       // last warp has a tile less than the others at most times.
@@ -231,10 +248,11 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
             uint4 lo = x[nt][j][0], hi = x[nt][j][1];
             if (turned) { lo = kvq_rotate(lo, turn[j][0]); hi = kvq_rotate(hi, turn[j][1]); }
             if (!have[nt]) lo = hi = make_uint4(0, 0, 0, 0);
-            qf[nt][j * 4][0] = lo.x; qf[nt][j * 4][1] = lo.y; qf[nt][j * 4 + 1][0] = lo.z; qf[nt][j * 4 + 1][1] = lo.w;
-            qf[nt][j * 4 + 2][0] = hi.x; qf[nt][j * 4 + 2][1] = hi.y; qf[nt][j * 4 + 3][0] = hi.z; qf[nt][j * 4 + 3][1] = hi.w;
+            ks_put(q_at + (nt * KJ + j) * 1024, lo);
+            ks_put(q_at + (nt * KJ + j) * 1024 + 512, hi);
           }
       }
+      asm volatile("" : "+r"(q_at)::"memory");  // what is read at q_at comes after
       // ---- the new token
       if (fresh) {
         constexpr int LPR = HD / 8;
@@ -261,10 +279,14 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         __syncwarp();
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < KJ * 4; j++) {
-          const uint2 kw = *reinterpret_cast<const uint2*>(&s_new[0][(j >> 2) * 64 + c * 16 + (j & 3) * 4]);
-          const float2 k0 = h2_to_f2(kw.x), k1 = h2_to_f2(kw.y), q0 = h2_to_f2(qf[0][j][0]), q1 = h2_to_f2(qf[0][j][1]);
-          s = fmaf(k0.x, q0.x, fmaf(k0.y, q0.y, fmaf(k1.x, q1.x, fmaf(k1.y, q1.y, s))));
+        for (int j = 0; j < KJ * 2; j++) {
+          const uint4 k = ld_128(&s_new[0][(j >> 1) * 64 + c * 16 + (j & 1) * 8]), q = ks_get(q_at + j * 512, 0);
+          const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, qw[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float2 k0 = h2_to_f2(kw[e]), q0 = h2_to_f2(qw[e]);
+            s = fmaf(k0.x, q0.x, fmaf(k0.y, q0.y, s));
+          }
         }
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
@@ -296,6 +318,13 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
 #pragma unroll
         for (int j = 0; j < KJ; j++) {
           const uint32_t w0[4] = {t.k[0][j].x, t.k[0][j].y, t.k[0][j].z, t.k[0][j].w}, w1[4] = {t.k[1][j].x, t.k[1][j].y, t.k[1][j].z, t.k[1][j].w};
+          uint32_t qw[NT][8];
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            const uint4 lo = ks_get(q_at + (nt * KJ + j) * 1024, i), hi = ks_get(q_at + (nt * KJ + j) * 1024 + 512, i);
+            qw[nt][0] = lo.x; qw[nt][1] = lo.y; qw[nt][2] = lo.z; qw[nt][3] = lo.w;
+            qw[nt][4] = hi.x; qw[nt][5] = hi.y; qw[nt][6] = hi.z; qw[nt][7] = hi.w;
+          }
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             __half2 a0, a1, a2, a3;
@@ -303,7 +332,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
             kvq_widen<FMT>(w1[e], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
-              ks_mma(e & 1 ? s_[nt] : s[nt], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), qf[nt][j * 4 + e][0], qf[nt][j * 4 + e][1]);
+              ks_mma(e & 1 ? s_[nt] : s[nt], ks_half2(a0), ks_half2(a1), ks_half2(a2), ks_half2(a3), qw[nt][2 * e], qw[nt][2 * e + 1]);
           }
         }
         const float ks0 = __low2float(t.s0) * a.scale2, ks1 = __low2float(t.s1) * a.scale2;
@@ -512,7 +541,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
 
 static inline int ks_ctas(const jg_dev* dev) { return KS_CTAS * dev->sm_count; }  // that a device runs at once; twice as many tickets: jg_kvq_ticket_bytes
 static inline int ks_slots(const jg_dev* dev) { return 2 * ks_ctas(dev); }  // pieces in the workspace
-static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 3>::PART : KsCfg<128, 3>::PART; }
+static inline size_t ks_part_floats(int hd) { return hd == 64 ? KsCfg<64, 4>::PART : KsCfg<128, 3>::PART; }
 
 template <int FMT, int HD, int NT, bool NEW>
 static int launch_split(jg_dev* dev, const KvqSplitArgs& a) {

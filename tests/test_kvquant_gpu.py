@@ -274,11 +274,12 @@ def test_attend_long_and_many(dev, H, G, hd, ahead, new, fmt):
     c.close()
 
 
-# Queries of a kv head on either side of 8, 16 and 24, where the kernel for few of them takes more columns, and beyond it; long caches, so that
+# Queries of a kv head on either side of 8, 16, 24 and 32, where the kernel for few of them takes more columns, and beyond it; long caches, so that
 # (sequence, kv head)s are shared
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 @pytest.mark.parametrize("H,G,hd,new", [(8, 1, 128, [2]), (8, 1, 128, [3, 3]), (8, 1, 64, [3]), (8, 1, 128, [4]), (12, 4, 64, [8, 7, 8]), (12, 4, 128, [6, 8]), (12, 4, 128, [9, 8]),
-                                        (2, 2, 64, [24]), (2, 2, 128, [25, 17]), (2, 1, 128, [9, 12])])
+                                        (2, 2, 64, [24]), (2, 2, 128, [25, 17]), (2, 1, 128, [9, 12]), (8, 1, 64, [4, 4]), (12, 4, 64, [10]), (12, 4, 64, [11, 9, 3]),
+                                        (2, 2, 64, [25, 32]), (2, 2, 64, [33, 30])])
 def test_attend_few_queries(dev, H, G, hd, new, fmt):
     ahead = [2907, 66, 0][:len(new)]
     c = Cache(dev, H, G, hd, fmt, 32, max(a + n for a, n in zip(ahead, new)), len(new) + 1, np.random.default_rng(21))
