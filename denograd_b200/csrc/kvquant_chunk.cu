@@ -28,7 +28,7 @@ constexpr int KC_SOFT_REGS = 144, KC_WIDEN_REGS = 72, KC_MMA_REGS = 48;       //
 static_assert(2 * KC_SOFT_REGS + 2 * KC_WIDEN_REGS + KC_MMA_REGS <= 5 * KC_REGS, "register shares exceed what a CTA is launched with");
 constexpr int KC_PLAN = 4;  // pieces that the plan is ahead
 constexpr int KC_HALF = KC_KEYS / 2;  // keys of a step of the softmax
-constexpr int KC_WHOLE = 8, KC_GRAIN = 6, KC_FIXED = 2;  // tiles: see the line of tiles
+constexpr int KC_WHOLE = 8, KC_SINGLE = 12, KC_GRAIN = 6, KC_FIXED = 2;  // tiles: see the line of tiles
 
 template <int HD>
 struct KcCfg {
@@ -192,11 +192,14 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     return v;
   };
   // An item costs what KC_FIXED tiles do beside its own.  Cutting one costs its CTAs a trip through memory each, 2 to 4 us: short items are
-  // not cut, others not into less than KC_GRAIN tiles.
+  // not cut, others not into less than KC_GRAIN tiles.  `uncut`: none is longer than KC_WHOLE tiles, or KC_SINGLE where there is a CTA for each (512 new
+  // positions of the 8B, 4 tiles: cut 33 us, 16.3; 45 behind 1100, 10 tiles, 8 items: 34, 23; 160 items of these: 48, 55; 45 behind
+  // 1900, 16 tiles: 32, 33).
   long long total = 0, u_lo = 0, u_hi = 0;
   int longest = 0, ctas = 1;
+  bool uncut = false;
   auto share = [&]() {
-    const long long most = longest <= KC_WHOLE ? total : total / KC_GRAIN;
+    const long long most = uncut ? total : total / KC_GRAIN;
     ctas = (int)max(1ll, min((long long)gridDim.x, most));
     if ((int)blockIdx.x >= ctas) return;
     if (total < (1 << 23)) {  // 512 CTAs at most: see the launch
@@ -219,6 +222,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     __syncthreads();
     total = 0;
     for (int w = 0; w < KC_THREADS / 32; w++) { total += s_sum[w]; longest = max(longest, s_longest[w]); }
+    uncut = longest <= KC_WHOLE;
     share();
     long long before = 0;
     for (int base = 0; base < entries && u_lo < u_hi; base += KC_THREADS) {  // the same for all threads
@@ -262,21 +266,21 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         int items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
         // Short items that leave half of the CTAs idle become items of half the rows, whose two streams share their keys (512 new positions of the
         // 8B 16.6 us, 18.7 without); and where each CTA has one at most, they count alike (18.7 us, 19.3 without).
-        if (longest <= KC_WHOLE && entries <= 16 && 2 * items <= (int)gridDim.x) {
+        uncut = longest <= (items <= (int)gridDim.x ? KC_SINGLE : KC_WHOLE);
+        if (uncut && entries <= 16 && 2 * items <= (int)gridDim.x) {
           rows = KC_ROWS / 2;
           per *= 2;
           KcPiece p;
           n = lane < a.B * per ? kc_item(a, lane / per, lane % per, rows, p) : 0;
           items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
         }
-        single = longest <= KC_WHOLE && items <= (int)gridDim.x;
+        single = uncut && items <= (int)gridDim.x;
         const long long mine = single ? (n > 0 ? a.c.G : 0) : cost(n), sum = scan64(mine);
         total = __shfl_sync(0xffffffffu, sum, 31);
         share();
         entry = max(0, __ffs(__ballot_sync(0xffffffffu, sum > u_lo)) - 1);
         at = __shfl_sync(0xffffffffu, sum - mine, entry);
       }
-      const bool cut = longest > KC_WHOLE;
       long long u = u_lo;
       int b = entry / per, tile = entry % per;
       for (;; planned++) {
@@ -296,7 +300,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           }
           p.g = (int)(u - at) / span;  // both below 2^31: see the limits of the cache
           const long long item = at + (long long)p.g * span;
-          if (!cut) {  // the CTA in whose stretch it begins has all of it
+          if (uncut) {  // the CTA in whose stretch it begins has all of it
             const bool mine = u == item;
             u = item + span;
             if (!mine) continue;
@@ -437,15 +441,6 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         return __half2float(scales[2 * (size_t)row_at((lane / PER % N) * ROWS + (warp & 3) * PER + lane % PER)]);
       };
       auto codes_at = [&](int i) { return ld_stream_128(codes + (size_t)row_at(row + i * ROWS) * HD); };
-      // the rows of a tile on their way into L2, one to a thread, where a tile of few rows is done before another comes from HBM
-      const bool hurry = p.left <= 128;
-      auto ahead = [&](int j, int page) {
-        const uint32_t begin = first_row(j, page);
-        const int r = u;
-        const size_t at = __shfl_sync(0xffffffffu, begin, r >> 4) + (uint32_t)(j * KC_KEYS + r <= last ? r & 15 : 0);
-        prefetch_l2(codes - sub * 16 + at * HD);
-        if ((r & 15) == 0) prefetch_l2(scales + 2 * at);
-      };
       int page = page_of(p.j0), page2 = page_of(p.j0 + 1);
       tile_at(p.j0, page);
       float s = scale_at();
@@ -453,10 +448,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       for (int i = 0; i < N; i++) x[i] = codes_at(i);
       page = page2;
       page2 = page_of(p.j0 + 2);
-      if (hurry && p.j0 + 1 < p.j1) ahead(p.j0 + 1, page);
       for (int j = p.j0; j < p.j1; j++, tiles++) {
         const uint32_t slot = tiles & 1;
-        if (hurry && j + 2 < p.j1) ahead(j + 2, page2);
         if (tiles >= 2) ok = mbar_wait(&empty[slot], ((tiles >> 1) - 1) & 1);
         if (!ok) break;
         unsigned char* to = tile + (size_t)slot * Cfg::KV_BYTES;

@@ -40,7 +40,6 @@ struct KvqSplitArgs {
 };
 
 constexpr int KS_WARPS = 4, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_CTAS = 3;  // CTAs to an SM
-constexpr int KS_AHEAD = 3;  // tiles of a warp that are asked into L2 when it begins
 constexpr int KS_GROUP = 8;  // pieces that are added up ahead of the others, where there are many
 
 template <int HD, int NT>
@@ -237,10 +236,6 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
           if (a.table) kt = ld_128(a.table + (size_t)p0 * HD + lane % (HD / 8) * 8);
         }
         if (n_tiles > 0) load(0, tile);
-        // the next tiles on their way into L2, a line to a lane: at the start nothing else keeps HBM busy
-#pragma unroll
-        for (int i = 1; i <= KS_AHEAD; i++)
-          if (i < n_tiles) prefetch_l2((lane < 16 ? a.c.k : a.c.v) + (row_of(i) + (lane & 15)) * HD);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll

@@ -290,7 +290,8 @@ def test_attend_few_queries(dev, H, G, hd, new, fmt):
 # Prompts that the tensor cores' form cuts into items of 128 rows where they leave half of the SMs idle, and into 256 where they do not: sequences and
 # rows on either side of the choice
 @pytest.mark.parametrize("H,G,hd,new,ahead", [(32, 8, 128, [300], 0), (32, 8, 64, [576], 0), (32, 8, 128, [577], 100), (32, 8, 64, [640], 0), (8, 1, 64, [129], 900), (4, 1, 64, [33] * 16, 0),
-                                              (4, 1, 64, [33] * 17, 0), (4, 4, 128, [128, 129, 256, 257], 40), (8, 1, 128, [700, 40], 200), (16, 8, 64, [64, 0, 65, 1, 200], 700)])
+                                              (4, 1, 64, [33] * 17, 0), (4, 4, 128, [128, 129, 256, 257], 40), (8, 1, 128, [700, 40], 200), (16, 8, 64, [64, 0, 65, 1, 200], 700), (4, 1, 64, [45], 1100), (8, 2, 128, [45], 1900),
+                                              (32, 8, 64, [45] * 20, 1000), (4, 1, 128, [900], 600)])
 def test_attend_prompts(dev, H, G, hd, new, ahead):
     c = Cache(dev, H, G, hd, "int8", 64, ahead + max(new), len(new) + 1, np.random.default_rng(22))
     attend(c, [ahead] * len(new), new, False, seed=14)
