@@ -25,6 +25,19 @@
 #ifdef __CUDACC__
 constexpr int FT_ROWS = 128, FT_KV = 128, FT_THREADS = 320, FT_ST = 2;
 
+// All columns of tensor memory, taken by one warp; every thread of the CTA calls it.  The successor may start only now: see tcgen05.cuh.
+__device__ __forceinline__ uint32_t ft_columns(uint32_t* s_tmem, bool taker) {
+  if (taker) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *s_tmem;
+  pdl_launch();
+  return tmem;
+}
 __device__ __forceinline__ void ft_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 __device__ __forceinline__ float ft_ex2(float x) {  // 2^x by the hardware's approximation (2^-22 relative), 0 for -inf
   float y;
@@ -109,15 +122,7 @@ __device__ __forceinline__ void flash_tc(P& p, int* err) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 9) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = s_tmem;
-  pdl_launch();  // only now: see tcgen05.cuh
+  const uint32_t tmem = ft_columns(&s_tmem, warp == 9);
   pdl_wait();
   const bool work = p.begin();  // the same for all threads
   const int n = work ? p.tiles : 0;

@@ -5,17 +5,22 @@
 // a tile crosses HBM as bytes and no 16-bit copy of the cache exists.
 //
 // A query row is a (position, query head) of one kv head; an item is 256 rows, two streams of 128, over the keys that its last
-// row sees, in tiles of 128.  Five warpgroups: softmax of either stream, a thread per row; one that loads and widens K, one for V;
-// the last issues the products and keeps the plan.  While one stream's exponentials run, the other's products do; a product with V
-// begins when the first half of its weights is there.  Tensor memory: S of both streams (P
-// takes its place as 16-bit pairs), O of both.  A row's maximum is a reference that its scores may pass by 2^8 before O is
-// rescaled in tensor memory, which is rare behind the first tiles.
+// row sees, in tiles of 128; an item of up to 128 rows has its tiles take turns between the streams, whose outputs meet at its end.  Five
+// warpgroups: softmax of either stream, a thread per row; one that loads and widens K, one for V; the last issues the products and keeps
+// the plan.  While one stream's exponentials run, the other's products do; a product with V begins when the first half of its weights is
+// there.  Tensor memory: S of both streams (P takes its place as 16-bit pairs), O of both.  A row's maximum is a reference that its scores
+// may pass by 2^8 before O is rescaled in tensor memory, which is rare behind the first tiles.
 //
 // The tiles of all items are one line, cut evenly over one CTA for each SM.  An item that several CTAs share meets in a
-// workspace; the last to arrive adds the pieces up in order.
+// workspace; the last to arrive adds the pieces up in order (3 us for two pieces of 256 x 64, 10 for five of 256 x 128: what one SM reads).
 //
-// What bounds it: per 256 rows x 128 keys x 128 columns four products of 512 cycles at the tensor peak, and 32768
-// exponentials at 16 a cycle, 2048 cycles either way; widening takes a fifth of the issue slots beside them.
+// What bounds it: per 256 rows x 128 keys x 128 columns four products of 512 cycles at the tensor peak, and 32768 exponentials at 16 a
+// cycle, 2048 cycles either way; such a unit takes 4000.  2048 positions of the 8B behind 6001, fp8: 230 us, 1.02 PFLOP/s.  The tensor pipe
+// and the exponentials' are each busy 47 % of the time, issue slots 45 %: the two softmax warps of a scheduler wait for tensor memory, their
+// maxima and votes, and fill each other's gaps only in part (without exponentials 200 us, without a softmax 171, without widening 212).
+// Tried and slower: two threads to a row on 16 warps (290: registers), the widening on 16 warps (265), products of half a tile's keys, all 128
+// scores in registers, a share of the exponentials as polynomials; rows of 64 values with weights apart from the scores, so that the next
+// scores are made meanwhile (82.3 and 83.9 us for 24 ragged chunks of the 1B).
 #include <math.h>
 
 #include "flash_tc.cuh"
@@ -159,15 +164,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 16) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = s_tmem;
-  pdl_launch();  // only now: see tcgen05.cuh
+  const uint32_t tmem = ft_columns(&s_tmem, warp == 16);
   pdl_wait();
 
   // ---- the line of tiles: how long it is, and where this CTA's stretch begins.  Entry e = (sequence, item of it), all kv heads.  Up to 32
