@@ -5,6 +5,7 @@ Layout:
   ffi.py     ctypes binding of that ABI (the Python twin of ts/ops_cuda.ts's Deno.dlopen table)
   device.py  CUDA (Compiled), CUDAAllocator, Buffer, Tensor, CUDAGraph — jsgrad/device.ts + runtime/allocator.ts
   nn.py      Linear, Int8Linear, RMSNorm, Embedding, Int8Embedding, state dicts — jsgrad/nn + models/llama3.ts
+  kvquant.py QuantKVCache: the KV cache in 8 bits, with what stores to it and attends over it
   llama.py   Attention, FeedForward, TransformerBlock, Transformer, TinyJit — jsgrad/models/llama.ts
   llama3.py  MODEL_PARAMS, Llama3 (load, prefill, greedy generation) — jsgrad/models/llama3.ts
   decoder.py, driver.py   what every decoder / driver shares: jit, sample, decode loop, prefill, chat, generate
