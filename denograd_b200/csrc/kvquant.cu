@@ -125,11 +125,11 @@ struct KvqWriteArgs {
   int ldq, ldx, table_rows, R, H;
 };
 
-constexpr int KW_THREADS = 256;
+constexpr int KW_THREADS = 128;
 
 // A thread for each eight values of a row's Q heads, and of its K heads together with V, of U neighbouring rows: all their loads
 // are on their way before any is waited for (positions and slots are not needed for the values, only for where they go).
-// Bound by its passes over rows and codes: 3800 rows of the 8B, 102 MB with the rotated queries, 20.3 us, 5 TB/s.
+// Bound by its passes over rows and codes: 3800 rows of the 8B, 86 MB with the rotated queries, 18.7 us, 4.6 TB/s; issue slots are 70 % busy.
 template <int FMT, int HD, int U>
 __global__ void __launch_bounds__(KW_THREADS) kvq_write_kernel(const KvqWriteArgs a) {
   constexpr int LPR = HD / 8;
@@ -177,10 +177,10 @@ __global__ void __launch_bounds__(KW_THREADS) kvq_write_kernel(const KvqWriteArg
 
 template <int FMT, int HD>
 static int launch_write(jg_dev* dev, const KvqWriteArgs& a) {
-  // Two rows to a thread where that leaves every SM eight CTAs; below, one.  3800 rows of the 8B: 21.2 us with one, 20.3 with two,
-  // 22.6 with four, 35 with eight (registers: fewer warps).
+  // Two rows to a thread where that leaves every SM sixteen CTAs; below, one.  3800 rows of the 8B: 20.3 us with one, 19.4 with two, 21.3
+  // with four (registers: fewer warps); 18.7 with CTAs of 128, 22.5 of 64.
   const unsigned long long per_row = (unsigned long long)(a.H + a.c.G) * (HD / 8), two = ((a.R + 1) / 2 * per_row + KW_THREADS - 1) / KW_THREADS;
-  if (two >= 8ull * dev->sm_count) return jg_launch(dev, "kvq_write", kvq_write_kernel<FMT, HD, 2>, dim3((unsigned)two), dim3(KW_THREADS), 0, a);
+  if (two >= 16ull * dev->sm_count) return jg_launch(dev, "kvq_write", kvq_write_kernel<FMT, HD, 2>, dim3((unsigned)two), dim3(KW_THREADS), 0, a);
   return jg_launch(dev, "kvq_write", kvq_write_kernel<FMT, HD, 1>, dim3((unsigned)((a.R * per_row + KW_THREADS - 1) / KW_THREADS)), dim3(KW_THREADS), 0, a);
 }
 
@@ -222,63 +222,67 @@ struct KvqReadArgs {
 constexpr int KR_THREADS = 256, KR_ROWS = 4;
 
 // A thread for each eight values of K and the eight of V beside them, of U neighbouring positions, whose loads are in flight together (8 ragged
-// stretches, 8B: 19.3 us with one position to a thread, 9.5 with four, 44 MB at 4.6 TB/s; 45 positions of the 1B 8.2 and 8.4 with the call).
+// stretches, 8B: 18 us with two positions to a thread, 10.3 with four, 44 MB at 4.3 TB/s; even ones, 201 MB, 35.2 us, 5.7 TB/s).
 template <int FMT, int HD>
 __global__ void __launch_bounds__(KR_THREADS) kvq_read_kernel(const KvqReadArgs a) {
   constexpr int LPR = HD / 8, U = KR_ROWS;
   pdl_launch();
   pdl_wait();
   const int b = blockIdx.y;
-  const unsigned per_row = (unsigned)a.c.G * LPR, at = blockIdx.x * (unsigned)KR_THREADS + threadIdx.x, group = at / per_row;
+  const unsigned per_row = (unsigned)a.c.G * LPR;
   const int count = a.count ? a.count[b] : a.max_count, first = a.first ? a.first[b] : b, p0 = a.pos[b], sq = a.seq ? a.seq[b] : b;
   const int n = min(count, a.max_count);
-  const long long i0 = (long long)group * U;
-  if (i0 >= n) return;
-  const int piece = (int)(at - group * per_row), g = piece / LPR, sub = piece % LPR;
   const bool known = (unsigned)sq < (unsigned)a.c.n_seq;
   const int32_t* bt_row = a.c.block_table + (size_t)(known ? sq : 0) * a.c.max_pages;
-  size_t from[U];
-  bool live[U];
+  for (unsigned at = blockIdx.x * KR_THREADS + threadIdx.x;; at += gridDim.x * KR_THREADS) {  // below 2^31: see the limit of a call
+    const unsigned group = at / per_row;
+    const long long i0 = (long long)group * U;
+    if (i0 >= n) return;
+    const int piece = (int)(at - group * per_row), g = piece / LPR, sub = piece % LPR;
+    size_t from[U];
+    bool live[U];
 #pragma unroll
-  for (int k = 0; k < U; k++) {
-    const long long t = p0 + i0 + k;
-    live[k] = known && i0 + k < n && t >= 0 && t < a.c.max_ctx;
-    from[k] = live[k] ? kvq_row(a.c, bt_row, (int)t, g) : 0;
-  }
-  uint2 kc[U], vc[U];
-  __half2 scale[U];
-#pragma unroll
-  for (int k = 0; k < U; k++) {
-    kc[k] = vc[k] = make_uint2(KVQ_ZERO<FMT>, KVQ_ZERO<FMT>);
-    scale[k] = __half2half2(__ushort_as_half(0));
-    if (live[k]) {
-      kc[k] = *reinterpret_cast<const uint2*>(a.c.k + from[k] * HD + sub * 8);
-      vc[k] = *reinterpret_cast<const uint2*>(a.c.v + from[k] * HD + sub * 8);
-      scale[k] = a.c.scales[from[k]];
+    for (int k = 0; k < U; k++) {
+      const long long t = p0 + i0 + k;
+      live[k] = known && i0 + k < n && t >= 0 && t < a.c.max_ctx;
+      from[k] = live[k] ? kvq_row(a.c, bt_row, (int)t, g) : 0;
     }
-  }
+    uint2 kc[U], vc[U];
+    __half2 scale[U];
 #pragma unroll
-  for (int k = 0; k < U; k++) {
-    const long long row = first + (i0 + k) * a.step;
-    if (i0 + k >= n || row < 0 || row >= a.R) continue;
-    const __half2 sk = __low2half2(scale[k]), sv = __hisnan(__low2half(scale[k])) ? sk : __high2half2(scale[k]);
-    __half2 h[4], w[4];
-    kvq_widen<FMT>(kc[k].x, h[0], h[1]);
-    kvq_widen<FMT>(kc[k].y, h[2], h[3]);
-    kvq_widen<FMT>(vc[k].x, w[0], w[1]);
-    kvq_widen<FMT>(vc[k].y, w[2], w[3]);
+    for (int k = 0; k < U; k++) {
+      kc[k] = vc[k] = make_uint2(KVQ_ZERO<FMT>, KVQ_ZERO<FMT>);
+      scale[k] = __half2half2(__ushort_as_half(0));
+      if (live[k]) {
+        kc[k] = *reinterpret_cast<const uint2*>(a.c.k + from[k] * HD + sub * 8);
+        vc[k] = *reinterpret_cast<const uint2*>(a.c.v + from[k] * HD + sub * 8);
+        scale[k] = a.c.scales[from[k]];
+      }
+    }
 #pragma unroll
-    for (int j = 0; j < 4; j++) { h[j] = __hmul2_rn(h[j], sk); w[j] = __hmul2_rn(w[j], sv); }
-    const size_t to = (size_t)row * a.ld + (size_t)g * HD + sub * 8;
-    *reinterpret_cast<uint4*>(a.k + to) = *reinterpret_cast<const uint4*>(h);
-    *reinterpret_cast<uint4*>(a.v + to) = *reinterpret_cast<const uint4*>(w);
+    for (int k = 0; k < U; k++) {
+      const long long row = first + (i0 + k) * a.step;
+      if (i0 + k >= n || row < 0 || row >= a.R) continue;
+      const __half2 sk = __low2half2(scale[k]), sv = __hisnan(__low2half(scale[k])) ? sk : __high2half2(scale[k]);
+      __half2 h[4], w[4];
+      kvq_widen<FMT>(kc[k].x, h[0], h[1]);
+      kvq_widen<FMT>(kc[k].y, h[2], h[3]);
+      kvq_widen<FMT>(vc[k].x, w[0], w[1]);
+      kvq_widen<FMT>(vc[k].y, w[2], w[3]);
+#pragma unroll
+      for (int j = 0; j < 4; j++) { h[j] = __hmul2_rn(h[j], sk); w[j] = __hmul2_rn(w[j], sv); }
+      const size_t to = (size_t)row * a.ld + (size_t)g * HD + sub * 8;
+      *reinterpret_cast<uint4*>(a.k + to) = *reinterpret_cast<const uint4*>(h);
+      *reinterpret_cast<uint4*>(a.v + to) = *reinterpret_cast<const uint4*>(w);
+    }
   }
 }
 
 template <int FMT, int HD>
 static int launch_read(jg_dev* dev, const KvqReadArgs& a, int B) {
   const unsigned long long per_row = (unsigned long long)a.c.G * (HD / 8), ctas = ((a.max_count + KR_ROWS - 1) / KR_ROWS * per_row + KR_THREADS - 1) / KR_THREADS;
-  return jg_launch(dev, "kvq_read", kvq_read_kernel<FMT, HD>, dim3((unsigned)ctas, (unsigned)B), dim3(KR_THREADS), 0, a);
+  const unsigned long long most = (20ull * dev->sm_count + B - 1) / B;  // CTAs: a ragged batch has many without rows (5, 10, 20 an SM, one each: 14.9, 12.3, 10.3, 11.4 us)
+  return jg_launch(dev, "kvq_read", kvq_read_kernel<FMT, HD>, dim3((unsigned)(ctas < most ? ctas : most), (unsigned)B), dim3(KR_THREADS), 0, a);
 }
 
 JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint64_t v, int32_t ld, int32_t R, uint64_t pos, uint64_t count,

@@ -104,26 +104,29 @@ __device__ __forceinline__ float kvq_inverse(float scale) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale));  // to 2^-23
   return r;
 }
-// Four values as a word of codes.  A scale beyond 512 (256) has codes whose values pass 65504: the largest that does not is 113 (240).
+// Eight values as two words of codes.  A scale beyond 512 (from 256 on) has codes whose values pass 65504: the largest that does not is 113 (240).
 // int8: the product is off by less than 2^-15 from x / scale, which is at most 127.  A quotient that is no tie is at least 2^-12 away
 // from one (x has 11 significant bits, scale 4), so rounding to multiples of 2^-13 first makes ties of the ties and of nothing
-// else.  Adding 1536 is that rounding, adding 1.5 2^23 the one to whole numbers, and 128 more the code's bias.
+// else.  Adding 1536 is that rounding, adding 1.5 2^23 less that the one to whole numbers, and 128 more the code's bias.
 template <int FMT>
-__device__ __forceinline__ uint32_t kvq_codes(const float (&x)[4], float scale, float inverse) {
-  if (!(scale > 0.f)) return KVQ_ZERO<FMT>;
-  const float top = FMT == KVQ_INT8 ? (scale > 512.f ? 113.f : 127.f) : (scale < 256.f ? 448.f : 240.f);
-  float q[4];
+__device__ __forceinline__ uint2 kvq_codes(float (&x)[8], float scale, float inverse) {
+  if (!(scale > 0.f)) return make_uint2(KVQ_ZERO<FMT>, KVQ_ZERO<FMT>);
+  if (FMT == KVQ_INT8 ? scale > 512.f : scale >= 256.f) {
+    const float top = (FMT == KVQ_INT8 ? 113.f : 240.f) * scale;
 #pragma unroll
-  for (int i = 0; i < 4; i++) q[i] = fminf(fmaxf(__fmul_rn(x[i], inverse), -top), top);
-  if (FMT == KVQ_INT8) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = __float_as_uint(__fadd_rn(__fadd_rn(__fadd_rn(q[i], 1536.f), -1536.f), 12583040.f));
-    return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
+    for (int i = 0; i < 8; i++) x[i] = fminf(fmaxf(x[i], -top), top);
   }
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
-  return lo | hi << 16;
+  if (FMT == KVQ_INT8) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = __float_as_uint(__fadd_rn(fmaf(x[i], inverse, 1536.f), 12583040.f - 1536.f));
+    return make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inverse, x[2 * i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
 }
 
 // Eight halves, four pairs, turned by (cos, sin): products of halves are exact in 32 bits, so each value is rounded there once and
@@ -166,10 +169,8 @@ __device__ __forceinline__ void kvq_quantise(const uint4& k, const uint4& v, uin
   unpack8(k, x);
   unpack8(v, y);
   const float sk = kvq_scale<FMT>(a), sv = kvq_scale<FMT>(b), ik = kvq_inverse<FMT>(sk), iv = kvq_inverse<FMT>(sv);
-  kc.x = kvq_codes<FMT>({x[0], x[1], x[2], x[3]}, sk, ik);
-  kc.y = kvq_codes<FMT>({x[4], x[5], x[6], x[7]}, sk, ik);
-  vc.x = kvq_codes<FMT>({y[0], y[1], y[2], y[3]}, sv, iv);
-  vc.y = kvq_codes<FMT>({y[4], y[5], y[6], y[7]}, sv, iv);
+  kc = kvq_codes<FMT>(x, sk, ik);
+  vc = kvq_codes<FMT>(y, sv, iv);
   scale = __floats2half2_rn(sk, sv);
 }
 #endif

@@ -169,6 +169,24 @@ def test_read(dev, fmt):
 
 
 # ------------------------------------------------------------------------------------------------ one new token a row
+def test_read_many_stretches(dev):
+    """More stretches than a launch has CTAs for at their full length: each goes over its rows in turns."""
+    rng = np.random.default_rng(26)
+    c = Cache(dev, 4, 2, 64, "int8", 16, 1400, 3, rng)
+    c.fill([1400, 900, 50])
+    B, most = 300, 1300
+    pos, seq, count = rng.integers(0, 60, B), rng.integers(0, 3, B), np.where(rng.random(B) < 0.2, most, rng.integers(0, 40, B))
+    first = np.concatenate([[0], np.cumsum(count)[:-1]])
+    k, v = c.kv.read(0, ints(dev, pos), count=ints(dev, count), first=ints(dev, first), seq=ints(dev, seq), max_count=most, rows=int(count.sum()) + 1)
+    k, v = k.numpy().reshape(-1, 2, 64), v.numpy().reshape(-1, 2, 64)
+    for b in range(B):
+        at = slice(first[b], first[b] + count[b])
+        same(k[at], c.k[seq[b], pos[b]:pos[b] + count[b]], f"K of {b}")
+        same(v[at], c.v[seq[b], pos[b]:pos[b] + count[b]], f"V of {b}")
+    assert not k[-1].any() and not v[-1].any()
+    c.close()
+
+
 @pytest.mark.parametrize("fmt", ["int8", "fp8"])
 @pytest.mark.parametrize("H,G,hd", SHAPES)
 def test_decode(dev, H, G, hd, fmt):
