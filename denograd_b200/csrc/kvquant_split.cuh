@@ -5,10 +5,10 @@
 //   out^T [hd x columns] += V^T [hd x 16 positions] . w^T        mma.sync.m16n8k16, 32-bit sums
 // The inner index of a product and the order of its rows are free as long as both operands agree, so a lane's fragments are 16
 // neighbouring codes of a row: of K as they lie, of V two rows at a time with their bytes interleaved.  So a lane loads just what it
-// multiplies, 16 bytes at a time and a tile ahead, straight into registers (32 sequences of 4100 positions of the 8B 67 us; staged in shared
-// memory 81).  V is multiplied by its scale as it is widened (exact), K's scale goes to the finished scores.  The queries' fragments lie in
-// shared memory, each lane's own, which leaves the registers to outputs and tiles (20 columns 26.3 us, 29.5 with them in registers; one
-// column group 67.5, 68.2).
+// multiplies, 16 bytes at a time and a tile ahead, straight into registers (32 sequences of 4100 positions of the 8B, with a call that
+// reads the new rows back, 67 us; staged in shared memory 81).  V is multiplied by its scale as it is widened (exact), K's scale goes to
+// the finished scores.  The queries' fragments lie in shared memory, each lane's own, which leaves the registers to outputs and tiles (20
+// columns 26.3 us, 29.5 with them in registers; one column group 67.5, 68.2).
 //
 // The running maximum is a reference that scores may pass by 2^6 before sums and outputs are rescaled: a vote a tile instead of three
 // rounds of shuffles.
@@ -18,9 +18,10 @@
 // kv head)s; those that others share are left in a workspace (at most two a CTA: its first and its last), and the last to arrive puts them
 // together in order.
 //
-// What bounds it.  32 x 4100 positions, 274 MB: the loops run at about 6 TB/s; 4.5 us pass before them (positions, page, first tiles: three
-// trips through memory), 5 behind (the warps meet, the pieces), and a stretch with two pieces ends 4 us after one with one.  Three column
-// groups run on eight warps an SM, 255 registers each: there latency bounds the loops (3.1 TB/s, issue slots a third full).
+// What bounds it.  32 x 4100 positions, 274 MB: 64 us, 4.3 TB/s as a whole.  The loops run at about 6 TB/s; 4.5 us pass before them
+// (positions, page, first tiles: three trips through memory), 5 behind (the warps meet, the pieces), and a stretch with two pieces ends
+// 4 us after one with one.  Three column groups run on eight warps an SM, 255 registers each: there latency bounds the loops (3.1 TB/s,
+// issue slots 38 % busy).
 #pragma once
 #include "kvquant.cuh"
 
