@@ -32,6 +32,7 @@ constexpr int KC_THREADS = 640, KC_REGS = 96;                                 //
 constexpr int KC_SOFT_REGS = 144, KC_WIDEN_REGS = 72, KC_MMA_REGS = 48;       // and from then on, by warpgroup
 static_assert(2 * KC_SOFT_REGS + 2 * KC_WIDEN_REGS + KC_MMA_REGS <= 5 * KC_REGS, "register shares exceed what a CTA is launched with");
 constexpr int KC_PLAN = 4;  // pieces that the plan is ahead
+constexpr int KC_FEW = 3, KC_BATCH = 4;  // pieces that one CTA adds up; pieces whose loads are in flight together
 constexpr int KC_HALF = KC_KEYS / 2;  // keys of a step of the softmax
 constexpr int KC_WHOLE = 8, KC_SINGLE = 12, KC_GRAIN = 6, KC_FIXED = 2;  // tiles: see the line of tiles
 
@@ -94,6 +95,15 @@ __device__ __forceinline__ float kc_max64(const float* v) {  // in four chains
   t1 = kc_max3(t1, v[62], v[63]);
   return fmaxf(kc_max3(t0, t1, t2), t3);
 }
+// Until as many CTAs have left their pieces: for a converged warp, with a limit.
+__device__ __forceinline__ bool kc_arrived(const unsigned int* ticket, unsigned int pieces) {
+  for (uint32_t i = 0; i < TC_SPIN_LIMIT; i++) {
+    unsigned int n;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(ticket) : "memory");
+    if (__all_sync(0xffffffffu, n >= pieces)) return true;
+  }
+  return false;
+}
 // pairs of floats: packed operands stay in register pairs, made once where they do not change
 __device__ __forceinline__ uint64_t kc_pair(float x, float y) {
   uint64_t r;
@@ -149,6 +159,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2][2], q_full[2], met, plan_full[KC_PLAN], plan_empty[KC_PLAN];
   __shared__ KcPiece s_plan[KC_PLAN];
   __shared__ uint32_t s_tmem;
+  __shared__ KcPiece s_shared[2];
   __shared__ unsigned int s_ticket;
   __shared__ float2 s_ml[2][128];
   __shared__ long long s_sum[KC_THREADS / 32], s_at;
@@ -258,22 +269,27 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         at = s_at;
         entry = s_entry;
       } else {
-        int n = tiles_of(lane);
-        longest = __reduce_max_sync(0xffffffffu, n);
-        int items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
-        // Short items that leave half of the CTAs idle become items of half the rows, whose two streams share their keys (512 new positions of the
+        int items;
+        long long mine, sum;
+        auto look = [&]() {  // at items of this many rows
+          KcPiece p;
+          const int n = lane < a.B * per ? kc_item(a, lane / per, lane % per, rows, p) : 0;
+          longest = __reduce_max_sync(0xffffffffu, n);
+          items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
+          uncut = longest <= (items <= (int)gridDim.x ? KC_SINGLE : KC_WHOLE);
+          single = uncut && items <= (int)gridDim.x;
+          mine = single ? (n > 0 ? a.c.G : 0) : cost(n);
+          sum = scan64(mine);
+          total = __shfl_sync(0xffffffffu, sum, 31);
+        };
+        look();
+        // Items that leave half of the CTAs idle become items of half the rows, whose two streams share their keys (512 new positions of the
         // 8B 16.6 us, 18.7 without); and where each CTA has one at most, they count alike (18.7 us, 19.3 without).
-        uncut = longest <= (items <= (int)gridDim.x ? KC_SINGLE : KC_WHOLE);
-        if (uncut && entries <= 16 && 2 * items <= (int)gridDim.x) {
+        if (entries <= 16 && 2 * (uncut ? items : total / KC_GRAIN) <= (long long)gridDim.x) {
           rows = KC_ROWS / 2;
           per *= 2;
-          KcPiece p;
-          n = lane < a.B * per ? kc_item(a, lane / per, lane % per, rows, p) : 0;
-          items = __popc(__ballot_sync(0xffffffffu, n > 0)) * a.c.G;
+          look();
         }
-        single = uncut && items <= (int)gridDim.x;
-        const long long mine = single ? (n > 0 ? a.c.G : 0) : cost(n), sum = scan64(mine);
-        total = __shfl_sync(0xffffffffu, sum, 31);
         share();
         entry = max(0, __ffs(__ballot_sync(0xffffffffu, sum > u_lo)) - 1);
         at = __shfl_sync(0xffffffffu, sum - mine, entry);
@@ -496,6 +512,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step;
       return at < p.n * a.n_rep && row >= 0 && row < a.R ? row : -1;
     };
+    int shared = 0;  // pieces of items that other CTAs have pieces of
     for (;; planned++) {
       const uint32_t planned_slot = planned % KC_PLAN;
       ok = ok && mbar_wait(&plan_full[planned_slot], (planned / KC_PLAN) & 1);
@@ -688,9 +705,19 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         }
       }
       if (whole) { release(); continue; }
-      // ---- an item that CTAs c_lo .. share: the last to arrive adds its pieces up in this order
+      // ---- a piece of an item that CTAs c_lo .. share.  A few pieces are added up by the last CTA to arrive, in their order; of many every CTA adds
+      // up its share behind all its own work, or one would read them all (2048 positions behind 6001: 231 us, 237 with shares; 45 behind
+      // 16000, 18 pieces of an item: 72 us, 41 with shares).
+      const bool few = p.pieces <= KC_FEW;
+      if (!few && tid == 0) s_shared[shared] = p;
       __threadfence();
       meet();
+      if (!few) {
+        if (tid == 0) atomicAdd(&a.tickets[p.c_lo], 1u);
+        shared++;
+        release();
+        continue;
+      }
       if (tid == 0) {
         s_ticket = atomicAdd(&a.tickets[p.c_lo], 1u);
         if (s_ticket == (unsigned)(p.pieces - 1)) a.tickets[p.c_lo] = 0;
@@ -729,6 +756,65 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       }
       store();
       release();
+    }
+    // ---- shared items, two at most: each CTA adds up its share of the rows, a thread sixteen values at a time, pieces in their order
+    for (int k = 0; k < shared && ok; k++) {
+      const KcPiece& p = s_shared[k];
+      unsigned int* tickets = a.tickets + p.c_lo;  // arrived; and gridDim.x further, done with waiting
+      ok = kc_arrived(tickets, (unsigned)p.pieces);
+      meet();
+      if (!ok) break;
+      if (tid == 0 && atomicAdd(tickets + gridDim.x, 1u) == (unsigned)(p.pieces - 1)) { tickets[0] = 0; tickets[gridDim.x] = 0; }
+      const int units = p.left * (HD / 16), mine = (int)blockIdx.x - p.c_lo, hi = (int)((long long)units * (mine + 1) / p.pieces);
+      for (int u = (int)((long long)units * mine / p.pieces) + tid; u < hi; u += 256) {
+        const int c = u / p.left, at = u - c * p.left;
+        float top = -INFINITY, sum = 0.f, x[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[i] = 0.f;
+#pragma unroll 1
+        for (int from = 0; from < p.pieces; from += KC_BATCH) {
+          float4 y[KC_BATCH][4];
+          float pm[KC_BATCH], pl[KC_BATCH];
+#pragma unroll
+          for (int e = 0; e < KC_BATCH; e++) {
+            const int n = from + e;
+            if (n >= p.pieces) break;
+            const float* src = a.part + (size_t)(2 * (p.c_lo + n) + (n == 0 ? 1 : 0)) * kc_part_floats(HD);
+            pm[e] = __ldcg(src + HD * KC_ROWS + at);
+            pl[e] = __ldcg(src + HD * KC_ROWS + KC_ROWS + at);
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[e][j] = __ldcg(reinterpret_cast<const float4*>(src) + (size_t)(c * 4 + j) * KC_ROWS + at);
+          }
+#pragma unroll
+          for (int e = 0; e < KC_BATCH; e++) {
+            if (from + e >= p.pieces) break;
+            const float then = fmaxf(top, pm[e]), base = then == -INFINITY ? 0.f : then, fade = ft_ex2(top - base), f = ft_ex2(pm[e] - base);
+            top = then;
+            sum = sum * fade + pl[e] * f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              x[4 * j] = x[4 * j] * fade + y[e][j].x * f;
+              x[4 * j + 1] = x[4 * j + 1] * fade + y[e][j].y * f;
+              x[4 * j + 2] = x[4 * j + 2] * fade + y[e][j].z * f;
+              x[4 * j + 3] = x[4 * j + 3] * fade + y[e][j].w * f;
+            }
+          }
+        }
+        const int row_head = p.row0 + at, i = row_head / a.n_rep;
+        const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step;
+        if (row < 0 || row >= a.R) continue;
+        const bool outside = p.bt == nullptr || (long long)p.p0 + i < 0 || (long long)p.p0 + i >= a.c.max_ctx;
+        const float f = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+        uint32_t w[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const __half2 h = __floats2half2_rn(x[2 * j] * f, x[2 * j + 1] * f);
+          w[j] = outside ? 0u : *reinterpret_cast<const uint32_t*>(&h);
+        }
+        uint4* to = reinterpret_cast<uint4*>(a.out + row * a.ldo + (size_t)(p.g * a.n_rep + row_head - i * a.n_rep) * HD + c * 16);
+        to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
     }
     if (!ok && lane == 0) atomicCAS(a.err, 0, 3);
   }
