@@ -11,8 +11,8 @@
 // there.  Tensor memory: S of both streams (P takes its place as 16-bit pairs), O of both.  A row's maximum is a reference that its scores
 // may pass by 2^8 before O is rescaled in tensor memory, which is rare behind the first tiles.
 //
-// The tiles of all items are one line, cut evenly over one CTA for each SM.  An item that several CTAs share meets in a
-// workspace; the last to arrive adds the pieces up in order (3 us for two pieces of 256 x 64, 10 for five of 256 x 128: what one SM reads).
+// The tiles of all items are one line, cut evenly over one CTA for each SM.  An item that several CTAs share meets in a workspace: two
+// pieces are added up by the last CTA to arrive (3 to 4 us), more by all of its CTAs, a share of the rows each; always in their order.
 //
 // What bounds it: per 256 rows x 128 keys x 128 columns four products of 512 cycles at the tensor peak, and 32768 exponentials at 16 a
 // cycle, 2048 cycles either way; such a unit takes 4000.  2048 positions of the 8B behind 6001, fp8: 230 us, 1.02 PFLOP/s.  The tensor pipe
@@ -32,9 +32,9 @@ constexpr int KC_THREADS = 640, KC_REGS = 96;                                 //
 constexpr int KC_SOFT_REGS = 144, KC_WIDEN_REGS = 72, KC_MMA_REGS = 48;       // and from then on, by warpgroup
 static_assert(2 * KC_SOFT_REGS + 2 * KC_WIDEN_REGS + KC_MMA_REGS <= 5 * KC_REGS, "register shares exceed what a CTA is launched with");
 constexpr int KC_PLAN = 4;  // pieces that the plan is ahead
-constexpr int KC_FEW = 3, KC_BATCH = 4;  // pieces that one CTA adds up; pieces whose loads are in flight together
+constexpr int KC_FEW = 2, KC_BATCH = 4;  // pieces that one CTA adds up; pieces whose loads are in flight together
 constexpr int KC_HALF = KC_KEYS / 2;  // keys of a step of the softmax
-constexpr int KC_WHOLE = 8, KC_SINGLE = 12, KC_GRAIN = 6, KC_FIXED = 2;  // tiles: see the line of tiles
+constexpr int KC_WHOLE = 8, KC_SINGLE = 12, KC_GRAIN = 2, KC_FIXED = 2;  // tiles: see the line of tiles
 
 template <int HD>
 struct KcCfg {
@@ -95,7 +95,8 @@ __device__ __forceinline__ float kc_max64(const float* v) {  // in four chains
   t1 = kc_max3(t1, v[62], v[63]);
   return fmaxf(kc_max3(t0, t1, t2), t3);
 }
-// Until as many CTAs have left their pieces: for a converged warp, with a limit.
+// Until as many CTAs have left their pieces: for a converged warp, with a limit.  They all run or have run: a launch has a CTA an SM, its
+// predecessors end by themselves, and its successor starts behind all of them (ft_columns).
 __device__ __forceinline__ bool kc_arrived(const unsigned int* ticket, unsigned int pieces) {
   for (uint32_t i = 0; i < TC_SPIN_LIMIT; i++) {
     unsigned int n;
@@ -200,9 +201,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     return v;
   };
   // An item costs what KC_FIXED tiles do beside its own.  Cutting one costs its CTAs a trip through memory each, 2 to 4 us: short items are
-  // not cut, others not into less than KC_GRAIN tiles.  `uncut`: none is longer than KC_WHOLE tiles, or KC_SINGLE where there is a CTA for each (512 new
-  // positions of the 8B, 4 tiles: cut 33 us, 16.3; 45 behind 1100, 10 tiles, 8 items: 34, 23; 160 items of these: 48, 55; 45 behind
-  // 1900, 16 tiles: 32, 33).
+  // not cut, others not into less than KC_GRAIN tiles (45 new positions of the 8B behind 3000: 2, 3, 4, 6 tiles 20, 21, 21, 30 us).  `uncut`: none is
+  // longer than KC_WHOLE tiles, or KC_SINGLE where there is a CTA for each (a prompt of 900, 8 tiles: cut 37 us, 26; of 1100, 9 tiles and 144
+  // items: 42, 30; 160 items of 10 tiles: 48, 55; 8 items of 10: 20, 23; of 16: 18, 33).
   long long total = 0, u_lo = 0, u_hi = 0;
   int longest = 0, ctas = 1;
   bool uncut = false;
@@ -705,9 +706,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         }
       }
       if (whole) { release(); continue; }
-      // ---- a piece of an item that CTAs c_lo .. share.  A few pieces are added up by the last CTA to arrive, in their order; of many every CTA adds
-      // up its share behind all its own work, or one would read them all (2048 positions behind 6001: 231 us, 237 with shares; 45 behind
-      // 16000, 18 pieces of an item: 72 us, 41 with shares).
+      // ---- a piece of an item that CTAs c_lo .. share.  Two pieces are added up by the last CTA to arrive; of more every CTA adds up its share
+      // behind all its own work, or one would read them all (2048 positions behind 6001, two pieces: 231 us, 237 with shares; 45 behind
+      // 1900, three: 28, 24; behind 16000, 18: 72, 41).
       const bool few = p.pieces <= KC_FEW;
       if (!few && tid == 0) s_shared[shared] = p;
       __threadfence();

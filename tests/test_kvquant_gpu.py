@@ -316,6 +316,16 @@ def test_attend_prompts(dev, H, G, hd, new, ahead):
     c.close()
 
 
+# Few rows behind long contexts: an item is cut into 2, 3 and many pieces, with rows left over, empty sequences among them, several on a CTA
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("H,G,hd,new,ahead", [(4, 1, 64, [9], 1900), (4, 1, 128, [45], 6000), (8, 1, 64, [45, 0, 33], 3100), (12, 4, 128, [50, 1], 2500), (3, 1, 64, [77], 12345),
+                                              (16, 2, 128, [31, 40, 32], 4000)])
+def test_attend_pieces(dev, H, G, hd, new, ahead, fmt):
+    c = Cache(dev, H, G, hd, fmt, 32, ahead + max(new), len(new) + 1, np.random.default_rng(27))
+    attend(c, [ahead - 611 * b for b in range(len(new))], new, False, seed=16)
+    c.close()
+
+
 @pytest.mark.parametrize("most", [3, 40])  # short chunks and long ones have kernels of their own
 def test_attend_rows_outside(dev, most):
     rng = np.random.default_rng(10)
