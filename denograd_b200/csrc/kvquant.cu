@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(KR_THREADS) kvq_read_kernel(const KvqReadArgs 
 template <int FMT, int HD>
 static int launch_read(jg_dev* dev, const KvqReadArgs& a, int B) {
   const unsigned long long per_row = (unsigned long long)a.c.G * (HD / 8), ctas = ((a.max_count + KR_ROWS - 1) / KR_ROWS * per_row + KR_THREADS - 1) / KR_THREADS;
-  const unsigned long long most = (20ull * dev->sm_count + B - 1) / B;  // CTAs: a ragged batch has many without rows (5, 10, 20 an SM, one each: 14.9, 12.3, 10.3, 11.4 us)
+  // A ragged batch has many CTAs without rows: 5, 10, 20 an SM, and one for each piece 14.9, 12.3, 10.3, 11.4 us.
+  const unsigned long long most = (20ull * dev->sm_count + B - 1) / B;
   return jg_launch(dev, "kvq_read", kvq_read_kernel<FMT, HD>, dim3((unsigned)(ctas < most ? ctas : most), (unsigned)B), dim3(KR_THREADS), 0, a);
 }
 
@@ -291,8 +292,8 @@ JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint6
   JG_REQUIRE(kv != nullptr && kv->dev == dev, "kvq_read: cache belongs to another device");
   JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_read: layer %d out of range", layer);
   const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
-  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && step > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
-             max_count, R, kv->d.max_batch);
+  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && step > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch),
+             "kvq_read: B=%d sequences of up to %d positions, R=%d rows, %d slots", B, max_count, R, kv->d.max_batch);
   JG_REQUIRE(ld >= G * hd && ld % 8 == 0, "kvq_read: rows of %d elements are no multiple of 8 or too short", ld);
   JG_REQUIRE(jg_aligned(k, 16) && jg_aligned(v, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_read: null or misaligned pointer");
   const unsigned long long pieces = (unsigned long long)max_count * G * (hd / 8);

@@ -38,8 +38,8 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   JG_REQUIRE(layer >= 0 && layer < kv->d.n_layers, "kvq_attn: layer %d out of range", layer);
   const int G = kv->d.n_kv_heads, hd = kv->d.head_dim;
   JG_REQUIRE(H == kv->d.n_heads, "kvq_attn: H=%d does not match the cache (n_heads %d)", H, kv->d.n_heads);
-  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && step > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch), "kvq_attn: B=%d sequences of up to %d positions, R=%d rows, %d slots", B,
-             max_count, R, kv->d.max_batch);
+  JG_REQUIRE(R > 0 && max_count > 0 && max_count <= kv->max_ctx && step > 0 && B > 0 && B <= 65535 && (seq != 0 || B <= kv->d.max_batch),
+             "kvq_attn: B=%d sequences of up to %d positions, R=%d rows, %d slots", B, max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
   // Few columns are read at HBM's pace or near it: 8 sequences behind 3001 positions of the 8B, 16 columns 21.3 us (the tensor cores' form 38), 20

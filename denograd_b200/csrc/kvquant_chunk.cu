@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
   unsigned char* sQ = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(kc_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* sK = sQ + 2 * Cfg::Q_BYTES;
   unsigned char* sV = sK + 2 * Cfg::KV_BYTES;
-  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2][2], q_full[2], met, plan_full[KC_PLAN], plan_empty[KC_PLAN];
+  __shared__ __align__(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], o_full[2][2], q_full[2], met;
+  __shared__ __align__(8) uint64_t plan_full[KC_PLAN], plan_empty[KC_PLAN];
   __shared__ KcPiece s_plan[KC_PLAN];
   __shared__ uint32_t s_tmem;
   __shared__ KcPiece s_shared[2];

@@ -471,7 +471,8 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         return s_ticket == (unsigned)(of - 1);
       };
       auto piece = [&](int p) -> float* { return a.part + (size_t)(2 * (c_lo + p) + (p == 0 ? 1 : 0)) * Cfg::PART; };
-      constexpr int NI = COLS * HD / (KS_THREADS * 4), BATCH = NI > 2 ? 2 : NI > 1 ? 4 : 8;  // groups of four values of a thread; pieces whose loads are in flight together
+      // groups of four values of a thread; pieces whose loads are in flight together
+      constexpr int NI = COLS * HD / (KS_THREADS * 4), BATCH = NI > 2 ? 2 : NI > 1 ? 4 : 8;
       float x[NI][4], top[NI], sum[NI];
       auto add_up = [&](int from, int to, int step) {
 #pragma unroll

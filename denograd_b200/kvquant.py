@@ -76,6 +76,7 @@ class QuantKVCache:
         ffi.call("jg_kvq_set_block_table", self.handle, table.ctypes.data_as(C.c_void_p))
 
     def nbytes(self) -> int:
+        """Of codes, scales and block table."""
         out = C.c_uint64(0)
         ffi.call("jg_kvq_bytes", self.handle, C.byref(out))
         return out.value

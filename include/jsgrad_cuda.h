@@ -307,7 +307,7 @@ typedef struct jg_kvq jg_kvq; /* paged 8-bit K/V pool of one model on one device
 int jg_kvq_create(jg_dev* dev, const jg_kvcache_desc* desc, int32_t format, jg_kvq** out);
 int jg_kvq_destroy(jg_kvq* kv);
 int jg_kvq_set_block_table(jg_kvq* kv, const int32_t* table); /* as jg_kvcache_set_block_table */
-int jg_kvq_bytes(jg_kvq* kv, uint64_t* out);
+int jg_kvq_bytes(jg_kvq* kv, uint64_t* out); /* codes, scales and block table; the first cache of a device also makes a workspace for all (39 MB) */
 /* apply_rotary_emb on Q and K + cache assignment (jsgrad/models/llama.ts:23-32,87) for R independent rows: row r of qkv, wq|wk|wv outputs
  * [(H + 2G) * hd], has position pos[r] of slot seq[r] (0: row r is slot r).  Q and K are rotated in 32 bits and rounded to fp16 once;
  * rotated Q goes to q_out (0: nowhere; qkv itself: in place), K and V into the cache.  table = 0: nothing is rotated.
