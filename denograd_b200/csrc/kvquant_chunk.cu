@@ -34,7 +34,6 @@ static_assert(2 * KC_SOFT_REGS + 2 * KC_WIDEN_REGS + KC_MMA_REGS <= 5 * KC_REGS,
 constexpr int KC_PLAN = 4;  // pieces that the plan is ahead
 constexpr int KC_FEW = 2, KC_BATCH = 4;  // pieces that one CTA adds up; pieces whose loads are in flight together
 constexpr int KC_HALF = KC_KEYS / 2;  // keys of a step of the softmax
-constexpr int KC_WHOLE = 8, KC_SINGLE = 12, KC_GRAIN = 2, KC_FIXED = 2;  // tiles: see the line of tiles
 
 template <int HD>
 struct KcCfg {
@@ -212,13 +211,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     const long long most = uncut ? total : total / KC_GRAIN;
     ctas = (int)max(1ll, min((long long)gridDim.x, most));
     if ((int)blockIdx.x >= ctas) return;
-    if (total < (1 << 23)) {  // 512 CTAs at most: see the launch
-      u_lo = blockIdx.x * (uint32_t)total / (uint32_t)ctas;
-      u_hi = (blockIdx.x + 1) * (uint32_t)total / (uint32_t)ctas;
-    } else {
-      u_lo = blockIdx.x * total / ctas;
-      u_hi = (blockIdx.x + 1) * total / ctas;
-    }
+    u_lo = kvq_cut<KC_BITS>(total, ctas, blockIdx.x);  // 512 CTAs at most: see the launch
+    u_hi = kvq_cut<KC_BITS>(total, ctas, blockIdx.x + 1);
   };
   if (entries > 32) {
     for (int e = tid; e < entries; e += KC_THREADS) {
@@ -331,8 +325,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           p.c_lo = p.pieces = 0;
           if (p.j1 - p.j0 < n) {
             const long long begin = item + KC_FIXED;
-            p.c_lo = (int)(((begin + 1) * ctas - 1) / total);
-            p.pieces = (int)(((begin + n) * ctas - 1) / total) - p.c_lo + 1;
+            p.c_lo = kvq_owner(total, ctas, begin);
+            p.pieces = kvq_owner(total, ctas, begin + n - 1) - p.c_lo + 1;
           }
           break;
         }
@@ -655,7 +649,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       };
       // ---- the result, or a piece of it
       const bool whole = p.j1 - p.j0 == p.n_tiles;
-      float* part = a.part + (size_t)(2 * blockIdx.x + (p.j0 == 0 ? 1 : 0)) * kc_part_floats(HD);  // [hd / 4][256][4], maxima, sums
+      float* part = a.part + (size_t)kvq_slot(blockIdx.x, p.j0 == 0) * kc_part_floats(HD);  // [hd / 4][256][4], maxima, sums
       int head, i;
       const long long row = row_of(p, head, i), to = row < 0 ? -1 : row * a.ldo + head * HD;
       const bool outside = p.bt == nullptr || (long long)p.p0 + i < 0 || (long long)p.p0 + i >= a.c.max_ctx;
@@ -715,19 +709,19 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       __threadfence();
       meet();
       if (!few) {
-        if (tid == 0) atomicAdd(&a.tickets[p.c_lo], 1u);
+        if (tid == 0) atomicAdd(&a.tickets[kc_ticket(p.c_lo)], 1u);
         shared++;
         release();
         continue;
       }
       if (tid == 0) {
-        s_ticket = atomicAdd(&a.tickets[p.c_lo], 1u);
-        if (s_ticket == (unsigned)(p.pieces - 1)) a.tickets[p.c_lo] = 0;
+        s_ticket = atomicAdd(&a.tickets[kc_ticket(p.c_lo)], 1u);
+        if (s_ticket == (unsigned)(p.pieces - 1)) a.tickets[kc_ticket(p.c_lo)] = 0;
       }
       meet();
       if (s_ticket != (unsigned)(p.pieces - 1) || idle || absent || !ok) { release(); continue; }
       __threadfence();
-      auto piece = [&](int k) -> const float* { return a.part + (size_t)(2 * (p.c_lo + k) + (k == 0 ? 1 : 0)) * kc_part_floats(HD); };
+      auto piece = [&](int k) -> const float* { return a.part + (size_t)kvq_slot(p.c_lo + k, k == 0) * kc_part_floats(HD); };
       float top = -INFINITY;
 #pragma unroll 4
       for (int k = 0; k < p.pieces; k++) top = fmaxf(top, __ldcg(piece(k) + HD * KC_ROWS + at));
@@ -762,11 +756,11 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     // ---- shared items, two at most: each CTA adds up its share of the rows, a thread sixteen values at a time, pieces in their order
     for (int k = 0; k < shared && ok; k++) {
       const KcPiece& p = s_shared[k];
-      unsigned int* tickets = a.tickets + p.c_lo;  // arrived; and gridDim.x further, done with waiting
-      ok = kc_arrived(tickets, (unsigned)p.pieces);
+      unsigned int *arrived = a.tickets + kc_ticket(p.c_lo), *done = a.tickets + kc_done_ticket(gridDim.x, p.c_lo);
+      ok = kc_arrived(arrived, (unsigned)p.pieces);
       meet();
       if (!ok) break;
-      if (tid == 0 && atomicAdd(tickets + gridDim.x, 1u) == (unsigned)(p.pieces - 1)) { tickets[0] = 0; tickets[gridDim.x] = 0; }
+      if (tid == 0 && atomicAdd(done, 1u) == (unsigned)(p.pieces - 1)) { *arrived = 0; *done = 0; }
       const int units = p.left * (HD / 16), mine = (int)blockIdx.x - p.c_lo, hi = (int)((long long)units * (mine + 1) / p.pieces);
       for (int u = (int)((long long)units * mine / p.pieces) + tid; u < hi; u += 256) {
         const int c = u / p.left, at = u - c * p.left;
@@ -781,7 +775,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           for (int e = 0; e < KC_BATCH; e++) {
             const int n = from + e;
             if (n >= p.pieces) break;
-            const float* src = a.part + (size_t)(2 * (p.c_lo + n) + (n == 0 ? 1 : 0)) * kc_part_floats(HD);
+            const float* src = a.part + (size_t)kvq_slot(p.c_lo + n, n == 0) * kc_part_floats(HD);
             pm[e] = __ldcg(src + HD * KC_ROWS + at);
             pl[e] = __ldcg(src + HD * KC_ROWS + KC_ROWS + at);
 #pragma unroll

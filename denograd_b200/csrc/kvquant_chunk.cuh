@@ -1,6 +1,7 @@
 // The tensor-core form of attention over the 8-bit cache: its arguments and the size of its workspace (kvquant_chunk.cu).
 #pragma once
 #include "kvquant.cuh"
+#include "kvquant_line.h"
 
 struct KvqChunkArgs {
   KvqLayer c;
@@ -18,7 +19,6 @@ struct KvqChunkArgs {
   int* err;
 };
 
-constexpr int KC_ROWS = 256, KC_KEYS = 128;  // query rows of an item, keys of a tile
 static inline int kc_ctas(const jg_dev* dev) { return dev->sm_count < 512 ? dev->sm_count : 512; }
 static inline int kc_slots(const jg_dev* dev) { return 2 * kc_ctas(dev); }  // pieces in the workspace
 __host__ __device__ constexpr size_t kc_part_floats(int hd) { return (size_t)KC_ROWS * (hd + 2); }  // outputs, maxima, sums

@@ -24,6 +24,7 @@
 // issue slots 38 % busy).
 #pragma once
 #include "kvquant.cuh"
+#include "kvquant_line.h"
 
 struct KvqSplitArgs {
   KvqLayer c;
@@ -40,8 +41,7 @@ struct KvqSplitArgs {
   unsigned int* tickets;                                 // [2 * CTAs], zero between launches
 };
 
-constexpr int KS_WARPS = 4, KS_THREADS = 32 * KS_WARPS, KS_UNIT = 16 * KS_WARPS, KS_CTAS = 3;  // CTAs to an SM
-constexpr int KS_GROUP = 8;  // pieces that are added up ahead of the others, where there are many
+constexpr int KS_THREADS = 32 * KS_WARPS, KS_CTAS = 3;  // CTAs to an SM
 
 template <int HD, int NT>
 struct KsCfg {
@@ -50,9 +50,7 @@ struct KsCfg {
   static constexpr size_t Q_BYTES = NT * KJ * 1024;             // a warp's fragments of q
   static constexpr size_t MERGE = KS_WARPS * COLS * HD * 4;     // the warps' outputs when they meet, in the place of these
   static constexpr int PART = COLS * (HD + 2);                  // floats of a piece: outputs, maxima, sums
-  // Units that a (sequence, kv head) costs beside its own.  One column group: 1, 3 and 6 within 1 %; more: 8 sequences of 5 positions behind 3001 of the
-  // 8B 30.9 us with 3, 29.5 with 5, 29.8 with 7 (30 ragged ones 25.5, 25.3, 27.1).
-  static constexpr int FIXED = NT == 1 ? 3 : 5;
+  static constexpr int FIXED = ks_fixed(NT);
 };
 
 #ifdef __CUDACC__
@@ -119,14 +117,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
   total *= a.c.G;
   const long long ctas = min((long long)gridDim.x, total);
   if (blockIdx.x >= ctas) return;
-  long long u_lo, u_hi;
-  if (total < (1 << 20)) {  // up to 4096 CTAs
-    u_lo = blockIdx.x * (uint32_t)total / (uint32_t)ctas;
-    u_hi = (blockIdx.x + 1) * (uint32_t)total / (uint32_t)ctas;
-  } else {
-    u_lo = blockIdx.x * total / ctas;
-    u_hi = (blockIdx.x + 1) * total / ctas;
-  }
+  const long long u_lo = kvq_cut<KS_BITS>(total, ctas, blockIdx.x), u_hi = kvq_cut<KS_BITS>(total, ctas, blockIdx.x + 1);
   int b = 0;
   long long at = 0;  // first unit of (b, head 0)
   for (int base = 0;; base += 32) {
@@ -415,7 +406,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         }
       __syncthreads();
       const bool whole = j0 == 0 && j1 == n_units;
-      float* part = whole ? nullptr : a.part + (size_t)(2 * blockIdx.x + (j0 == 0 ? 1 : 0)) * Cfg::PART;
+      float* part = whole ? nullptr : a.part + (size_t)kvq_slot(blockIdx.x, j0 == 0) * Cfg::PART;
       auto store = [&](int idx, const float (&x)[4]) {  // four finished values of a column
         const int col = idx / HD, i = col / a.n_rep;
         const long long row = row0 + (long long)i * a.step;
@@ -455,10 +446,10 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         }
       }
       if (whole) { __syncthreads(); continue; }
-      // ---- pieces of a (sequence, kv head) that CTAs c_lo .. c_hi share: the last to arrive adds them up in this order.  Many are added up in
+      // ---- pieces of a (sequence, kv head) that several CTAs, from c_lo on, share: the last to arrive adds them up in this order.  Many are added up in
       // groups of neighbours first, as these are done: one CTA reads 30 pieces in 10 us.
       const long long begin = item + Cfg::FIXED, last = begin + n_units - 1;
-      const int c_lo = (int)(((begin + 1) * ctas - 1) / total), c_hi = (int)(((last + 1) * ctas - 1) / total), pieces = c_hi - c_lo + 1;
+      const int c_lo = kvq_owner(total, ctas, begin), pieces = kvq_owner(total, ctas, last) - c_lo + 1;
       auto arrive = [&](unsigned int* ticket, int of) -> bool {  // whether this CTA is the last
         __syncthreads();
         if (tid == 0) {
@@ -470,7 +461,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         __syncthreads();
         return s_ticket == (unsigned)(of - 1);
       };
-      auto piece = [&](int p) -> float* { return a.part + (size_t)(2 * (c_lo + p) + (p == 0 ? 1 : 0)) * Cfg::PART; };
+      auto piece = [&](int p) -> float* { return a.part + (size_t)kvq_slot(c_lo + p, p == 0) * Cfg::PART; };
       // groups of four values of a thread; pieces whose loads are in flight together
       constexpr int NI = COLS * HD / (KS_THREADS * 4), BATCH = NI > 2 ? 2 : NI > 1 ? 4 : 8;
       float x[NI][4], top[NI], sum[NI];
@@ -507,14 +498,12 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
             }
         }
       };
-      int step = 1;
-      if (pieces > KS_GROUP + KS_GROUP / 2) {
-        step = KS_GROUP;
-        const int from = ((int)blockIdx.x - c_lo) / KS_GROUP * KS_GROUP, to = min(from + KS_GROUP, pieces);
-        if (!arrive(&a.tickets[c_lo + from], to - from)) continue;
-        add_up(from, to, 1);
+      const KsGroup group = ks_group((int)blockIdx.x - c_lo, pieces, c_lo);
+      if (group.ticket >= 0) {
+        if (!arrive(&a.tickets[group.ticket], group.to - group.from)) continue;
+        add_up(group.from, group.to, 1);
         __syncthreads();  // all have read what is written over now
-        float* dst = piece(from);
+        float* dst = piece(group.from);
 #pragma unroll
         for (int e = 0; e < NI; e++) {
           const int idx = (tid + e * KS_THREADS) * 4;
@@ -522,8 +511,8 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
           if (idx % HD == 0) { __stcg(dst + COLS * HD + idx / HD, top[e]); __stcg(dst + COLS * HD + COLS + idx / HD, sum[e]); }
         }
       }
-      if (!arrive(&a.tickets[gridDim.x + c_lo], (pieces + step - 1) / step)) continue;
-      add_up(0, pieces, step);
+      if (!arrive(&a.tickets[ks_last_ticket(gridDim.x, c_lo)], ks_groups(pieces, group.step))) continue;
+      add_up(0, pieces, group.step);
 #pragma unroll
       for (int e = 0; e < NI; e++) {
         const float inv = sum[e] == 0.f ? 0.f : __fdiv_rn(1.f, sum[e]);
