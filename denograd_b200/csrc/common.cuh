@@ -144,6 +144,24 @@ static inline int jg_launch(jg_dev* dev, const char* name, void (*kern)(KArgs...
                             Args... args) {
   return jg_launch_cluster(dev, name, kern, grid, block, smem, 1, args...);
 }
+// A kernel whose CTAs wait for one another: a cooperative launch, which begins when all of them can run at once, whatever another stream (another
+// handle on the same GPU) has in flight.  It begins behind its predecessor; its successor may begin early.
+template <typename... KArgs, typename... Args>
+static inline int jg_launch_together(jg_dev* dev, const char* name, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = dev->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, KArgs(args)...);
+  if (e != cudaSuccess) return jg_cuda_fail(e, name, __FILE__, __LINE__);
+  return jg_after_launch(dev, name);
+}
 #endif
 
 // ------------------------------------------------------------------------------------------------ device side

@@ -94,8 +94,8 @@ __device__ __forceinline__ float kc_max64(const float* v) {  // in four chains
   t1 = kc_max3(t1, v[62], v[63]);
   return fmaxf(kc_max3(t0, t1, t2), t3);
 }
-// Until as many CTAs have left their pieces: for a converged warp, with a limit.  They all run or have run: a launch has a CTA an SM, its
-// predecessors end by themselves, and its successor starts behind all of them (ft_columns).
+// Until as many CTAs have left their pieces: for a converged warp, with a limit.  They all run or have run: the launch is a cooperative one, and
+// none of its CTAs waits for anything outside it.
 __device__ __forceinline__ bool kc_arrived(const unsigned int* ticket, unsigned int pieces) {
   for (uint32_t i = 0; i < TC_SPIN_LIMIT; i++) {
     unsigned int n;
@@ -177,7 +177,6 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   const uint32_t tmem = ft_columns(&s_tmem, warp == 16);
-  pdl_wait();
 
   // ---- the line of tiles: how long it is, and where this CTA's stretch begins.  Entry e = (sequence, item of it), all kv heads.  Up to 32
   // entries are the plan's own business; more are looked at by all threads.
@@ -837,7 +836,7 @@ static int launch_chunk(jg_dev* dev, const KvqChunkArgs& a) {
     ready[dev->ordinal & 7] = true;
   }
   dev->tc_pending = true;
-  return jg_launch(dev, "kvq_attn", kern, dim3((unsigned)kc_ctas(dev)), dim3(KC_THREADS), KcCfg<HD>::SMEM, a);
+  return jg_launch_together(dev, "kvq_attn", kern, dim3((unsigned)kc_ctas(dev)), dim3(KC_THREADS), KcCfg<HD>::SMEM, a);
 }
 
 int kvq_chunk(jg_dev* dev, int format, int hd, const KvqChunkArgs& a) {

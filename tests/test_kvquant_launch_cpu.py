@@ -1,0 +1,84 @@
+"""How the kernels of the 8-bit KV cache are launched, and what the library remembers of it: kvquant*.cu over a stand-in for the CUDA runtime that
+launches nothing and writes down what it was asked for."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+from denograd_b200 import build as B
+from denograd_b200 import ffi
+from tests.test_kvquant_cpu import CALLS, HOOKS, LAUNCHES, desc
+from tests.util import ROOT
+
+ATTRIBUTES = """
+#include <cuda_runtime_api.h>
+extern "C" {
+__attribute__((visibility("default"))) int fake_cooperative = 0, fake_early = 0, fake_grid = 0;  // of the last launch
+cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t* c, const void*, void**) {
+  fake_launches++;
+  fake_cooperative = fake_early = 0;
+  fake_grid = (int)(c->gridDim.x * c->gridDim.y * c->gridDim.z);
+  for (unsigned i = 0; i < c->numAttrs; i++) {
+    if (c->attrs[i].id == cudaLaunchAttributeCooperative) fake_cooperative = c->attrs[i].val.cooperative;
+    if (c->attrs[i].id == cudaLaunchAttributeProgrammaticStreamSerialization) fake_early = c->attrs[i].val.programmaticStreamSerializationAllowed;
+  }
+  return cudaSuccess;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    d = tmp_path_factory.mktemp("fake")
+    (d / "hooks.cu").write_text(HOOKS)
+    plain = "cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t*, const void*, void**) { fake_launches++; return cudaSuccess; }\n"
+    head, rest = LAUNCHES.split(plain)
+    counter = head.split('extern "C" {\n')[1]
+    (d / "launches.cpp").write_text(ATTRIBUTES.replace('extern "C" {\n', 'extern "C" {\n' + counter) + rest)
+    so = str(d / "libfake.so")
+    kvq = sorted(f for f in os.listdir(B.CSRC) if f.startswith("kvquant") and f.endswith(".cu"))
+    subprocess.run([B.nvcc(), *B.ARCH, *B.FLAGS, "-I", B.CSRC, "-cudart", "none", "-shared", "-o", so, str(d / "hooks.cu"), str(d / "launches.cpp"),
+                    os.path.join(ROOT, "tests", "fake_cudart.cpp"), os.path.join(B.CSRC, "device.cu"), *[os.path.join(B.CSRC, f) for f in kvq]], check=True)
+    lib = C.CDLL(so)
+    for name, args in ffi.SIGNATURES.items():
+        if name.startswith(("jg_kvq_", "jg_device_", "jg_graph_")):
+            getattr(lib, name).argtypes = args
+    lib.jg_last_error.restype = C.c_char_p
+    return lib
+
+
+@pytest.fixture
+def dev(lib):
+    h = C.c_void_p()
+    assert lib.jg_device_open(0, C.byref(h)) == 0
+    return h
+
+
+@pytest.fixture
+def kv(lib, dev):
+    h = C.c_void_p()
+    assert lib.jg_kvq_create(dev, C.byref(desc()), ffi.KVQ_INT8, C.byref(h)) == 0
+    yield h
+    assert lib.jg_kvq_destroy(h) == 0
+
+
+def last(lib, what):
+    return C.c_int.in_dll(lib, "fake_" + what).value
+
+
+@pytest.mark.parametrize("fmt", [ffi.KVQ_INT8, ffi.KVQ_E4M3])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_ctas_that_wait_for_one_another_run_at_once(lib, dev, fmt, head_dim):
+    """The pieces of a long item are added up by all its CTAs, each of which waits for the others': without a cooperative launch two handles' launches
+    on one GPU could each have half of the SMs and wait for the other half."""
+    h = C.c_void_p()
+    assert lib.jg_kvq_create(dev, C.byref(desc(head_dim=head_dim)), fmt, C.byref(h)) == 0
+    width = 8 * head_dim
+    many = dict(CALLS["attn"][0], max_count=60, ldo=width, ldq=width)
+    assert lib.jg_kvq_attn(dev, h, *many.values()) == 0
+    assert last(lib, "cooperative") == 1 and last(lib, "early") == 0
+    few = dict(many, max_count=1)
+    assert lib.jg_kvq_attn(dev, h, *few.values()) == 0
+    assert last(lib, "cooperative") == 0 and last(lib, "early") == 1  # nobody waits there
+    assert lib.jg_kvq_destroy(h) == 0
