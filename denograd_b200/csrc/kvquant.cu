@@ -203,6 +203,7 @@ JG_API int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, 
   a.q_out = (__half*)q_out; a.qkv = (const __half*)qkv; a.table = (const __half*)table;
   a.pos = (const int32_t*)pos; a.seq = (const int32_t*)seq;
   a.ldq = ldq; a.ldx = ldx; a.table_rows = table_rows; a.R = R; a.H = H;
+  if (q_out) jg_mark_fresh(dev, q_out, (uint64_t)R * ldq * 2);  // what is written may be the next call's weight matrix, here and below
   if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_write<KVQ_INT8, 64>(dev, a) : launch_write<KVQ_INT8, 128>(dev, a);
   return hd == 64 ? launch_write<KVQ_E4M3, 64>(dev, a) : launch_write<KVQ_E4M3, 128>(dev, a);
 }
@@ -303,6 +304,8 @@ JG_API int jg_kvq_read(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t k, uint6
   a.k = (__half*)k; a.v = (__half*)v;
   a.pos = (const int32_t*)pos; a.count = (const int32_t*)count; a.first = (const int32_t*)first; a.seq = (const int32_t*)seq;
   a.ld = ld; a.R = R; a.max_count = max_count; a.step = step;
+  jg_mark_fresh(dev, k, (uint64_t)R * ld * 2);
+  jg_mark_fresh(dev, v, (uint64_t)R * ld * 2);
   if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_read<KVQ_INT8, 64>(dev, a, B) : launch_read<KVQ_INT8, 128>(dev, a, B);
   return hd == 64 ? launch_read<KVQ_E4M3, 64>(dev, a, B) : launch_read<KVQ_E4M3, 128>(dev, a, B);
 }

@@ -27,6 +27,7 @@ JG_API int jg_kvq_decode(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, i
   a.limit = table && table_rows < kv->max_ctx ? table_rows : kv->max_ctx;
   a.scale2 = (float)(1.4426950408889634 / sqrt((double)hd));
   a.part = dev->kvq_part; a.tickets = dev->kvq_tickets;
+  jg_mark_fresh(dev, out, (uint64_t)B * ldo * 2);  // may be the next call's weight matrix
   if (kv->format == JG_KVQ_INT8) return hd == 64 ? launch_split<KVQ_INT8, 64, 1, true>(dev, a) : launch_split<KVQ_INT8, 128, 1, true>(dev, a);
   return hd == 64 ? launch_split<KVQ_E4M3, 64, 1, true>(dev, a) : launch_split<KVQ_E4M3, 128, 1, true>(dev, a);
 }
@@ -42,6 +43,7 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
              "kvq_attn: B=%d sequences of up to %d positions, R=%d rows, %d slots", B, max_count, R, kv->d.max_batch);
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
+  jg_mark_fresh(dev, out, (uint64_t)R * ldo * 2);
   // Few columns are read at HBM's pace or near it: 8 sequences behind 3001 positions of the 8B, 16 columns 21.3 us (the tensor cores' form 38), 20
   // columns 26.3 (38), 32 sequences of these 71 (93); 24 sequences behind 4000 of the 1B, 28 columns 54 (67).  A lane's outputs have to fit its
   // registers: 32 columns of 128 values would take 42 us, against 38.

@@ -11,6 +11,9 @@ from denograd_b200 import ffi
 from tests.test_kvquant_cpu import CALLS, HOOKS, LAUNCHES, desc
 from tests.util import ROOT
 
+FRESH = """
+extern "C" __attribute__((visibility("default"))) int fake_is_fresh(jg_dev* dev, uint64_t p) { return jg_is_fresh(dev, (const void*)p); }
+"""
 ATTRIBUTES = """
 #include <cuda_runtime_api.h>
 extern "C" {
@@ -31,7 +34,7 @@ cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t* c, const void*, void**
 @pytest.fixture(scope="module")
 def lib(tmp_path_factory):
     d = tmp_path_factory.mktemp("fake")
-    (d / "hooks.cu").write_text(HOOKS)
+    (d / "hooks.cu").write_text(HOOKS + FRESH)
     plain = "cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t*, const void*, void**) { fake_launches++; return cudaSuccess; }\n"
     head, rest = LAUNCHES.split(plain)
     counter = head.split('extern "C" {\n')[1]
@@ -45,6 +48,7 @@ def lib(tmp_path_factory):
         if name.startswith(("jg_kvq_", "jg_device_", "jg_graph_")):
             getattr(lib, name).argtypes = args
     lib.jg_last_error.restype = C.c_char_p
+    lib.fake_is_fresh.argtypes = [C.c_void_p, C.c_uint64]
     return lib
 
 
@@ -82,3 +86,21 @@ def test_ctas_that_wait_for_one_another_run_at_once(lib, dev, fmt, head_dim):
     assert lib.jg_kvq_attn(dev, h, *few.values()) == 0
     assert last(lib, "cooperative") == 0 and last(lib, "early") == 1  # nobody waits there
     assert lib.jg_kvq_destroy(h) == 0
+
+
+# a call, its arguments in place of the usual ones, and what it writes: (argument, bytes)
+@pytest.mark.parametrize("name,args,written", [
+    ("write", dict(q_out=1 << 20, ldq=520, R=5), [("q_out", 5 * 520 * 2)]), ("write", dict(q_out=0, ldq=0), []), ("decode", dict(out=1 << 20, ldo=520, B=5), [("out", 5 * 520 * 2)]),
+    ("attn", dict(out=1 << 20, ldo=512, R=20), [("out", 20 * 512 * 2)]), ("attn", dict(out=1 << 20, ldo=512, R=200, max_count=60), [("out", 200 * 512 * 2)]),
+    ("read", dict(k=1 << 20, v=1 << 24, ld=136, R=20), [("k", 20 * 136 * 2), ("v", 20 * 136 * 2)])])
+def test_what_is_written_is_no_weight_to_read_early(lib, dev, kv, name, args, written):
+    """Projections ask for their weights ahead of their dependency, but not for a matrix that the launches in front of them write: K and V as they are read
+    back, say, whose product with queries is the next call."""
+    args = dict(CALLS[name][0], **args)
+    assert getattr(lib, f"jg_kvq_{name}")(dev, kv, *args.values()) == 0, lib.jg_last_error()
+    for what, n in written:
+        at = args[what]
+        assert [lib.fake_is_fresh(dev, p) for p in (at - 2, at, at + n // 2, at + n - 2, at + n)] == [0, 1, 1, 1, 0]
+    assert not lib.fake_is_fresh(dev, 1 << 28) and not lib.fake_is_fresh(dev, CALLS[name][0]["pos"])
+    assert lib.jg_device_sync(dev) == 0
+    assert not any(lib.fake_is_fresh(dev, args[what]) for what, _ in written)

@@ -1,5 +1,6 @@
 """Sums of the 8-bit cache's attention that many CTAs share, on the GPU: contexts whose items lie so that one CTA has the last piece of an item, a group by
-itself, and the first piece of the next one (tests/kvquant_line_walk.cpp lists them).  Every call gives the same bits, whatever ran before it."""
+itself, and the first piece of the next one (tests/kvquant_line_walk.cpp lists them).  Every call gives the same bits, whatever ran before it.
+And rows that are read back and then taken as weights."""
 import numpy as np
 import pytest
 
@@ -51,3 +52,27 @@ def test_neighbouring_items_of_many_pieces(dev, H, G, hd, ahead, new, fmt):
     c.check_stored()
     c.close()
     other.close()
+
+
+@pytest.mark.parametrize("M", [1, 4, 16, 200])
+def test_rows_read_back_are_the_next_projection(dev, M):
+    """q.K^T as a projection whose weights are the K rows of the call in front of it: those of this turn, not of the last one."""
+    rng = np.random.default_rng(33)
+    hd, n = 128, 4096
+    c = Cache(dev, 1, 1, hd, "int8", 64, n, 2, rng)
+    c.fill([n, n])
+    q = rng.standard_normal((M, hd)).astype(np.float16)
+    qt, zero = Tensor(q, device=dev), ints(dev, [0])
+    k, v = (Tensor.zeros((n, hd), "float16", dev) for _ in range(2))
+    slots = [ints(dev, [0]), ints(dev, [1])]
+    outs = [Tensor.empty((M, n), "float16", dev) for _ in range(8)]
+    dev.synchronize()
+    for i, out in enumerate(outs):
+        c.kv.read(0, zero, seq=slots[i & 1], max_count=n, k=k, v=v)
+        dev.call("jg_linear", out.ptr, qt.ptr, k.ptr, 0, 0, M, n, hd)
+    for i, out in enumerate(outs):
+        held = c.k[i & 1, :, 0].astype(np.float64)
+        want, size = q.astype(np.float64) @ held.T, np.abs(q.astype(np.float64)) @ np.abs(held).T
+        # rounded to fp16 once, behind a sum of 128 exact products in 32 bits
+        assert (np.abs(out.numpy() - want) <= 2.0 ** -11 * np.abs(want) + 2.0 ** -25 + hd * 2.0 ** -23 * size).all(), i
+    c.close()
