@@ -652,7 +652,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       int head, i;
       const long long row = row_of(p, head, i), to = row < 0 ? -1 : row * a.ldo + head * HD;
       const bool outside = p.bt == nullptr || (long long)p.p0 + i < 0 || (long long)p.p0 + i >= a.c.max_ctx;
-      // 32 columns from c on of the warp's rows, as halves in the place of its queries (whose products are done)
+      // 32 columns from c on of the warp's rows, as halves in the place of its queries (whose products are done).  Zeros where there is nothing to see;
+      // where all scores are -inf (an infinite query) the sum is 0 and the row NaN, as a softmax is.
       auto gather = [&](int c, const float* o, float f) {
 #pragma unroll
         for (int k = 0; k < 32; k += 8) {
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       };
       const int at = q * 128 + r;
       if (ok && !idle && !absent) {
-        const float f = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+        const float f = __fdiv_rn(1.f, sum);
 #pragma unroll 1
         for (int c = 0; c < HD; c += 32) {
           float o[32];
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       sum = 0.f;
 #pragma unroll 4
       for (int k = 0; k < p.pieces; k++) sum = fmaf(__ldcg(piece(k) + HD * KC_ROWS + KC_ROWS + at), ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base), sum);
-      const float f = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+      const float f = __fdiv_rn(1.f, sum);
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         const long long row = (long long)(a.first ? a.first[p.b] : p.b) + (long long)i * a.step;
         if (row < 0 || row >= a.R) continue;
         const bool outside = p.bt == nullptr || (long long)p.p0 + i < 0 || (long long)p.p0 + i >= a.c.max_ctx;
-        const float f = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+        const float f = __fdiv_rn(1.f, sum);
         uint32_t w[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) {

@@ -411,7 +411,8 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         const int col = idx / HD, i = col / a.n_rep;
         const long long row = row0 + (long long)i * a.step;
         if (col >= n_cols || row < 0 || row >= a.R) return;
-        const bool outside = !NEW && (bt == nullptr || (long long)p0 + i >= a.limit || (long long)p0 + i < 0);
+        // zeros where there is nothing to see; where all scores are -inf (an infinite query) the sum is 0 and the row NaN, as a softmax is
+        const bool outside = bt == nullptr || (!NEW && ((long long)p0 + i >= a.limit || (long long)p0 + i < 0));
         const __half2 h0 = __floats2half2_rn(outside ? 0.f : x[0], outside ? 0.f : x[1]), h1 = __floats2half2_rn(outside ? 0.f : x[2], outside ? 0.f : x[3]);
         *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)(g * a.n_rep + col % a.n_rep) * HD + idx % HD) = make_uint2(ks_half2(h0), ks_half2(h1));
       };
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
           x[0] = fmaf(y0.x, f, x[0]); x[1] = fmaf(y0.y, f, x[1]); x[2] = fmaf(y1.x, f, x[2]); x[3] = fmaf(y1.y, f, x[3]);
         }
         if (whole) {
-          const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+          const float inv = __fdiv_rn(1.f, sum);
           x[0] *= inv; x[1] *= inv; x[2] *= inv; x[3] *= inv;
           store(idx, x);
         } else {
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
       add_up(0, pieces, group.step);
 #pragma unroll
       for (int e = 0; e < NI; e++) {
-        const float inv = sum[e] == 0.f ? 0.f : __fdiv_rn(1.f, sum[e]);
+        const float inv = __fdiv_rn(1.f, sum[e]);
         x[e][0] *= inv; x[e][1] *= inv; x[e][2] *= inv; x[e][3] *= inv;
         store((tid + e * KS_THREADS) * 4, x[e]);
       }
