@@ -38,6 +38,8 @@ struct jg_dev {
   uint64_t fresh_lo[16], fresh_hi[16];
   unsigned fresh_n;
 };
+// Who gave up, in the error word: 1 to 5 are the tensor-core projections' and the single-kernel step's, these the chunk kernel's of the 8-bit KV cache.
+enum { JG_WAIT_KVQ_PLAN = 6, JG_WAIT_KVQ_CODES, JG_WAIT_KVQ_PRODUCTS, JG_WAIT_KVQ_SOFTMAX, JG_WAIT_KVQ_PIECES };
 int jg_check_device_errors(jg_dev* dev);  // after a stream synchronise: JG_ETIMEDOUT if a bounded wait gave up
 
 struct jg_graph {

@@ -122,8 +122,9 @@ int jg_check_device_errors(jg_dev* dev) {
     jg_pair_reset(dev);
     if (dev->kvq_tickets) cudaMemsetAsync(dev->kvq_tickets, 0, jg_kvq_ticket_bytes(dev), dev->stream);
     jg_set_error("a device-side wait gave up (code %d: 1 = TMA producer, 2 = MMA issuer, 3 = epilogue of a tensor-core "
-                 "projection, 4 = grid barrier of the single-kernel decode step); results since the last synchronisation "
-                 "are invalid", code);
+                 "projection, 4 = grid barrier of the single-kernel decode step, 5 = a bulk copy of it; chunks over the 8-bit KV cache: "
+                 "%d = plan, %d = codes, %d = products, %d = softmax, %d = pieces of other CTAs); results since the last synchronisation "
+                 "are invalid", code, JG_WAIT_KVQ_PLAN, JG_WAIT_KVQ_CODES, JG_WAIT_KVQ_PRODUCTS, JG_WAIT_KVQ_SOFTMAX, JG_WAIT_KVQ_PIECES);
     return JG_ETIMEDOUT;
   }
   return JG_OK;

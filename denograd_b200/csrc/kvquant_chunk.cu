@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         if (lane == 0) { s_plan[slot] = p; ft_arrive(&plan_full[slot]); }
         if (p.b < 0) break;
       }
-      if (!ok && lane == 0) atomicCAS(a.err, 0, 1);
+      if (!ok && lane == 0) atomicCAS(a.err, 0, JG_WAIT_KVQ_PLAN);
     } else if (warp == 16) {
       // ---- products
       constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(KC_KEYS >> 3) << 17) | (8u << 24);
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           if (more) commit(&k_empty[then]);
         }
       }
-      if (!ok && lane == 0) atomicCAS(a.err, 0, 2);
+      if (!ok && lane == 0) atomicCAS(a.err, 0, JG_WAIT_KVQ_PRODUCTS);
     }
   } else if (warp >= 8) {
     // ---- keys, or values: codes to halves, into 128-byte swizzled rows
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         page2 = page_of(j + 3);
       }
     }
-    if (!ok && lane == 0) atomicCAS(a.err, 0, 1);
+    if (!ok && lane == 0) atomicCAS(a.err, 0, JG_WAIT_KVQ_CODES);
   } else {
     // ---- softmax: a thread for each row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KC_SOFT_REGS));
@@ -758,6 +758,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       const KcPiece& p = s_shared[k];
       unsigned int *arrived = a.tickets + kc_ticket(p.c_lo), *done = a.tickets + kc_done_ticket(gridDim.x, p.c_lo);
       ok = kc_arrived(arrived, (unsigned)p.pieces);
+      if (!ok && lane == 0) atomicCAS(a.err, 0, JG_WAIT_KVQ_PIECES);
       meet();
       if (!ok) break;
       if (tid == 0 && atomicAdd(done, 1u) == (unsigned)(p.pieces - 1)) { *arrived = 0; *done = 0; }
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         to[1] = make_uint4(w[4], w[5], w[6], w[7]);
       }
     }
-    if (!ok && lane == 0) atomicCAS(a.err, 0, 3);
+    if (!ok && lane == 0) atomicCAS(a.err, 0, JG_WAIT_KVQ_SOFTMAX);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();

@@ -2,6 +2,7 @@
 launches nothing and writes down what it was asked for."""
 import ctypes as C
 import os
+import re
 import subprocess
 
 import pytest
@@ -11,7 +12,8 @@ from denograd_b200 import ffi
 from tests.test_kvquant_cpu import CALLS, HOOKS, LAUNCHES, desc
 from tests.util import ROOT
 
-FRESH = """
+MORE_HOOKS = """
+extern "C" __attribute__((visibility("default"))) void fake_give_up(jg_dev* dev, int code) { *dev->err_word = code; }
 extern "C" __attribute__((visibility("default"))) int fake_is_fresh(jg_dev* dev, uint64_t p) { return jg_is_fresh(dev, (const void*)p); }
 """
 ATTRIBUTES = """
@@ -34,7 +36,7 @@ cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t* c, const void*, void**
 @pytest.fixture(scope="module")
 def lib(tmp_path_factory):
     d = tmp_path_factory.mktemp("fake")
-    (d / "hooks.cu").write_text(HOOKS + FRESH)
+    (d / "hooks.cu").write_text(HOOKS + MORE_HOOKS)
     plain = "cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t*, const void*, void**) { fake_launches++; return cudaSuccess; }\n"
     head, rest = LAUNCHES.split(plain)
     counter = head.split('extern "C" {\n')[1]
@@ -49,6 +51,7 @@ def lib(tmp_path_factory):
             getattr(lib, name).argtypes = args
     lib.jg_last_error.restype = C.c_char_p
     lib.fake_is_fresh.argtypes = [C.c_void_p, C.c_uint64]
+    lib.fake_give_up.argtypes = [C.c_void_p, C.c_int]
     return lib
 
 
@@ -104,3 +107,18 @@ def test_what_is_written_is_no_weight_to_read_early(lib, dev, kv, name, args, wr
     assert not lib.fake_is_fresh(dev, 1 << 28) and not lib.fake_is_fresh(dev, CALLS[name][0]["pos"])
     assert lib.jg_device_sync(dev) == 0
     assert not any(lib.fake_is_fresh(dev, args[what]) for what, _ in written)
+
+
+def test_a_wait_that_gave_up_is_named(lib, dev, kv):
+    """Its own codes for the kernel of chunks, in the message as they are in the kernel."""
+    with open(os.path.join(B.CSRC, "kvquant_chunk.cu")) as f:
+        used = set(re.findall(r"atomicCAS\(a\.err, 0, (\w+)\)", f.read()))
+    names = ["JG_WAIT_KVQ_PLAN", "JG_WAIT_KVQ_CODES", "JG_WAIT_KVQ_PRODUCTS", "JG_WAIT_KVQ_SOFTMAX", "JG_WAIT_KVQ_PIECES"]
+    assert used == set(names)
+    for code, what in zip(range(6, 11), ("plan", "codes", "products", "softmax", "pieces of other CTAs")):
+        assert lib.jg_kvq_attn(dev, kv, *dict(CALLS["attn"][0], max_count=60).values()) == 0
+        lib.fake_give_up(dev, code)
+        assert lib.jg_device_sync(dev) == ffi.JG_ETIMEDOUT
+        message = lib.jg_last_error().decode()
+        assert f"code {code}:" in message and f"{code} = {what}" in message and "8-bit KV cache" in message
+        assert lib.jg_device_sync(dev) == 0
