@@ -122,3 +122,9 @@ def test_a_wait_that_gave_up_is_named(lib, dev, kv):
         message = lib.jg_last_error().decode()
         assert f"code {code}:" in message and f"{code} = {what}" in message and "8-bit KV cache" in message
         assert lib.jg_device_sync(dev) == 0
+
+
+def test_bytes_are_those_of_codes_scales_and_table(lib, kv):
+    n = C.c_uint64()
+    assert lib.jg_kvq_bytes(kv, C.byref(n)) == 0
+    assert n.value == 2 * 12 * 16 * 2 * (2 * 64 + 4) + 3 * 4 * 4  # layers, pages, positions, kv heads; without the workspace

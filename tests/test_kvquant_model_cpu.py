@@ -1,0 +1,52 @@
+"""Llama models with an 8-bit KV cache under tensor parallelism, without a GPU: which calls each rank makes."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from denograd_b200 import ffi
+from tests.golden.gen_golden import TINY
+from tests.test_kvquant_cpu import KvqRecorder
+
+
+class Descs(KvqRecorder):
+    descs: list = []
+
+    def call(self, name, *args):
+        if name == "jg_kvq_create":
+            d = args[1]._obj
+            Descs.descs.append({f: getattr(d, f) for f, _ in ffi.KvDesc._fields_})
+        super().call(name, *args)
+
+
+@pytest.mark.parametrize("kv_dtype", ["int8", "fp8"])
+@pytest.mark.parametrize("rank", [0, 1])
+def test_a_rank_of_two(monkeypatch, kv_dtype, rank):
+    """Each rank has the cache of its own heads; everything else is what the fp16 cache's model calls."""
+    from tests import fake_ffi
+    monkeypatch.setattr(fake_ffi, "Recorder", Descs)
+    monkeypatch.setattr(Descs, "descs", [])
+    with fake_ffi.recording() as rec:
+        from denograd_b200.device import Device
+        from denograd_b200.llama3 import Llama3
+        from denograd_b200.multi import TensorParallel
+        tp = TensorParallel.__new__(TensorParallel)
+        tp.dev, tp.rank, tp.world, tp.handle = Device["CUDA"], rank, 2, C.c_void_p(0x77)
+        tp.peer_capacity = tp.twoshot_capacity = tp._partial_ptr = 0
+        made = {}
+        for kv in ("float16", kv_dtype):
+            llm = Llama3(size="1B", args=TINY, kv_dtype=kv, max_context=64, max_batch=3, tied_output=True, temperature=0, tp=tp)
+            n = len(rec.calls)
+            llm.model._step(llm.model._workspace(3))
+            llm.model._forward_rows(np.zeros((2, 12), np.int32), 3, last=True)
+            made[kv] = rec.kernels(n)
+            llm.model.new_cache()
+        d = Descs.descs[0]
+        assert len(Descs.descs) == 2 and (d["n_heads"], d["n_kv_heads"], d["head_dim"], d["n_layers"], d["max_batch"]) == (2, 1, 64, 2, 3)
+        decode, write, attend = ([c for c in made[kv_dtype] if c[0] == "jg_kvq_" + x] for x in ("decode", "write", "attn"))
+        assert len(decode) == len(write) == len(attend) == TINY["n_layers"]
+        assert all(c[-1] == 2 for c in decode + write + attend)  # this rank's query heads
+        assert all(c[-2] == 3 for c in decode) and all(c[-2] == 24 for c in write) and all(c[-4:-1] == (2, 12, 2) for c in attend)
+        attention = ("jg_kvq_", "jg_attn", "jg_rope")
+        assert [c[0] for c in made[kv_dtype] if not c[0].startswith(attention)] == [c[0] for c in made["float16"] if not c[0].startswith(attention)]
+        del llm, tp

@@ -74,3 +74,28 @@ def test_a_new_query_that_is_not_finite(dev, n):
     c.kv.decode(0, Tensor(y, device=dev), ints(dev, [c.n, -1, 2 ** 31 - 1]), out=out)
     assert not out.numpy().any()  # outside the cache
     c.close()
+
+
+@pytest.mark.parametrize("kv_dtype", ["int8", "fp8"])
+def test_a_rank_by_itself(dev, kv_dtype):
+    """A model under tensor parallelism, of one rank: the cache holds what the plain model's does, to the bit, behind the same tokens."""
+    from denograd_b200 import synth
+    from denograd_b200.llama3 import Llama3
+    from denograd_b200.multi import TensorParallel
+    from tests.golden.gen_golden import TINY
+    toks = synth.prompt_tokens(20, TINY["vocab_size"], batch=2, seed=3)
+    tp = TensorParallel(dev, 0, 1, TensorParallel.unique_id())
+    ids, held = [], []
+    for rank in (None, tp):
+        llm = Llama3(size="1B", args=TINY, kv_dtype=kv_dtype, max_context=64, max_batch=2, tied_output=True, temperature=0, tp=rank).load_synthetic()
+        m = llm.model
+        ids.append(llm.generate(toks, 8, batched=True))
+        held.append(m._kv.read(0, ints(dev, [0, 0]), max_count=20, step=2, rows=40)[0].numpy())  # the first layer's: no sum between ranks is in it yet
+        dev.synchronize()
+        m._forward_jit.clear()
+        m._loop_graph.clear()
+        del llm, m
+    dev.synchronize()
+    tp.close()
+    assert (ids[0] == ids[1]).all() and held[0].any()
+    np.testing.assert_array_equal(held[0].view(np.uint16), held[1].view(np.uint16))
