@@ -87,6 +87,8 @@ class QuantKVCache:
         seq[r] (None: slot r).  Rotated Q goes to `q_out`, which may be `qkv`.  The rows name different positions."""
         x, ldx, R = _rows(self.dev, "qkv", qkv, self._qkv)
         to, ldq, _ = _rows(self.dev, "q_out", q_out, self._q, R) if q_out is not None else (0, 0, 0)
+        if to == x and ldq != ldx and R > 1:  # its rows would be written over those of qkv that are still to be read
+            raise ValueError(f"q_out is qkv, with rows of {ldq} and not {ldx}")
         table, n = self._table(freqs_cis)
         self.dev.call("jg_kvq_write", self.handle, layer, to, ldq, x, ldx, table, n, _ints(self.dev, "pos", pos, R), _ints(self.dev, "seq", seq, R), R, self.n_heads)
 

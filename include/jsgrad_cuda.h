@@ -310,7 +310,7 @@ int jg_kvq_set_block_table(jg_kvq* kv, const int32_t* table); /* as jg_kvcache_s
 int jg_kvq_bytes(jg_kvq* kv, uint64_t* out); /* codes, scales and block table; the first cache of a device also makes a workspace for all (39 MB) */
 /* apply_rotary_emb on Q and K + cache assignment (jsgrad/models/llama.ts:23-32,87) for R independent rows: row r of qkv, wq|wk|wv outputs
  * [(H + 2G) * hd], has position pos[r] of slot seq[r] (0: row r is slot r).  Q and K are rotated in 32 bits and rounded to fp16 once;
- * rotated Q goes to q_out (0: nowhere; qkv itself: in place), K and V into the cache.  table = 0: nothing is rotated.
+ * rotated Q goes to q_out (0: nowhere; qkv itself with ldq = ldx: in place), K and V into the cache.  table = 0: nothing is rotated.
  * A row whose slot or position lies outside the cache or the table is skipped. */
 int jg_kvq_write(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t q_out, int32_t ldq, uint64_t qkv, int32_t ldx, uint64_t table,
                  int32_t table_rows, uint64_t pos, uint64_t seq, int32_t R, int32_t H);

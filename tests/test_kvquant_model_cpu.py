@@ -1,4 +1,4 @@
-"""Llama models with an 8-bit KV cache under tensor parallelism, without a GPU: which calls each rank makes."""
+"""Llama models with an 8-bit KV cache under tensor parallelism, without a GPU: which calls each rank makes.  And what `write` refuses of its output."""
 import ctypes as C
 
 import numpy as np
@@ -50,3 +50,21 @@ def test_a_rank_of_two(monkeypatch, kv_dtype, rank):
         attention = ("jg_kvq_", "jg_attn", "jg_rope")
         assert [c[0] for c in made[kv_dtype] if not c[0].startswith(attention)] == [c[0] for c in made["float16"] if not c[0].startswith(attention)]
         del llm, tp
+
+
+def test_rotated_queries_in_place_have_the_same_rows(monkeypatch):
+    from tests import fake_ffi
+    monkeypatch.setattr(fake_ffi, "Recorder", KvqRecorder)
+    with fake_ffi.recording() as rec:
+        from denograd_b200.device import Device, Tensor
+        from denograd_b200.kvquant import QuantKVCache
+        kv = QuantKVCache(Device["CUDA"], 1, 8, 2, 64, 100, 3, page_size=16)
+        x, pos = Tensor.empty((3, 768), "float16"), Tensor.empty((3,), "int32")
+        kv.write(0, x, pos, q_out=x)
+        n = len(rec.calls)
+        with pytest.raises(ValueError, match="rows of 512 and not 768"):  # row 1 of the result would lie in row 0's K
+            kv.write(0, x, pos, q_out=Tensor(x.buf, shape=(4, 512)))
+        assert len(rec.calls) == n
+        one = x.view_rows(0, 1)
+        kv.write(0, one, pos, q_out=Tensor(one.buf, shape=(1, 512)))  # a row by itself has no other
+        del kv
