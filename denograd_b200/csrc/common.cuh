@@ -193,6 +193,11 @@ __device__ __forceinline__ uint4 ld_stream_128(const void* p) {
 // 128-bit cached load (activations, KV rows: L1/L2 resident or reused)
 __device__ __forceinline__ uint4 ld_128(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
+__device__ __forceinline__ float ex2(float x) {  // 2^x by the hardware's approximation (2^-22 relative), 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float2 h2_to_f2(uint32_t u) {
   __half2 h = *reinterpret_cast<__half2*>(&u);
   return __half22float2(h);

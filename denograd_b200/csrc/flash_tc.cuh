@@ -39,11 +39,6 @@ __device__ __forceinline__ uint32_t ft_columns(uint32_t* s_tmem, bool taker) {
   return tmem;
 }
 __device__ __forceinline__ void ft_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
-__device__ __forceinline__ float ft_ex2(float x) {  // 2^x by the hardware's approximation (2^-22 relative), 0 for -inf
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
   uint32_t r[32];
   asm volatile(
@@ -280,15 +275,15 @@ __device__ __forceinline__ void flash_tc(P& p, int* err) {
 #pragma unroll
       for (int c = 0; c < FT_KV; c += 4) { t0 = fmaxf(t0, v[c]); t1 = fmaxf(t1, v[c + 1]); t2 = fmaxf(t2, v[c + 2]); t3 = fmaxf(t3, v[c + 3]); }
       const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), base = top == -INFINITY ? 0.f : top * sc;
-      l *= ft_ex2(m == -INFINITY ? -INFINITY : m * sc - base);
+      l *= ex2(m == -INFINITY ? -INFINITY : m * sc - base);
       m = top;
       float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
 #pragma unroll
       for (int c = 0; c < FT_KV; c += 4) {
-        a0 += ft_ex2(fmaf(v[c], sc, -base));
-        a1 += ft_ex2(fmaf(v[c + 1], sc, -base));
-        a2 += ft_ex2(fmaf(v[c + 2], sc, -base));
-        a3 += ft_ex2(fmaf(v[c + 3], sc, -base));
+        a0 += ex2(fmaf(v[c], sc, -base));
+        a1 += ex2(fmaf(v[c + 1], sc, -base));
+        a2 += ex2(fmaf(v[c + 2], sc, -base));
+        a3 += ex2(fmaf(v[c + 3], sc, -base));
       }
       l += (a0 + a1) + (a2 + a3);
     }
@@ -298,13 +293,13 @@ __device__ __forceinline__ void flash_tc(P& p, int* err) {
       s_l[q][r] = l;
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const float other = s_m[q ^ 1][r], both = fmaxf(base, other), zero = both == -INFINITY ? 0.f : both;
-      l = l * ft_ex2(base - zero) + s_l[q ^ 1][r] * ft_ex2(other - zero);
+      l = l * ex2(base - zero) + s_l[q ^ 1][r] * ex2(other - zero);
       base = both;
     }
     const float ex = p.extra2();
     if (ex != -INFINITY) {  // an entry that takes weight and has no value
       const float both = fmaxf(base, ex);
-      l = l * ft_ex2(base - both) + ft_ex2(ex - both);
+      l = l * ex2(base - both) + ex2(ex - both);
       base = both;
     }
     if (base == -INFINITY) base = 0.f;
@@ -319,7 +314,7 @@ __device__ __forceinline__ void flash_tc(P& p, int* err) {
         uint32_t w[32];
 #pragma unroll
         for (int k = 0; k < 32; k++) {
-          const float x = ft_ex2(fmaf(v[c + 2 * k], sc, -base)) * rl, y = ft_ex2(fmaf(v[c + 2 * k + 1], sc, -base)) * rl;
+          const float x = ex2(fmaf(v[c + 2 * k], sc, -base)) * rl, y = ex2(fmaf(v[c + 2 * k + 1], sc, -base)) * rl;
           if (P::BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(y), "f"(x));
           else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k]) : "f"(y), "f"(x));
         }

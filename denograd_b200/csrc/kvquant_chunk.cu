@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           }
           const float top = kc_max64(v) * a.scale2;
           if (__any_sync(0xffffffffu, top > m + 8.f)) {
-            const float then = fmaxf(m, top), fade = then == m ? 1.f : ft_ex2(m - then);
+            const float then = fmaxf(m, top), fade = then == m ? 1.f : ex2(m - then);
             m = then;
             const uint64_t f2 = kc_pair(fade, fade);
             l0 = kc_fma2(l0, f2, kc_pair(0.f, 0.f));
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
 #pragma unroll
           for (int k = 0; k < 64; k += 4) {
             const float2 x = kc_split(kc_fma2(kc_pair(v[k], v[k + 1]), scale2, base2)), y = kc_split(kc_fma2(kc_pair(v[k + 2], v[k + 3]), scale2, base2));
-            const float x0 = ft_ex2(x.x), x1 = ft_ex2(x.y), y0 = ft_ex2(y.x), y1 = ft_ex2(y.y);
+            const float x0 = ex2(x.x), x1 = ex2(x.y), y0 = ex2(y.x), y1 = ex2(y.y);
             l0 = kc_add2(l0, kc_pair(x0, x1));
             l1 = kc_add2(l1, kc_pair(y0, y1));
             asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[k / 2]) : "f"(x1), "f"(x0));
@@ -629,8 +629,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
         if (q == 0) {
           const float2 o = *ml;
           const float then = fmaxf(m, o.x), base = then == -INFINITY ? 0.f : then;
-          own = ft_ex2(m - base);
-          others = ft_ex2(o.x - base);
+          own = ex2(m - base);
+          others = ex2(o.x - base);
           sum = sum * own + o.y * others;
           m = then;
         }
@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       const float base = top == -INFINITY ? 0.f : top;
       sum = 0.f;
 #pragma unroll 4
-      for (int k = 0; k < p.pieces; k++) sum = fmaf(__ldcg(piece(k) + HD * KC_ROWS + KC_ROWS + at), ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base), sum);
+      for (int k = 0; k < p.pieces; k++) sum = fmaf(__ldcg(piece(k) + HD * KC_ROWS + KC_ROWS + at), ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base), sum);
       const float f = __fdiv_rn(1.f, sum);
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
           float4 y[8];
 #pragma unroll
           for (int e = 0; e < 8; e++) y[e] = __ldcg(from + (size_t)e * KC_ROWS);
-          const float w = ft_ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base);
+          const float w = ex2(__ldcg(piece(k) + HD * KC_ROWS + at) - base);
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             o[4 * e] = fmaf(y[e].x, w, o[4 * e]); o[4 * e + 1] = fmaf(y[e].y, w, o[4 * e + 1]);
@@ -785,7 +785,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
 #pragma unroll
           for (int e = 0; e < KC_BATCH; e++) {
             if (from + e >= p.pieces) break;
-            const float then = fmaxf(top, pm[e]), base = then == -INFINITY ? 0.f : then, fade = ft_ex2(top - base), f = ft_ex2(pm[e] - base);
+            const float then = fmaxf(top, pm[e]), base = then == -INFINITY ? 0.f : then, fade = ex2(top - base), f = ex2(pm[e] - base);
             top = then;
             sum = sum * fade + pl[e] * f;
 #pragma unroll

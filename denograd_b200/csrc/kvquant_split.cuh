@@ -54,11 +54,6 @@ struct KsCfg {
 };
 
 #ifdef __CUDACC__
-__device__ __forceinline__ float ks_ex2(float x) {  // 2^x by the hardware's approximation (2^-22 relative), 0 for -inf
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void ks_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -344,7 +339,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
               top = fmaxf(top, m[nt][e]);
-              const float fade = top == m[nt][e] ? 1.f : ks_ex2(m[nt][e] - top);
+              const float fade = top == m[nt][e] ? 1.f : ex2(m[nt][e] - top);
               m[nt][e] = top;
               l[nt][e] *= fade;
 #pragma unroll
@@ -355,7 +350,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
           const float b0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
-          const float e0 = ks_ex2(s[nt][0] - b0), e1 = ks_ex2(s[nt][1] - b1), e2 = ks_ex2(s[nt][2] - b0), e3 = ks_ex2(s[nt][3] - b1);
+          const float e0 = ex2(s[nt][0] - b0), e1 = ex2(s[nt][1] - b1), e2 = ex2(s[nt][2] - b0), e3 = ex2(s[nt][3] - b1);
           l[nt][0] += e0 + e2;
           l[nt][1] += e1 + e3;
           w[nt][0] = ks_transpose(ks_half2(__floats2half2_rn(e0, e1)));
@@ -425,13 +420,13 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         float x[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < KS_WARPS; w++) {
-          const float f = ks_ex2(s_m[w][col] - base);
+          const float f = ex2(s_m[w][col] - base);
           const float4 y = *reinterpret_cast<const float4*>(so + (size_t)w * COLS * HD + idx);
           sum = fmaf(s_l[w][col], f, sum);
           x[0] = fmaf(y.x, f, x[0]); x[1] = fmaf(y.y, f, x[1]); x[2] = fmaf(y.z, f, x[2]); x[3] = fmaf(y.w, f, x[3]);
         }
         if (NEW && entry) {
-          const float f = ks_ex2(s_m[KS_WARPS][col] - base);
+          const float f = ex2(s_m[KS_WARPS][col] - base);
           const uint2 y = *reinterpret_cast<const uint2*>(&s_new[1][idx % HD]);
           const float2 y0 = h2_to_f2(y.x), y1 = h2_to_f2(y.y);
           sum += f;
@@ -489,7 +484,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
 #pragma unroll
             for (int e = 0; e < NI; e++) {
               if (p + k * step >= to) continue;
-              const float then = fmaxf(top[e], pm[k][e]), base = then == -INFINITY ? 0.f : then, fade = ks_ex2(top[e] - base), f = ks_ex2(pm[k][e] - base);
+              const float then = fmaxf(top[e], pm[k][e]), base = then == -INFINITY ? 0.f : then, fade = ex2(top[e] - base), f = ex2(pm[k][e] - base);
               top[e] = then;
               sum[e] = sum[e] * fade + pl[k][e] * f;
               x[e][0] = x[e][0] * fade + y[k][e].x * f;

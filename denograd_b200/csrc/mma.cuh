@@ -31,10 +31,5 @@ __device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint3
   hi = pack_bf16(x, y);
   lo = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
 }
-__device__ __forceinline__ float ex2(float x) {  // 2^x by the hardware's approximation (2^-22 relative), 0 for -inf
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 constexpr float LOG2E = 1.4426950408889634f;
 #endif
