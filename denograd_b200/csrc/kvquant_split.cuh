@@ -138,7 +138,6 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
     const int32_t* bt;
     const int T = sequence(b, p0, n_new, bt);
     const int n_units = max(1, (T + KS_UNIT - 1) / KS_UNIT), span = n_units + Cfg::FIXED;  // its units lie behind its fixed cost
-    const bool stored = NEW && bt != nullptr;  // there is a new token, at p0
     const long long row0 = NEW ? b : (a.first ? a.first[b] : b);
     const int n_cols = n_new * a.n_rep;
     for (int g = (int)((u - at) / span); g < a.c.G && u < u_hi; g++) {
@@ -147,6 +146,10 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
       u = min(item + span, u_hi);
       const int j1 = max(0, (int)(u - item) - Cfg::FIXED);
       if (j0 == j1) continue;
+      if (NEW && bt == nullptr) {  // a row outside the cache: nothing is stored, nothing seen
+        for (int x = tid * 4; x < a.n_rep * HD; x += KS_THREADS * 4) *reinterpret_cast<uint2*>(a.out + (size_t)b * a.ldo + (size_t)g * a.n_rep * HD + x) = make_uint2(0u, 0u);
+        continue;
+      }
       const int t_lo = j0 * KS_UNIT, t_hi = min(T, j1 * KS_UNIT);
       const int n_tiles = t_hi > t_lo + warp * 16 ? (t_hi - t_lo - warp * 16 + KS_UNIT - 1) / KS_UNIT : 0;  // of this warp
 
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
       Tile tile;
       // The new token is an entry of its own when the warps' sums meet, made by the CTA with the end of its sequence and stored on the way.  Its
       // last warp has a tile less than the others at most times.
-      const bool entry = stored && j1 == n_units, fresh = NEW && entry && warp == KS_WARPS - 1;
+      const bool entry = NEW && j1 == n_units, fresh = entry && warp == KS_WARPS - 1;
       uint4 kx, vx, kt;
       {
         uint4 x[NT][KJ][2], turn[KJ][2];
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
 #pragma unroll
           for (int j = 0; j < KJ; j++) { x[nt][j][0] = ld_128(q + j * 64); x[nt][j][1] = ld_128(q + j * 64 + 8); }
         }
-        const bool turned = NEW && a.table && stored;
+        const bool turned = NEW && a.table;
         if (turned)
 #pragma unroll
           for (int j = 0; j < KJ; j++) {
@@ -407,7 +410,7 @@ __global__ void __launch_bounds__(KS_THREADS, NT == 1 ? KS_CTAS : 2) kvq_split_k
         const long long row = row0 + (long long)i * a.step;
         if (col >= n_cols || row < 0 || row >= a.R) return;
         // zeros where there is nothing to see; where all scores are -inf (an infinite query) the sum is 0 and the row NaN, as a softmax is
-        const bool outside = bt == nullptr || (!NEW && ((long long)p0 + i >= a.limit || (long long)p0 + i < 0));
+        const bool outside = !NEW && (bt == nullptr || (long long)p0 + i >= a.limit || (long long)p0 + i < 0);
         const __half2 h0 = __floats2half2_rn(outside ? 0.f : x[0], outside ? 0.f : x[1]), h1 = __floats2half2_rn(outside ? 0.f : x[2], outside ? 0.f : x[3]);
         *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)(g * a.n_rep + col % a.n_rep) * HD + idx % HD) = make_uint2(ks_half2(h0), ks_half2(h1));
       };
