@@ -65,7 +65,8 @@ def main(argv=None) -> int:
     g.add_argument("--tokenizer", default="")
     g.add_argument("--max-new", type=int, default=32)
     g.add_argument("--max-context", type=int, default=0)
-    g.add_argument("--kv-dtype", default="float16", choices=["float16", "int8", "fp8"], help="element type of a Llama model's KV cache")
+    g.add_argument("--kv-dtype", default="float16", choices=["float16", "int8", "fp8"], help="element type of a Llama model's KV cache; 8 bits halve it, but a "
+                   "short conversation's tokens take longer than with float16 (8B: 3.37 ms each, 3.16)")
     g.add_argument("--seed", type=int, default=0)
     g.add_argument("--temperature", type=float, default=0.0)
     g.add_argument("--top-k", type=int, default=0)

@@ -44,9 +44,9 @@ JG_API int jg_kvq_attn(jg_dev* dev, jg_kvq* kv, int32_t layer, uint64_t out, int
   JG_REQUIRE(ldq >= H * hd && ldq % 8 == 0 && ldo >= H * hd && ldo % 8 == 0, "kvq_attn: rows of %d and %d elements are no multiple of 8 or too short", ldq, ldo);
   JG_REQUIRE(jg_aligned(out, 16) && jg_aligned(q, 16) && jg_aligned(pos, 4) && count % 4 == 0 && first % 4 == 0 && seq % 4 == 0, "kvq_attn: null or misaligned pointer");
   jg_mark_fresh(dev, out, (uint64_t)R * ldo * 2);
-  // Few columns are read at HBM's pace or near it: 8 sequences behind 3001 positions of the 8B, 16 columns 21.3 us (the tensor cores' form 38), 20
-  // columns 26.3 (38), 32 sequences of these 71 (93); 24 sequences behind 4000 of the 1B, 28 columns 54 (67).  A lane's outputs have to fit its
-  // registers: 32 columns of 128 values would take 42 us, against 38.
+  // Few columns are read at HBM's pace or near it: 8 sequences behind 3001 positions of the 8B, 16 columns 24.8 us (the tensor cores' form 37.7), 20
+  // columns 28.6 (37.7), 24 columns 28.7 (37.7), 32 sequences of 20 columns 71 (96); 24 sequences behind 4000 of the 1B, 28 columns 56 (75).  A lane's
+  // outputs have to fit its registers: 32 columns of 128 values would take 42 us, against 38.
   if ((long long)max_count * (H / G) <= (hd == 64 ? 32 : 24)) {
     KvqSplitArgs s = {};
     s.c = kvq_layer(kv, layer);

@@ -12,12 +12,15 @@
 // may pass by 2^8 before O is rescaled in tensor memory, which is rare behind the first tiles.
 //
 // The tiles of all items are one line, cut evenly over one CTA for each SM.  An item that several CTAs share meets in a workspace: two
-// pieces are added up by the last CTA to arrive (3 to 4 us), more by all of its CTAs, a share of the rows each; always in their order.
+// pieces are added up by the last CTA to arrive (3 to 4 us), more by all of its CTAs, a share of the rows each; always in their order.  These wait for
+// one another, so the launch is a cooperative one, which begins behind its predecessor: 2 us a call more than the times of the comparisons below,
+// which were taken with launches that begin early.
 //
 // What bounds it: per 256 rows x 128 keys x 128 columns four products of 512 cycles at the tensor peak, and 32768 exponentials at 16 a
-// cycle, 2048 cycles either way; such a unit takes 4000.  2048 positions of the 8B behind 6001, fp8: 230 us, 1.02 PFLOP/s.  The tensor pipe
+// cycle, 2048 cycles either way; such a unit takes 4000.  2048 positions of the 8B behind 6001, fp8: 239 us, 0.98 PFLOP/s, in
+// a short run, 265 us, 0.89 PFLOP/s, in a long one under the power limit (1.66 GHz).  The tensor pipe
 // and the exponentials' are each busy 47 % of the time, issue slots 45 %: the two softmax warps of a scheduler wait for tensor memory, their
-// maxima and votes, and fill each other's gaps only in part (without exponentials 200 us, without a softmax 171, without widening 212).
+// maxima and votes, and fill each other's gaps only in part (of 233 us: without exponentials 200, without a softmax 171, without widening 212).
 // Tried and slower: two threads to a row on 16 warps (290: registers), the widening on 16 warps (265), products of half a tile's keys, all 128
 // scores in registers, a share of the exponentials as polynomials; rows of 64 values with weights apart from the scores, so that the next
 // scores are made meanwhile (82.3 and 83.9 us for 24 ragged chunks of the 1B).

@@ -30,7 +30,7 @@ KVQ_LINE int kvq_slot(int cta, bool first) { return 2 * cta + (first ? 1 : 0); }
 // Few queries (kvquant_split.cuh): units of 64 positions; pieces that are added up ahead of the others, where there are many.
 constexpr int KS_WARPS = 4, KS_UNIT = 16 * KS_WARPS, KS_GROUP = 8, KS_BITS = 20;
 // Units that a (sequence, kv head) costs beside its own, by column groups.  One: 1, 3 and 6 within 1 %; more: 8 sequences of 5 positions behind 3001 of
-// the 8B 30.9 us with 3, 29.5 with 5, 29.8 with 7 (30 ragged ones 25.5, 25.3, 27.1).
+// the 8B, in L2, 30.9 us with 3, 29.5 with 5, 29.8 with 7 (30 ragged ones 25.5, 25.3, 27.1).
 constexpr int ks_fixed(int groups) { return groups == 1 ? 3 : 5; }
 // A piece's group: pieces from .. to - 1 of the item, added up first and counted at `ticket` (-1: there is none).  Not grouped: the piece itself.
 struct KsGroup {

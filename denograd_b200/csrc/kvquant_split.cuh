@@ -8,7 +8,7 @@
 // multiplies, 16 bytes at a time and a tile ahead, straight into registers (32 sequences of 4100 positions of the 8B, with a call that
 // reads the new rows back, 67 us; staged in shared memory 81).  V is multiplied by its scale as it is widened (exact), K's scale goes to
 // the finished scores.  The queries' fragments lie in shared memory, each lane's own, which leaves the registers to outputs and tiles (20
-// columns 26.3 us, 29.5 with them in registers; one column group 67.5, 68.2).
+// columns behind 8 x 3001 positions in L2 26.3 us, 29.5 with them in registers; from HBM 28.6.  One column group 67.5, 68.2).
 //
 // The running maximum is a reference that scores may pass by 2^6 before sums and outputs are rescaled: a vote a tile instead of three
 // rounds of shuffles.

@@ -54,7 +54,9 @@ class Llama3(Driver):
     args: dict = field(default_factory=dict)
     last_seen_toks: list = field(default_factory=list)
     tokenizer: object | None = None  # denograd_b200.tokenizer.Tokenizer, needed by _system / chat only
-    kv_dtype: str = "float16"  # of the KV cache: 'float16' | 'int8' | 'fp8' (kvquant.py)
+    # of the KV cache: 'float16' | 'int8' | 'fp8' (kvquant.py).  8 bits are for many or long conversations: one or two rows of fp16 weights take their steps
+    # as a single kernel with the fp16 cache only (8B, one row: 3.16 ms a token, 3.37 with 8 bits)
+    kv_dtype: str = "float16"
 
     def __post_init__(self):
         if self.quantize not in ("float16", "int8", "nf4", None):

@@ -297,7 +297,7 @@ int jg_attn_decode_noalloc(jg_dev* dev, uint64_t out, uint64_t qkv, uint64_t k_l
  *      paged pool with a code a value and a scale for each (position, kv head) of K and of V: 2 * head_dim + 4 bytes instead of
  *      4 * head_dim.  JG_KVQ_INT8: scale = max|x| / 127 rounded up to 4 significant bits, code = rint(x / scale).  JG_KVQ_E4M3: e4m3 codes
  *      with a power of two as the scale.  Either way code * scale is an fp16 number and attention multiplies those, exactly.
- *      A position whose K or V holds a NaN or an infinity makes NaN of every query that sees it, and of no other.
+ *      A position whose K or V holds a NaN or an infinity makes NaN of every query that sees it, and of no other; a query that holds one is NaN.
  *      The desc is jg_kvcache_create's (n_split is not used; 1 to 8 query heads per kv head).  Rows are fp16; ld* counts elements
  *      between rows, a multiple of 8; a row's columns behind the named ones are left alone.  Positions and slots come from device memory and
  *      are checked there: whatever lies outside the cache is not followed.  The rows of one call name different (slot, position)s. */
