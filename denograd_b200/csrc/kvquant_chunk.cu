@@ -709,21 +709,24 @@ __global__ void __launch_bounds__(KC_THREADS, 1) kvq_chunk_kernel(const KvqChunk
       // 1900, three: 28, 24; behind 16000, 18: 72, 41).
       const bool few = p.pieces <= KC_FEW;
       if (!few && tid == 0) s_shared[shared] = p;
-      __threadfence();
       meet();
       if (!few) {
-        if (tid == 0) atomicAdd(&a.tickets[kc_ticket(p.c_lo)], 1u);
+        if (tid == 0) {
+          __threadfence();  // all warps' pieces, which this thread knows of by their meeting, ahead of the count
+          atomicAdd(&a.tickets[kc_ticket(p.c_lo)], 1u);
+        }
         shared++;
         release();
         continue;
       }
       if (tid == 0) {
+        __threadfence();
         s_ticket = atomicAdd(&a.tickets[kc_ticket(p.c_lo)], 1u);
         if (s_ticket == (unsigned)(p.pieces - 1)) a.tickets[kc_ticket(p.c_lo)] = 0;
+        __threadfence();
       }
       meet();
       if (s_ticket != (unsigned)(p.pieces - 1) || idle || absent || !ok) { release(); continue; }
-      __threadfence();
       auto piece = [&](int k) -> const float* { return a.part + (size_t)kvq_slot(p.c_lo + k, k == 0) * kc_part_floats(HD); };
       float top = -INFINITY;
 #pragma unroll 4
