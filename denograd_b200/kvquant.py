@@ -150,7 +150,7 @@ class QuantKVCache:
         """(pos, count, first, seq, sequences, max_count, step) of a call."""
         B = pos.buf.size
         if max_count is None:
-            if B == 0 or R % B or count is not None or first is not None:
+            if R % B or count is not None or first is not None:
                 raise ValueError("max_count is needed where sequences have different numbers of rows")
             max_count = R // B
         if step is None:

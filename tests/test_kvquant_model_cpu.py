@@ -68,19 +68,3 @@ def test_rotated_queries_in_place_have_the_same_rows(monkeypatch):
         one = x.view_rows(0, 1)
         kv.write(0, one, pos, q_out=Tensor(one.buf, shape=(1, 512)))  # a row by itself has no other
         del kv
-
-
-def test_no_sequences(monkeypatch):
-    from tests import fake_ffi
-    monkeypatch.setattr(fake_ffi, "Recorder", KvqRecorder)
-    with fake_ffi.recording() as rec:
-        from denograd_b200.device import Device, Tensor
-        from denograd_b200.kvquant import QuantKVCache
-        kv = QuantKVCache(Device["CUDA"], 1, 8, 2, 64, 100, 3, page_size=16)
-        n = len(rec.calls)
-        with pytest.raises(ValueError, match="max_count"):
-            kv.attend(0, Tensor.empty((4, 512), "float16"), Tensor.empty((0,), "int32"), out=Tensor.empty((4, 512), "float16"))
-        with pytest.raises(ValueError, match="max_count"):
-            kv.read(0, Tensor.empty((0,), "int32"), rows=4)
-        assert not [c for c in rec.calls[n:] if c[0].startswith("jg_kvq_")]
-        del kv
